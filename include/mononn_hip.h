@@ -75,6 +75,12 @@ int mononn_module_summary(mononn_module* m, const char** text, size_t* len);
  *           parameter order, live-out bytes in root-tuple order, temp bytes.  Pass NULL to skip. */
 int mononn_module_buffer_info(const mononn_module* m, int* n_params, const int64_t** param_bytes,
                               int* n_liveouts, const int64_t** liveout_bytes, int64_t* temp_bytes);
+/* Live-outs that are updated in place: the results of the custom call mononn$kv_append live in the buffers of the entry
+ * parameters that hold its caches.  *parameter receives the number of that parameter, or -1 for a live-out with a buffer
+ * of its own.  The slot of an in-place live-out stays in the argument list of mononn_launch; its pointer is neither read
+ * nor written and may be NULL.
+ * No counterpart in the reference. */
+int mononn_module_liveout_parameter(const mononn_module* m, int index, int* parameter);
 /* grid / block / dynamic LDS of the launch (best_tuning_spec.json keys grid_dim, block_dim, smem_size;
  * README.md:199-200) and the number of grid-wide barriers in the kernel. */
 /* Whether the module brings its own temp arena (the caller would then pass NULL in the temp slot of

@@ -54,6 +54,7 @@ def _load_library() -> ctypes.CDLL:
     lib.mononn_module_code_object.argtypes = [c.c_void_p, P(c.c_void_p), P(c.c_size_t)]
     lib.mononn_module_buffer_info.argtypes = [c.c_void_p, P(c.c_int), P(P(c.c_int64)), P(c.c_int), P(P(c.c_int64)),
                                               P(c.c_int64)]
+    lib.mononn_module_liveout_parameter.argtypes = [c.c_void_p, c.c_int, P(c.c_int)]
     lib.mononn_module_launch_dims.argtypes = [c.c_void_p, P(c.c_int), P(c.c_int), P(c.c_int), P(c.c_int)]
     lib.mononn_module_regional_barriers.argtypes = [c.c_void_p, P(c.c_int)]
     lib.mononn_module_owns_temp.argtypes = [c.c_void_p]
@@ -82,7 +83,7 @@ _lib = _load_library()
 EXPORTED_SYMBOLS = [
     "mononn_last_error", "mononn_version", "mononn_compile", "mononn_tune", "mononn_compile_from_spec_dir",
     "mononn_module_destroy", "mononn_module_kernel_name", "mononn_module_spec_json", "mononn_module_source",
-    "mononn_module_code_object", "mononn_module_summary", "mononn_module_buffer_info", "mononn_module_launch_dims", "mononn_module_regional_barriers", "mononn_module_owns_temp",
+    "mononn_module_code_object", "mononn_module_summary", "mononn_module_buffer_info", "mononn_module_liveout_parameter", "mononn_module_launch_dims", "mononn_module_regional_barriers", "mononn_module_owns_temp",
     "mononn_module_num_constants", "mononn_module_constant_info", "mononn_module_set_constant", "mononn_module_load",
     "mononn_launch", "mononn_launch_static_temp", "mononn_static_temp_bytes", "mononn_module_synchronize", "mononn_module_global", "mononn_time_kernel", "mononn_module_stage_clock", "mononn_module_stage_name", "mononn_module_dump", "mononn_device_count", "mononn_device_info"]
 
@@ -182,6 +183,15 @@ class MonoNNModule:
                                               ctypes.byref(lp), ctypes.byref(temp)))
         return {"parameters": [pp[i] for i in range(npar.value)], "liveouts": [lp[i] for i in range(nlo.value)],
                 "temp": temp.value}
+
+    def liveout_parameters(self) -> List[int]:
+        """Per live-out: the entry parameter whose buffer it updates in place, or -1."""
+        out = []
+        for i in range(len(self.buffer_info()["liveouts"])):
+            p = ctypes.c_int()
+            _check(_lib.mononn_module_liveout_parameter(self._h, i, ctypes.byref(p)))
+            out.append(p.value)
+        return out
 
     def launch_dims(self) -> dict:
         g, b, s, nb = ctypes.c_int(), ctypes.c_int(), ctypes.c_int(), ctypes.c_int()
@@ -303,9 +313,10 @@ class MonoNNModule:
         self.launch_raw(self.buffer_pointers(), stream)
         self.synchronize(stream)
         outs = []
+        held = [b["liveouts"][i] if p < 0 else b["params"][p] for i, p in enumerate(self.liveout_parameters())]
         # bf16 results come back as their uint16 bit patterns (NumPy has no bfloat16; mononn_amd.bf16 converts)
         npdt = {"f16": np.float16, "bf16": np.uint16, "f32": np.float32, "s32": np.int32, "pred": np.bool_, "s64": np.int64, "u8": np.uint8, "s8": np.int8}
-        for t, o in zip(b["liveouts"], out_dtypes_dims):
+        for t, o in zip(held, out_dtypes_dims):
             outs.append(t.cpu().numpy().view(npdt[o["dtype"]]).reshape(o["dims"]).copy())
         return outs
 

@@ -166,6 +166,15 @@ int mononn_module_buffer_info(const mononn_module* m, int* n_params, const int64
   });
 }
 
+int mononn_module_liveout_parameter(const mononn_module* m, int index, int* parameter) {
+  return guarded([&] {
+    require(m != nullptr && parameter != nullptr, "NULL argument");
+    auto& lp = m->impl->hip_program().liveout_parameter;
+    require(index >= 0 && index < static_cast<int>(lp.size()), "live-out index out of range");
+    *parameter = lp[static_cast<size_t>(index)];
+  });
+}
+
 int mononn_module_owns_temp(const mononn_module* m) { return (m && m->impl->owns_temp()) ? 1 : 0; }
 
 int mononn_module_launch_dims(const mononn_module* m, int* grid, int* block, int* smem, int* barriers) {

@@ -122,6 +122,11 @@ GemmTuning default_gemm_tuning(const graph::GemmDesc& g, const LaunchShape& ls, 
 void validate_gemm_tuning(const graph::GemmDesc& g, const LaunchShape& ls, const GemmTuning& t, bool has_prologue = false);
 bool gemm_uses_mfma(const graph::GemmDesc& g);
 
+// one of the custom calls of hlo::OperatorConfig (device/mononn_operators.h); grid: workgroups of the launch
+NodeFunction generate_operator(const graph::Program& prog, const graph::Node& node, const LaunchShape& ls, int grid);
+// temp bytes of a paged attention's partial results
+int64_t paged_attention_part_bytes(const hlo::Instr* parts, int grid, int waves);
+
 // dry runs used by the merge passes
 bool can_merge_clusters(const graph::Program& prog, const std::vector<const hlo::Instr*>& producer,
                         const std::vector<const hlo::Instr*>& consumer,

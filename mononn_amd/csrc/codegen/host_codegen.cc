@@ -27,6 +27,10 @@ std::string generate_host_driver(const HipProgram& hp) {
   };
   list("kParamBytes", hp.param_bytes);
   list("kLiveoutBytes", hp.liveout_bytes);
+  // parameter whose buffer holds the live-out, or -1
+  s << "static const int kLiveoutParameter[] = {";
+  for (size_t i = 0; i < hp.liveout_parameter.size(); ++i) s << (i ? ", " : "") << hp.liveout_parameter[i];
+  s << (hp.liveout_parameter.empty() ? "-1" : "") << "};\n";
   s << "static const int kNumParams = " << hp.param_bytes.size() << ", kNumLiveouts = " << hp.liveout_bytes.size() << ";\n"
     << "static const size_t kTempBytes = " << hp.temp_bytes << ";\n"
     << "static const int kGrid = " << hp.grid << ", kBlock = " << hp.block << ", kSmem = " << hp.smem << ";\n"
@@ -132,7 +136,8 @@ int main(int argc, char** argv) {
 
   for (int i = 0; i < kNumLiveouts; ++i) {
     std::vector<char> out(kLiveoutBytes[i]);
-    CHECK(hipMemcpy(out.data(), bufs[kNumParams + i], out.size(), hipMemcpyDeviceToHost));
+    void* from = kLiveoutParameter[i] >= 0 ? bufs[kLiveoutParameter[i]] : bufs[kNumParams + i];
+    CHECK(hipMemcpy(out.data(), from, out.size(), hipMemcpyDeviceToHost));
     std::ofstream f("liveout_" + std::to_string(i) + ".bin", std::ios::binary);
     f.write(out.data(), static_cast<std::streamsize>(out.size()));
   }

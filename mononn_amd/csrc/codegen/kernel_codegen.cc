@@ -31,6 +31,8 @@ graph::BuildOptions build_options_from(const spec::GraphSpecification& s) {
   o.fold_layer_norm = s.hip.layer_norm_folding;
   o.pack_left_operands = s.hip.pack_left_operands;
   o.fuse_attention_out_proj = s.hip.attention_out_proj_fusion;
+  o.grid = s.runtime.grid_dim.x;
+  o.waves = s.runtime.block_dim.x / 64;
   o.reuse_temp_slots = s.hip.barrier != "flags_coherent";   // the fence-free barrier needs write-once addresses
   for (auto& kv : s.gemm_spec_list)
     if (kv.second.split_k > 1) o.gemm_split_k[kv.first] = kv.second.split_k;
@@ -356,7 +358,11 @@ HipProgram generate_program(const graph::Program& prog, spec::GraphSpecification
     hp.constants.push_back(ci);
   }
   for (auto* p : prog.parameters) hp.param_bytes.push_back(p->shape.byte_size());
-  for (auto* l : prog.live_outs) hp.liveout_bytes.push_back(l->shape.byte_size());
+  for (auto* l : prog.live_outs) {
+    hp.liveout_bytes.push_back(l->shape.byte_size());
+    auto ip = prog.in_place.find(l);
+    hp.liveout_parameter.push_back(ip == prog.in_place.end() ? -1 : static_cast<int>(ip->second->parameter_number));
+  }
   hp.temp_bytes = prog.temp_bytes;
 
   // node functions, de-duplicated by text
@@ -443,6 +449,8 @@ HipProgram generate_program(const graph::Program& prog, spec::GraphSpecification
       t.part = part;
       t.preload_b = spec.hip.operand_preload;
       f = generate_gemm(prog, n, ls, t);
+    } else if (n.kind == NodeKind::kOperator) {
+      f = generate_operator(prog, n, ls, hp.grid);
     } else {
       ClusterTuning t;
       if (n.has_reduce) {
@@ -514,7 +522,7 @@ HipProgram generate_program(const graph::Program& prog, spec::GraphSpecification
     }
     NodeReport rep;
     rep.name = n.name;
-    rep.kind = n.kind == NodeKind::kGemm ? "gemm" : n.kind == NodeKind::kAttention ? "attention" : (n.row_program ? "cluster_reduce" : "cluster_elewise");
+    rep.kind = n.kind == NodeKind::kGemm ? "gemm" : n.kind == NodeKind::kAttention ? "attention" : n.kind == NodeKind::kOperator ? "operator" : (n.row_program ? "cluster_reduce" : "cluster_elewise");
     rep.function = fn;
     rep.stage = n.stage;
     rep.units = f.num_units;
@@ -586,7 +594,11 @@ HipProgram generate_program(const graph::Program& prog, spec::GraphSpecification
   }
   if (any_regional) pre << "#define MONONN_REGIONAL_SYNC 1\n";
   pre << "#define MONONN_BARRIER_BUDGET_TICKS " << static_cast<long long>(spec.hip.barrier_timeout_ms) * 100000 << "ull   // wall clock: 100 MHz\n";
-  pre << "#include \"headers.h\"\n\n";
+  pre << "#include \"headers.h\"\n";
+  bool any_operator = false;
+  for (auto& n : prog.nodes) any_operator = any_operator || n.kind == NodeKind::kOperator;
+  if (any_operator) pre << "#include \"operators.h\"\n";
+  pre << "\n";
   for (auto& c : hp.constants) {
     std::ostringstream d;
     d << "__device__ __attribute__((aligned(256))) unsigned char " << c.symbol << "[" << std::max<int64_t>(c.device_bytes, 1) << "];";
@@ -793,6 +805,7 @@ HipProgram generate_program(const graph::Program& prog, spec::GraphSpecification
   hp.preamble = pre.str();
   hp.body = src.str();
   hp.files["headers.h"] = device::kPreludeText;
+  if (any_operator) hp.files["operators.h"] = device::kOperatorsText;
   hp.files["main.hip"] = hp.preamble + glob.str() + hp.body;
   hp.files["host_main.cpp"] = generate_host_driver(hp);
   return hp;

@@ -53,6 +53,7 @@ struct HipProgram {
   std::string preamble, body;
   std::vector<std::string> global_decls;
   std::vector<int64_t> param_bytes, liveout_bytes;
+  std::vector<int> liveout_parameter;   // entry parameter that a live-out updates in place (its own slot is not used), or -1
   int64_t temp_bytes = 0;
   std::vector<ConstantInfo> constants;
   std::vector<NodeReport> nodes;

@@ -1,0 +1,168 @@
+// Device functions of the operator nodes: a call of the matching template of device/mononn_operators.h with the shapes of
+// the custom call as its arguments.
+#include <algorithm>
+#include <cstdio>
+#include <sstream>
+
+#include "codegen/cluster_codegen.h"
+#include "common/status.h"
+
+namespace mononn {
+namespace codegen {
+
+using hlo::Instr;
+using hlo::OperatorConfig;
+
+namespace {
+
+std::string float_literal(double v) {
+  char buf[64];
+  std::snprintf(buf, sizeof buf, "%.9g", v);
+  std::string s = buf;
+  if (s.find_first_of(".en") == std::string::npos) s += ".0";
+  return s + "f";
+}
+
+// elements of one access: the largest power of two up to 16 bytes that divides all of `extents`
+int run_length(hlo::DType t, std::initializer_list<int64_t> extents) {
+  int v = 16 / hlo::dtype_bytes(t);
+  for (int64_t e : extents)
+    while (e % v != 0) v /= 2;
+  return v;
+}
+
+// Heads of a token that one thread takes with the sines it has computed: as many as leave every compute unit `resident`
+// threads, at most 8 (what the loads of one thread may hold in registers).
+int heads_per_thread(int64_t tokens, int64_t heads, int64_t pieces, int64_t resident) {
+  int64_t h = 1;
+  while (h < 8 && 2 * h <= heads && tokens * pieces * ((heads + 2 * h - 1) / (2 * h)) >= resident) h *= 2;
+  return static_cast<int>(h);
+}
+
+bool read_in_kernel(const graph::Program& prog, const Instr* root) {
+  for (auto& n : prog.nodes)
+    if (std::find(n.inputs.begin(), n.inputs.end(), root) != n.inputs.end()) return true;
+  return false;
+}
+
+}  // namespace
+
+int64_t paged_attention_part_bytes(const Instr* parts, int grid, int waves) {
+  const auto& q = parts->operands[0]->shape.dims;
+  const int64_t group = q[1] / parts->operands[1]->shape.dims[2];
+  const int64_t blocks = q[0] * group <= 32 ? 1 : waves;   // all sequences have at most 32 query rows
+  return 2 * int64_t(grid) * blocks * ((q[2] + 31) / 32 * 1024 + 64) * 4;
+}
+
+NodeFunction generate_operator(const graph::Program& prog, const graph::Node& node, const LaunchShape& ls, int grid) {
+  const Instr* ins = node.members[0];
+  const OperatorConfig& c = ins->oper;
+  NodeFunction f;
+  PointerTable ptrs;
+  std::ostringstream body;
+  std::vector<std::string> in;
+  // storage roots of the operands, as arguments in0 ..
+  auto input = [&](size_t i) { return ptrs.input(prog.storage_root(ins->operands[i]), ins->operands[i]->shape.dtype); };
+  auto dims = [&](size_t i) -> const std::vector<int64_t>& { return ins->operands[i]->shape.dims; };
+  auto ctype = [&](size_t i) { return std::string(hlo::dtype_ctype(ins->operands[i]->shape.dtype)); };
+  auto flag = [](bool b) { return b ? "true" : "false"; };
+  const int64_t block = ls.block_size, cus = 256;
+  auto check_units = [&](int64_t units) {
+    MONONN_CHECK(units >= 1 && units < (int64_t(1) << 31), kResourceExhausted) << node.name << " has too many work units";
+    f.num_units = units;
+  };
+
+  switch (c.kind) {
+    case OperatorConfig::kRope: {
+      const int64_t T = dims(0)[0], H = dims(0)[1], D = dims(0)[2], R = 2 * dims(2)[0];
+      const int vec = run_length(ins->shape.dtype, {R / 2, D, D - R});
+      const int64_t pieces = R / 2 / vec + (D - R) / vec;
+      const int heads = heads_per_thread(T, H, pieces, cus * block);
+      const std::string x = input(0), pos = input(1), freq = input(2), out = ptrs.output(ins);
+      body << "mononn_dev::rope_unit<" << ctype(0) << ", " << T << ", " << H << ", " << D << ", " << R << ", " << flag(c.interleaved) << ", " << vec << ", " << heads << ", "
+           << flag(read_in_kernel(prog, ins)) << ">(unit, " << x << ", " << pos << ", " << freq << ", " << out << ", " << float_literal(c.amplitude) << ");";
+      check_units((T * pieces * ((H + heads - 1) / heads) + block - 1) / block);
+      break;
+    }
+    case OperatorConfig::kKvAppend: {
+      const int64_t T = dims(0)[0], H = dims(0)[1], D = dims(0)[2], R = ins->operands.size() == 8 ? 2 * dims(7)[0] : 0;
+      const int vec = R > 0 ? run_length(ins->shape.tuple[0].dtype, {R / 2, D, D - R}) : run_length(ins->shape.tuple[0].dtype, {D});
+      const int64_t pieces = (R > 0 ? R / 2 / vec : 0) + (D - R) / vec;
+      // keys and values side by side: twice the registers of the rotation alone
+      const int heads = std::min(4, heads_per_thread(T, H, pieces, cus * block));
+      bool coherent = false;
+      for (auto* o : node.outputs) coherent = coherent || read_in_kernel(prog, o);
+      const std::string k = input(0), v = input(1);
+      // the caches are read by nothing else in the kernel, and written at their parameters' addresses
+      const std::string kc = ptrs.output(ins->operands[2]), vc = ptrs.output(ins->operands[3]);
+      const std::string table = input(4), qs = input(5), cl = input(6), freq = R > 0 ? input(7) : "nullptr";
+      body << "mononn_dev::kv_append_unit<" << ctype(0) << ", " << T << ", " << dims(4)[0] << ", " << H << ", " << D << ", " << R << ", " << flag(c.interleaved) << ", " << vec << ", " << heads
+           << ", " << dims(2)[1] << ", " << dims(2)[0] << ", " << dims(4)[1] << ", " << flag(coherent) << ">(unit, " << k << ", " << v << ", " << kc << ", " << vc << ", " << table << ", " << qs
+           << ", " << cl << ", " << freq << ", " << float_literal(c.amplitude) << ");";
+      check_units((T * pieces * ((H + heads - 1) / heads) + block - 1) / block);
+      break;
+    }
+    case OperatorConfig::kPagedAttentionParts:
+    case OperatorConfig::kPagedAttention: {
+      const bool parts_stage = c.kind == OperatorConfig::kPagedAttentionParts;
+      const Instr* parts = parts_stage ? ins : ins->operands[0];
+      const Instr* result = parts_stage ? nullptr : ins;
+      if (parts_stage)
+        for (auto* u : ins->users)
+          if (u->oper.kind == OperatorConfig::kPagedAttention) result = u;
+      MONONN_CHECK(result != nullptr && parts->oper.kind == OperatorConfig::kPagedAttentionParts, kInternal) << node.name << ": a paged attention without its other stage";
+      const auto &q = parts->operands[0]->shape.dims, &kc = parts->operands[1]->shape.dims, &table = parts->operands[3]->shape.dims;
+      body << "typedef mononn_dev::PagedAttention<" << hlo::dtype_ctype(result->shape.dtype) << ", " << q[0] << ", " << table[0] << ", " << q[1] << ", " << kc[2] << ", " << q[2] << ", " << kc[1]
+           << ", " << kc[0] << ", " << table[1] << ", " << c.window << ", " << grid << ", " << flag(read_in_kernel(prog, result)) << "> Attention; ";
+      if (parts_stage) {
+        const std::string qp = input(0), kp = input(1), vp = input(2), tp = input(3), sp = input(4), lp = input(5);
+        const std::string out = ptrs.output(result), pp = ptrs.output(ins);
+        body << "Attention::partial(unit, " << qp << ", " << kp << ", " << vp << ", " << tp << ", " << sp << ", " << lp << ", " << out << ", " << pp << ", " << float_literal(c.scale) << ", smem);";
+        const int64_t D = q[2], waves = ls.waves();
+        const int64_t kp_bytes = D * 2 + 16, vp_bytes = (D * 2 + 63) / 128 * 128 + 64, tiles = (D + 31) / 32;
+        // mirrors PagedAttention::lds_bytes
+        int64_t nn = waves;
+        while (nn > 1 && (nn * 32 * (kp_bytes + vp_bytes) > 160 * 1024 || nn * D * 128 + nn * 256 > 160 * 1024)) nn /= 2;
+        f.smem_bytes = static_cast<int>(std::max({2 * 64 * (kp_bytes + vp_bytes), nn * 32 * (kp_bytes + vp_bytes), nn * (tiles * 4096 + 256)}));
+        body << " static_assert(Attention::lds_bytes() == " << f.smem_bytes << ", \"LDS\");";
+      } else {
+        const std::string pp = input(0), sp = input(1), lp = input(2);
+        body << "Attention::join(unit, " << pp << ", " << sp << ", " << lp << ", " << ptrs.output(ins) << ");";
+      }
+      check_units(grid);
+      break;
+    }
+    case OperatorConfig::kMatvecW4: {
+      const int64_t M = dims(0)[0], K = dims(0)[1], N = dims(1)[0], group = K / dims(2)[1];
+      const bool zeros = ins->operands.size() == 4;
+      // Waves that share a tile of 16 weight rows by splitting the columns: the arrangement with the shortest longest
+      // wave over the whole launch, the fewest shares among equals.
+      const int64_t tiles = (N + 15) / 16, chunks = (K + 127) / 128, passes = (M + 63) / 64;
+      int64_t wk = 1, best = -1;
+      for (int64_t w = 1; w <= ls.waves(); w *= 2) {
+        if (ls.waves() % w != 0) break;
+        const int64_t units = (tiles + ls.waves() / w - 1) / (ls.waves() / w) * passes;
+        const int64_t longest = (units + grid - 1) / grid * ((chunks + w - 1) / w);
+        if (best < 0 || longest < best) best = longest, wk = w;
+      }
+      const int64_t mt = std::min<int64_t>((M + 15) / 16, 4), per = ls.waves() / wk;
+      const std::string x = input(0), w = input(1), s = input(2), z = zeros ? input(3) : "nullptr", out = ptrs.output(ins);
+      body << "mononn_dev::MatvecW4<" << ctype(0) << ", " << M << ", " << N << ", " << K << ", " << group << ", " << flag(zeros) << ", " << wk << ", " << flag(read_in_kernel(prog, ins))
+           << ">::unit(unit, " << x << ", " << w << ", " << s << ", " << z << ", " << out << ", smem);";
+      f.smem_bytes = wk > 1 ? static_cast<int>(ls.waves() * mt * 1024) : 0;
+      check_units((tiles + per - 1) / per * ((M + 16 * mt - 1) / (16 * mt)));
+      break;
+    }
+    default: MONONN_FAIL(kInternal) << node.name << " is not an operator";
+  }
+  std::ostringstream os;
+  os << "__device__ __forceinline__ void @NAME@(int unit";
+  for (auto& e : ptrs.entries) os << ", " << (e.is_output ? "" : "const ") << hlo::dtype_ctype(e.dtype) << "* " << e.name;
+  os << ", char* smem) {\n  " << body.str() << "\n}\n";
+  f.text = os.str();
+  f.pointers = ptrs.entries;
+  return f;
+}
+
+}  // namespace codegen
+}  // namespace mononn

@@ -1,0 +1,912 @@
+// Operators of a decoding step over a paged key / value cache (gfx950 / CDNA4, wave64): rotary positions, the append to
+// the cache, attention of new tokens over it, and products of a few rows with 4-bit weights.  Part of the generated
+// translation unit of modules that call them (custom calls `mononn$...`); each function is one unit of a stage of the
+// monolithic kernel.
+//
+// Run-time indices come from device memory and are never trusted: offsets of sequences are clamped to the token count,
+// lengths to what the page table can hold, page numbers to the pool (reads) or skipped (writes), so that every address
+// is in range whatever the data.
+#pragma once
+
+#ifndef MONONN_LDS_READ_TR16
+// 4 x 16 elements of 16 bits per group of 16 lanes: lane i gives the address of 4 elements, elements 4 (i % 4) .. of row
+// i / 4, and receives column i of the four rows
+typedef short mononn_short4 __attribute__((ext_vector_type(4)));
+#define MONONN_LDS_READ_TR16(p) __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) mononn_short4*)(p))
+#endif
+
+namespace mononn_dev {
+
+template <class T>
+struct IsBf16 { static constexpr bool value = false; };
+template <>
+struct IsBf16<__bf16> { static constexpr bool value = true; };
+
+// stores of a result: written through where a later stage of the kernel reads it, ordinary otherwise
+template <bool COHERENT, class T, int N>
+__device__ __forceinline__ void store_run(T* p, const T (&v)[N]) {
+  constexpr int BYTES = N * (int)sizeof(T);
+  if constexpr (BYTES == 2 || BYTES == 1) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if constexpr (COHERENT) st1(p + i, v[i]);
+      else st1_plain(p + i, v[i]);
+    }
+  } else {
+    if constexpr (COHERENT) stN<T, N>(p, v);
+    else stN_plain<T, N>(p, v);
+  }
+}
+template <class T, int N>
+__device__ __forceinline__ void load_run(const T* p, T (&v)[N]) {
+  struct alignas(N * sizeof(T)) Run { T e[N]; };
+  const Run r = *reinterpret_cast<const Run*>(p);
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = r.e[i];
+}
+
+__device__ __forceinline__ int clamp_int(int v, int lo, int hi) { return v < lo ? lo : (v > hi ? hi : v); }
+
+// ---------------------------------------------------------------------------------------------
+// rotary positions
+// ---------------------------------------------------------------------------------------------
+// Pair i of a head turns by position * inv_freq[i].  The angle is reduced to a fraction of a turn in 64 bits: at
+// position 10^6 a 32-bit angle is off by 0.03 rad.
+__device__ __forceinline__ void rotation_of(int position, float inv_freq, float amplitude, float& c, float& s) {
+  double turns = (double)position * (double)inv_freq * 0.15915494309189533577;
+  turns -= __builtin_rint(turns);
+  float sn, cs;
+  sincospif(2.0f * (float)turns, &sn, &cs);
+  c = cs * amplitude;
+  s = sn * amplitude;
+}
+
+// A head of D elements, the first R of them rotated, cut into pieces a thread handles: VEC pairs (two runs of VEC
+// elements) of the rotated part, or VEC elements that are copied.  Pairs are (i, i + R / 2), or (2 i, 2 i + 1) when
+// INTERLEAVED.
+template <class T, int D, int R, bool INTERLEAVED, int VEC>
+struct RotaryHead {
+  static constexpr int kTurned = R / 2 / VEC;
+  static constexpr int kPieces = kTurned + (D - R) / VEC;
+  static constexpr int kRuns = R > 0 ? 2 : 1;
+  float c[VEC], s[VEC];
+  int first, second;   // element offsets of the piece's runs; second < 0: a copied piece
+
+  __device__ __forceinline__ RotaryHead(int piece, int position, const float* inv_freq, float amplitude) {
+    if (piece < kTurned) {
+      first = INTERLEAVED ? 2 * piece * VEC : piece * VEC;
+      second = INTERLEAVED ? first + VEC : first + R / 2;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) rotation_of(position, inv_freq[piece * VEC + i], amplitude, c[i], s[i]);
+    } else {
+      first = R + (piece - kTurned) * VEC;
+      second = -1;
+    }
+  }
+  __device__ __forceinline__ bool turned() const { return second >= 0; }
+  __device__ __forceinline__ void load(const T* head, T (&x)[2][VEC]) const {
+    load_run<T, VEC>(head + first, x[0]);
+    if (turned()) load_run<T, VEC>(head + second, x[1]);
+  }
+  // rounded once, to the element type
+  __device__ __forceinline__ void turn(T (&x)[2][VEC]) const {
+    if (!turned()) return;
+    T y[2][VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      // element i of the two runs read as pair number: pair i is (run 0, run 1)[i], or consecutive elements
+      const float a = (float)(INTERLEAVED ? x[2 * i / VEC][2 * i % VEC] : x[0][i]);
+      const float b = (float)(INTERLEAVED ? x[(2 * i + 1) / VEC][(2 * i + 1) % VEC] : x[1][i]);
+      const T u = (T)(a * c[i] - b * s[i]), v = (T)(a * s[i] + b * c[i]);
+      if constexpr (INTERLEAVED) {
+        y[2 * i / VEC][2 * i % VEC] = u;
+        y[(2 * i + 1) / VEC][(2 * i + 1) % VEC] = v;
+      } else {
+        y[0][i] = u;
+        y[1][i] = v;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) x[0][i] = y[0][i], x[1][i] = y[1][i];
+  }
+  template <bool COHERENT>
+  __device__ __forceinline__ void store(T* head, const T (&x)[2][VEC]) const {
+    store_run<COHERENT, T, VEC>(head + first, x[0]);
+    if (turned()) store_run<COHERENT, T, VEC>(head + second, x[1]);
+  }
+};
+
+// y[t, h] = x[t, h] turned by positions[t].  A thread keeps the sines of one piece and takes HEADS heads of a token.
+template <class T, int TOKENS, int H, int D, int R, bool INTERLEAVED, int VEC, int HEADS, bool COHERENT>
+__device__ __forceinline__ void rope_unit(int unit, const T* x, const int* positions, const float* inv_freq, T* y, float amplitude) {
+  using Head = RotaryHead<T, D, R, INTERLEAVED, VEC>;
+  constexpr int STRIDE = (H + HEADS - 1) / HEADS;   // neighbouring threads take neighbouring heads
+  const long item = (long)unit * MONONN_BLOCK_SIZE + thread_id();
+  if (item >= (long)TOKENS * STRIDE * Head::kPieces) return;
+  const int piece = (int)(item % Head::kPieces), h0 = (int)(item / Head::kPieces % STRIDE), t = (int)(item / Head::kPieces / STRIDE);
+  T v[HEADS][2][VEC];
+  const T* row = x + (long)t * H * D;
+  const Head head(piece, positions[t], inv_freq, amplitude);
+#pragma unroll
+  for (int k = 0; k < HEADS; ++k)
+    if (h0 + k * STRIDE < H) head.load(row + (h0 + k * STRIDE) * D, v[k]);
+#pragma unroll
+  for (int k = 0; k < HEADS; ++k)
+    if (h0 + k * STRIDE < H) {
+      head.turn(v[k]);
+      head.template store<COHERENT>(y + ((long)t * H + h0 + k * STRIDE) * D, v[k]);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// sequences of a batch
+// ---------------------------------------------------------------------------------------------
+struct Sequence {
+  int start, len;   // its tokens among the call's tokens
+  int ctx;          // keys of the sequence, the new tokens among them
+};
+template <int TOKENS, int MAX_KEYS>
+__device__ __forceinline__ Sequence sequence_at(const int* query_start, const int* context_len, int b) {
+  Sequence s;
+  s.start = clamp_int(query_start[b], 0, TOKENS);
+  s.len = clamp_int(query_start[b + 1], s.start, TOKENS) - s.start;
+  s.ctx = clamp_int(context_len[b], 0, MAX_KEYS);
+  return s;
+}
+// the sequence that holds token t, or -1: the last b with query_start[b] <= t, if its tokens reach t
+template <int SEQS>
+__device__ __forceinline__ int sequence_of(const int* query_start, int t) {
+  int lo = 0, hi = SEQS;   // query_start[lo] <= t < query_start[hi], if at all
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (query_start[mid] <= t) lo = mid;
+    else hi = mid;
+  }
+  return query_start[lo] <= t && t < query_start[lo + 1] ? lo : -1;
+}
+
+// ---------------------------------------------------------------------------------------------
+// append to the paged cache
+// ---------------------------------------------------------------------------------------------
+// Token i of sequence b has position context_len[b] - new tokens + i and goes to row position % PAGE of page
+// page_table[b, position / PAGE]; the key is turned by its position on the way.  Positions outside the table and
+// pages outside the pool are left out.
+template <class T, int TOKENS, int SEQS, int H, int D, int R, bool INTERLEAVED, int VEC, int HEADS, int PAGE, int PAGES, int WIDTH, bool COHERENT>
+__device__ __forceinline__ void kv_append_unit(int unit, const T* k, const T* v, T* k_cache, T* v_cache, const int* page_table, const int* query_start, const int* context_len,
+                                               const float* inv_freq, float amplitude) {
+  using Head = RotaryHead<T, D, R, INTERLEAVED, VEC>;
+  constexpr int STRIDE = (H + HEADS - 1) / HEADS;
+  const long item = (long)unit * MONONN_BLOCK_SIZE + thread_id();
+  if (item >= (long)TOKENS * STRIDE * Head::kPieces) return;
+  const int piece = (int)(item % Head::kPieces), h0 = (int)(item / Head::kPieces % STRIDE), t = (int)(item / Head::kPieces / STRIDE);
+  const int b = sequence_of<SEQS>(query_start, t);
+  if (b < 0) return;
+  const Sequence s = sequence_at<TOKENS, WIDTH * PAGE>(query_start, context_len, b);
+  const int position = s.ctx - s.len + (t - s.start);
+  if (position < 0) return;   // position < WIDTH * PAGE follows from the clamped length
+  const int page = page_table[(long)b * WIDTH + position / PAGE];
+  if (page < 0 || page >= PAGES) return;
+  const long to = ((long)page * PAGE + position % PAGE) * H * D, from = (long)t * H * D;
+  const Head head(piece, position, inv_freq, amplitude);
+  T kx[HEADS][2][VEC], vx[HEADS][2][VEC];
+#pragma unroll
+  for (int i = 0; i < HEADS; ++i)
+    if (h0 + i * STRIDE < H) {
+      head.load(k + from + (h0 + i * STRIDE) * D, kx[i]);
+      head.load(v + from + (h0 + i * STRIDE) * D, vx[i]);
+    }
+#pragma unroll
+  for (int i = 0; i < HEADS; ++i)
+    if (h0 + i * STRIDE < H) {
+      head.turn(kx[i]);
+      head.template store<COHERENT>(k_cache + to + (h0 + i * STRIDE) * D, kx[i]);
+      head.template store<COHERENT>(v_cache + to + (h0 + i * STRIDE) * D, vx[i]);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// attention over the paged cache
+// ---------------------------------------------------------------------------------------------
+__device__ __forceinline__ float half_wave_other(float v) { return lane_xor(v, 32); }
+
+// The query rows of a sequence for one key / value head are its new tokens times the G = H / HKV query heads that
+// share it (row = token * G + head of the group), in tiles: ROWS = 32 per wave in a *wide* item, 32 in all in a
+// *narrow* one (a sequence with at most 32 rows: decoding).  An item (sequence, key head, tile) works through its
+// keys in steps: 64 keys that all waves share in a wide item, 32 keys per wave in a narrow one.
+//
+// The steps of all items, in order, are dealt to the workgroups in equal contiguous ranges, whatever the lengths of
+// the sequences: every workgroup reads the same number of keys.  Items that end inside a range are written out by it;
+// a range that begins or ends inside an item leaves the running maximum, sum and output of its part in memory, and
+// the next stage (`join`) adds those up: the range in which an item begins owns it.
+//
+// Per step, with S^T = K Q^T and O^T += V^T P^T on v_mfma_f32_32x32x16: queries lie along the lanes in both products, so
+// the maximum, the sum and the rescaling of a query stay in its lane (and the lane 32 further on), and the
+// probabilities leave the first product in the lanes that feed the second (a lane's 8 accumulator rows are the 8 keys
+// of one contraction step, in an order that the transposed reads of V follow).
+template <class T, int TOKENS, int SEQS, int H, int HKV, int D, int PAGE, int PAGES, int WIDTH, int WINDOW, int GRID, bool COHERENT>
+struct PagedAttention {
+  static constexpr int NW = MONONN_BLOCK_SIZE / kWaveSize;
+  static constexpr int G = H / HKV;
+  static constexpr int MAX_KEYS = WIDTH * PAGE;
+  static constexpr bool kBf16 = IsBf16<T>::value;
+  static constexpr int CPR = D / 8;              // 16-byte pieces of a row
+  static constexpr int DT = (D + 31) / 32;       // tiles of 32 output elements
+  static constexpr int QS = D / 16;              // contraction steps of the first product
+  // LDS rows: keys are read 16 bytes per lane down 32 rows (an odd number of 16-byte pieces spreads them over the
+  // banks), values 32 bytes of 4 rows per 16 lanes (a pitch of 64 modulo 128 bytes keeps the rows apart; it covers
+  // the last tile's 32 columns where D is not a multiple of 32)
+  static constexpr int KP = D * 2 + 16;
+  static constexpr int VP = (D * 2 + 63) / 128 * 128 + 64;
+  static_assert(VP >= D * 2 && VP >= DT * 64, "value rows");
+  static constexpr int kWideKeys = 64;
+  static constexpr int kWideBuffer = kWideKeys * (KP + VP);
+  static constexpr int kWaveBuffer = 32 * (KP + VP);
+  static constexpr int kLdsLimit = 160 * 1024;
+  static constexpr int narrow_waves(int n) { return n * kWaveBuffer <= kLdsLimit && n * D * 128 + n * 256 <= kLdsLimit ? n : narrow_waves(n / 2); }
+  static constexpr int NN = narrow_waves(NW);    // waves that take part in a narrow item
+  static constexpr int kNarrowKeys = 32 * NN;
+  static constexpr int kPartWave = DT * 1024 + 64;          // floats: output tiles as they lie in the registers, maxima, sums
+  static constexpr int kPart = (TOKENS * G <= 32 ? 1 : NW) * kPartWave;   // floats of one partial result; two per workgroup
+  static constexpr int kMergeBytes = NN * (DT * 4096 + 256);
+  static constexpr int lds_bytes() {
+    int n = 2 * kWideBuffer;
+    if (NN * kWaveBuffer > n) n = NN * kWaveBuffer;
+    return kMergeBytes > n ? kMergeBytes : n;
+  }
+
+  struct Item {
+    int b, h, tile;
+    Sequence s;
+    bool narrow;
+    int first, steps;   // first step (a multiple of the step's keys) and how many
+  };
+
+  static __device__ __forceinline__ bool is_narrow(int len) { return len * G <= 32; }
+  static __device__ __forceinline__ int tiles_of(int len) { return is_narrow(len) ? (len > 0 ? 1 : 0) : (len * G + 32 * NW - 1) / (32 * NW); }
+  // keys [lo, hi) that some row of the tile sees, as steps; at least one step, so that empty rows are written too
+  static __device__ __forceinline__ void tile_steps(const Sequence& s, int tile, int& first, int& steps) {
+    const bool narrow = is_narrow(s.len);
+    const int rows = narrow ? 32 : 32 * NW, keys = narrow ? kNarrowKeys : kWideKeys;
+    const int t0 = tile * rows / G;
+    int t1 = ((tile + 1) * rows - 1) / G;
+    if (t1 > s.len - 1) t1 = s.len - 1;
+    const int p0 = s.ctx - s.len + t0, p1 = s.ctx - s.len + t1;
+    const int lo = WINDOW > 0 && p0 - WINDOW + 1 > 0 ? p0 - WINDOW + 1 : 0;
+    const int hi = p1 + 1;   // <= ctx
+    first = lo / keys;
+    steps = hi > lo ? (hi + keys - 1) / keys - first : 0;
+    if (steps < 1) steps = 1;
+  }
+  static __device__ __forceinline__ int head_steps(const Sequence& s) {
+    int n = 0, f, k;
+    const int tiles = tiles_of(s.len);
+    for (int i = 0; i < tiles; ++i) {
+      tile_steps(s, i, f, k);
+      n += k;
+    }
+    return n;
+  }
+  static __device__ __forceinline__ Sequence sequence(const int* qs, const int* cl, int b) { return sequence_at<TOKENS, MAX_KEYS>(qs, cl, b); }
+
+  // Sums over the sequences: lane l of a wave takes sequence l of every 64.
+  static __device__ __forceinline__ int steps_of(const int* qs, const int* cl, int b) { return b < SEQS ? HKV * head_steps(sequence(qs, cl, b)) : 0; }
+#ifndef MONONN_ONE_THREAD
+  // steps of the whole call
+  static __device__ __forceinline__ int total_steps(const int* qs, const int* cl) {
+    int n = 0;
+    for (int base = 0; base < SEQS; base += kWaveSize) n += wave_all_reduce(steps_of(qs, cl, base + lane_id()), [](int a, int c) { return a + c; });
+    return __builtin_amdgcn_readfirstlane(n);
+  }
+  // the sequence that holds step `rem` of the call; `rem` becomes the step inside it
+  static __device__ __forceinline__ int sequence_with_step(const int* qs, const int* cl, int& rem) {
+    int found = SEQS - 1;
+    for (int base = 0; base < SEQS; base += kWaveSize) {
+      const int v = steps_of(qs, cl, base + lane_id());
+      int upto = v;   // inclusive sum over the lanes
+#pragma unroll
+      for (int off = 1; off < kWaveSize; off <<= 1) {
+        const int o = __shfl_up(upto, off, kWaveSize);
+        if (lane_id() >= off) upto += o;
+      }
+      const unsigned long long behind = __ballot(upto > rem);
+      if (behind != 0) {
+        const int l = __builtin_ctzll(behind);
+        found = base + l;
+        rem -= __shfl(upto - v, l, kWaveSize);
+        break;
+      }
+      rem -= __shfl(upto, kWaveSize - 1, kWaveSize);
+    }
+    rem = __builtin_amdgcn_readfirstlane(rem);
+    return __builtin_amdgcn_readfirstlane(clamp_int(found, 0, SEQS - 1));
+  }
+#else   // for a host build that runs one thread at a time
+  static __device__ __forceinline__ int total_steps(const int* qs, const int* cl) {
+    int n = 0;
+    for (int b = 0; b < SEQS; ++b) n += steps_of(qs, cl, b);
+    return n;
+  }
+  static __device__ __forceinline__ int sequence_with_step(const int* qs, const int* cl, int& rem) {
+    for (int b = 0; b < SEQS; ++b) {
+      if (rem < steps_of(qs, cl, b)) return b;
+      rem -= steps_of(qs, cl, b);
+    }
+    return SEQS - 1;
+  }
+#endif
+  // the item that holds step `at` of the call (0 <= at < total_steps) and the step inside it
+  static __device__ __forceinline__ Item locate(const int* qs, const int* cl, int at, int& inside) {
+    Item it;
+    int rem = at;
+    it.b = sequence_with_step(qs, cl, rem);
+    it.s = sequence(qs, cl, it.b);
+    it.s.start = __builtin_amdgcn_readfirstlane(it.s.start);
+    it.s.len = __builtin_amdgcn_readfirstlane(it.s.len);
+    it.s.ctx = __builtin_amdgcn_readfirstlane(it.s.ctx);
+    it.narrow = is_narrow(it.s.len);
+    int per_head = head_steps(it.s);
+    if (per_head < 1) per_head = 1;
+    it.h = clamp_int(rem / per_head, 0, HKV - 1);
+    rem -= it.h * per_head;
+    const int tiles = tiles_of(it.s.len);
+    it.tile = 0;
+    tile_steps(it.s, 0, it.first, it.steps);
+    while (rem >= it.steps && it.tile + 1 < tiles) {
+      rem -= it.steps;
+      ++it.tile;
+      tile_steps(it.s, it.tile, it.first, it.steps);
+    }
+    inside = clamp_int(rem, 0, it.steps - 1);
+    return it;
+  }
+  // Ranges follow each other inside an XCD (workgroup u runs on XCD u % 8 of an even deal): the tiles of one key head
+  // then read its keys through the same L2.
+  static __device__ __forceinline__ int range_of(int unit) { return GRID % kXcds == 0 ? unit % kXcds * (GRID / kXcds) + unit / kXcds : unit; }
+  static __device__ __forceinline__ int range_begin(int total, int range) { return (int)((long)total * range / GRID); }
+
+  // ---- loads -----------------------------------------------------------------------------------------------------
+  static __device__ __forceinline__ int page_of(const int* table, int b, int key) {
+    key = clamp_int(key, 0, MAX_KEYS - 1);
+    return clamp_int(table[(long)b * WIDTH + key / PAGE], 0, PAGES - 1);
+  }
+  static __device__ __forceinline__ long row_offset(int page, int key, int h) {
+    key = clamp_int(key, 0, MAX_KEYS - 1);
+    return (((long)page * PAGE + key % PAGE) * HKV + h) * D;
+  }
+  static __device__ __forceinline__ half8_t load_piece(const T* p) { return *reinterpret_cast<const half8_t*>(p); }
+
+  // the lane's query row: operand of the first product, and the keys it sees, [lo, hi]
+  struct Rows {
+    half8_t q[QS];
+    int lo, hi;
+    bool valid;
+    long out;   // element offset of the row
+  };
+  static __device__ __forceinline__ long row_element(const Item& it, int row) {
+    return ((long)clamp_int(it.s.start + row / G, 0, TOKENS - 1) * H + it.h * G + row % G) * D;
+  }
+  static __device__ __forceinline__ void load_rows(const T* q, const Item& it, int row0, Rows& r) {
+    const int lane = lane_id(), count = it.s.len * G;
+    int row = row0 + (lane & 31);
+    r.valid = row < count;
+    if (!r.valid) row = count > 0 ? count - 1 : 0;
+    const int t = row / G;
+    r.out = row_element(it, row);
+#pragma unroll
+    for (int i = 0; i < QS; ++i) r.q[i] = load_piece(q + r.out + i * 16 + (lane >> 5) * 8);
+    r.hi = it.s.ctx - it.s.len + t;
+    r.lo = WINDOW > 0 ? r.hi - WINDOW + 1 : 0;
+  }
+
+  struct State {
+    float16_t o[DT];
+    float m, l;   // of the lane's query; l of the lane's half of the keys until finish()
+    __device__ __forceinline__ void clear() {
+      m = -1e30f;
+      l = 0.0f;
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
+    }
+    __device__ __forceinline__ void finish() { l += half_wave_other(l); }
+  };
+
+  // BLOCKS x 32 keys from LDS on 32 query rows.  `check`: some row does not see all of these keys.
+  template <int BLOCKS>
+  static __device__ __forceinline__ void step(const char* kbuf, const char* vbuf, int key0, const Rows& r, State& st, float scale_log2, bool check) {
+    const int lane = lane_id(), half = lane >> 5;
+    float16_t s[BLOCKS];
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[b][i] = 0.0f;
+      const char* row = kbuf + (b * 32 + (lane & 31)) * KP + half * 16;
+#pragma unroll
+      for (int i = 0; i < QS; ++i) s[b] = mfma_32x32x16<kBf16>(*reinterpret_cast<const half8_t*>(row + i * 32), r.q[i], s[b]);
+    }
+    if (check) {
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int key = key0 + b * 32 + 8 * (i / 4) + 4 * half + i % 4;
+          s[b][i] = key >= r.lo && key <= r.hi ? s[b][i] : -__builtin_inff();
+        }
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
+    top = fmaxf(top, half_wave_other(top)) * scale_log2;
+    const float m = fmaxf(st.m, top);
+    if (__any(m > st.m)) {   // the same for the whole wave
+      const float a = __builtin_amdgcn_exp2f(st.m - m);
+      st.l *= a;
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) st.o[t][i] *= a;
+      st.m = m;
+    }
+    // probabilities are rounded to the element type for the second product; the sum takes the unrounded ones
+    float sum = 0.0f;
+    half8_t p[BLOCKS][2];
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float e = __builtin_amdgcn_exp2f(s[b][i] * scale_log2 - m);
+        sum += e;
+        p[b][i / 8][i % 8] = __builtin_bit_cast(half_t, (T)e);
+      }
+    st.l += sum;
+    const int i16 = lane & 15;
+    const char* vrow = vbuf + (4 * half + i16 / 4) * VP + ((lane >> 4) & 1) * 32 + (i16 & 3) * 8;
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          struct { mononn_short4 lo, hi; } v;
+          v.lo = MONONN_LDS_READ_TR16(vrow + (b * 32 + k * 16) * VP + t * 64);
+          v.hi = MONONN_LDS_READ_TR16(vrow + (b * 32 + k * 16 + 8) * VP + t * 64);
+          st.o[t] = mfma_32x32x16<kBf16>(__builtin_bit_cast(half8_t, v), p[b][k], st.o[t]);
+        }
+  }
+
+  // ---- results ---------------------------------------------------------------------------------------------------
+  // four output elements of the lane's row: d = 32 * (g / 4) + 8 * (g % 4) + 4 * (lane / 32)
+  static __device__ __forceinline__ void store_group(T* out, const Rows& r, int g, float a, float b, float c, float d) {
+    const int at = (g / 4) * 32 + (g % 4) * 8 + (lane_id() >> 5) * 4;
+    if (!r.valid || at >= D) return;
+    const T v[4] = {(T)a, (T)b, (T)c, (T)d};
+    store_run<COHERENT, T, 4>(out + r.out + at, v);
+  }
+  static __device__ __forceinline__ void store_part(float* to, int g, float a, float b, float c, float d) {
+    const float v[4] = {a, b, c, d};
+    stN<float, 4>(to + g * 256 + lane_id() * 4, v);
+  }
+  // maximum and sum of the 32 queries behind the tiles
+  static __device__ __forceinline__ void store_part_sums(float* to, float m, float l) {
+    const int lane = lane_id();
+    st1(to + DT * 1024 + lane, lane < 32 ? m : l);
+  }
+  static __device__ __forceinline__ float inverse(float l) { return l > 0.0f || l != l ? 1.0f / l : 0.0f; }   // a row without keys: zeros
+
+  // ---- wide items ------------------------------------------------------------------------------------------------
+  static constexpr int kRuns = (kWideKeys * CPR + MONONN_BLOCK_SIZE - 1) / MONONN_BLOCK_SIZE;   // pieces of K (and of V) a thread moves per step
+  static __device__ __forceinline__ void wide_pages(const int* table, const Item& it, int key0, int (&page)[kRuns]) {
+#pragma unroll
+    for (int i = 0; i < kRuns; ++i) page[i] = page_of(table, it.b, key0 + (thread_id() + i * MONONN_BLOCK_SIZE) / CPR);
+  }
+  static __device__ __forceinline__ void wide_load(const T* kc, const T* vc, const Item& it, int key0, const int (&page)[kRuns], half8_t (&k)[kRuns], half8_t (&v)[kRuns]) {
+#pragma unroll
+    for (int i = 0; i < kRuns; ++i) {
+      const int at = thread_id() + i * MONONN_BLOCK_SIZE;
+      const long off = row_offset(page[i], key0 + at / CPR, it.h) + at % CPR * 8;
+      k[i] = load_piece(kc + off);
+      v[i] = load_piece(vc + off);
+    }
+  }
+  // rows behind the sequence's last key become zeros: whatever those cells hold, NaN included, must not reach 0 * v
+  static __device__ __forceinline__ void wide_store(char* buf, int key0, int ctx, const half8_t (&k)[kRuns], const half8_t (&v)[kRuns]) {
+#pragma unroll
+    for (int i = 0; i < kRuns; ++i) {
+      const int at = thread_id() + i * MONONN_BLOCK_SIZE, row = at / CPR, c = at % CPR;
+      if (kWideKeys * CPR % MONONN_BLOCK_SIZE != 0 && row >= kWideKeys) break;
+      const bool in = key0 + row < ctx;
+      const half8_t zero = {0, 0, 0, 0, 0, 0, 0, 0};
+      *reinterpret_cast<half8_t*>(buf + row * KP + c * 16) = in ? k[i] : zero;
+      *reinterpret_cast<half8_t*>(buf + kWideKeys * KP + row * VP + c * 16) = in ? v[i] : zero;
+    }
+  }
+  static __device__ __forceinline__ void wide(const T* q, const T* kc, const T* vc, const int* table, T* out, float* part, const Item& it, int from, int count, bool whole,
+                                              float scale_log2, char* smem, int& turn) {
+    const int wave = __builtin_amdgcn_readfirstlane(wave_id());
+    const int rows = it.s.len * G, row0 = it.tile * 32 * NW + wave * 32;
+    const bool live = row0 < rows;
+    Rows r;
+    load_rows(q, it, row0, r);
+    // keys that the wave's first and last row see
+    const int t_first = row0 / G, t_last = (row0 + 31 < rows ? row0 + 31 : rows - 1) / G;
+    const int p_first = it.s.ctx - it.s.len + t_first, p_last = it.s.ctx - it.s.len + t_last;
+    State st;
+    st.clear();
+    half8_t k[kRuns], v[kRuns];
+    int page[kRuns];
+    const int begin = (it.first + from) * kWideKeys;
+    wide_pages(table, it, begin, page);
+    wide_load(kc, vc, it, begin, page, k, v);
+    wide_pages(table, it, begin + kWideKeys, page);
+    for (int i = 0; i < count; ++i) {
+      const int key0 = begin + i * kWideKeys;
+      char* buf = smem + turn * kWideBuffer;
+      turn ^= 1;
+      wide_store(buf, key0, it.s.ctx, k, v);
+      __syncthreads();
+      if (i + 1 < count) {
+        wide_load(kc, vc, it, key0 + kWideKeys, page, k, v);
+        wide_pages(table, it, key0 + 2 * kWideKeys, page);
+      }
+      const bool none = !live || key0 > p_last || (WINDOW > 0 && key0 + kWideKeys - 1 < p_first - WINDOW + 1);
+      if (!none) {
+        const bool check = key0 + kWideKeys - 1 > p_first || (WINDOW > 0 && key0 < p_last - WINDOW + 1);
+        step<2>(buf, buf + kWideKeys * KP, key0, r, st, scale_log2, check);
+      }
+    }
+    st.finish();
+    if (!live) return;
+    if (whole) {
+      const float inv = inverse(st.l);
+#pragma unroll
+      for (int g = 0; g < DT * 4; ++g) store_group(out, r, g, st.o[g / 4][g % 4 * 4] * inv, st.o[g / 4][g % 4 * 4 + 1] * inv, st.o[g / 4][g % 4 * 4 + 2] * inv, st.o[g / 4][g % 4 * 4 + 3] * inv);
+    } else {
+      float* to = part + wave * kPartWave;
+#pragma unroll
+      for (int g = 0; g < DT * 4; ++g) store_part(to, g, st.o[g / 4][g % 4 * 4], st.o[g / 4][g % 4 * 4 + 1], st.o[g / 4][g % 4 * 4 + 2], st.o[g / 4][g % 4 * 4 + 3]);
+      store_part_sums(to, st.m, st.l);
+    }
+  }
+
+  // ---- narrow items ----------------------------------------------------------------------------------------------
+  static constexpr int kMine = CPR / 2;   // pieces of K (and of V) a lane moves per step: 32 rows over 64 lanes
+  static __device__ __forceinline__ void narrow_load(const T* kc, const T* vc, const int* table, const Item& it, int key0, half8_t (&k)[kMine], half8_t (&v)[kMine]) {
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int at = lane_id() + i * kWaveSize, key = key0 + at / CPR;
+      const long off = row_offset(page_of(table, it.b, key), key, it.h) + at % CPR * 8;
+      k[i] = load_piece(kc + off);
+      v[i] = load_piece(vc + off);
+    }
+  }
+  static __device__ __forceinline__ void narrow(const T* q, const T* kc, const T* vc, const int* table, T* out, float* part, const Item& it, int from, int count, bool whole,
+                                                float scale_log2, char* smem) {
+    const int wave = __builtin_amdgcn_readfirstlane(wave_id());
+    const bool live = wave < NN;
+    Rows r;
+    load_rows(q, it, 0, r);
+    State st;
+    st.clear();
+    __syncthreads();   // the buffers may still be read by a wide item's last step
+    if (live) {
+      char* kbuf = smem + wave * kWaveBuffer;
+      char* vbuf = kbuf + 32 * KP;
+      const int p_first = it.s.ctx - it.s.len, p_last = it.s.ctx - 1;
+      half8_t k[kMine], v[kMine];
+      const int begin = (it.first + from) * kNarrowKeys + wave * 32;
+      narrow_load(kc, vc, table, it, begin, k, v);
+      for (int i = 0; i < count; ++i) {
+        const int key0 = begin + i * kNarrowKeys;
+#pragma unroll
+        for (int j = 0; j < kMine; ++j) {
+          const int at = lane_id() + j * kWaveSize, row = at / CPR, c = at % CPR;
+          const bool in = key0 + row < it.s.ctx;
+          const half8_t zero = {0, 0, 0, 0, 0, 0, 0, 0};
+          *reinterpret_cast<half8_t*>(kbuf + row * KP + c * 16) = in ? k[j] : zero;
+          *reinterpret_cast<half8_t*>(vbuf + row * VP + c * 16) = in ? v[j] : zero;
+        }
+        if (i + 1 < count) narrow_load(kc, vc, table, it, key0 + kNarrowKeys, k, v);
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();   // the wave's own rows: written above, read below
+        const bool none = key0 > p_last || (WINDOW > 0 && key0 + 31 < p_first - WINDOW + 1);
+        if (!none) {
+          const bool check = key0 + 31 > p_first || (WINDOW > 0 && key0 < p_last - WINDOW + 1);
+          step<1>(kbuf, vbuf, key0, r, st, scale_log2, check);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+      }
+    }
+    st.finish();
+    // the waves' shares of the keys meet in LDS; every wave then adds up some of the output groups
+    __syncthreads();
+    float* sums = reinterpret_cast<float*>(smem);             // [NN][64]: maxima, sums
+    float* tiles = sums + NN * 64;                            // [NN][DT * 4][64][4]
+    if (live) {
+      sums[wave * 64 + lane_id()] = lane_id() < 32 ? st.m : st.l;
+#pragma unroll
+      for (int g = 0; g < DT * 4; ++g) {
+        const float4_t o = {st.o[g / 4][g % 4 * 4], st.o[g / 4][g % 4 * 4 + 1], st.o[g / 4][g % 4 * 4 + 2], st.o[g / 4][g % 4 * 4 + 3]};
+        *reinterpret_cast<float4_t*>(tiles + (wave * DT * 4 + g) * 256 + lane_id() * 4) = o;
+      }
+    }
+    __syncthreads();
+    const int query = lane_id() & 31;
+    float m = -1e30f, l = 0.0f, w[NN];
+#pragma unroll
+    for (int i = 0; i < NN; ++i) m = fmaxf(m, sums[i * 64 + query]);
+#pragma unroll
+    for (int i = 0; i < NN; ++i) {
+      w[i] = __builtin_amdgcn_exp2f(sums[i * 64 + query] - m);
+      l += w[i] * sums[i * 64 + 32 + query];
+    }
+    const float inv = whole ? inverse(l) : 1.0f;
+    for (int g = wave; g < DT * 4; g += NW) {
+      float4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int i = 0; i < NN; ++i) o += w[i] * *reinterpret_cast<const float4_t*>(tiles + (i * DT * 4 + g) * 256 + lane_id() * 4);
+      if (whole) store_group(out, r, g, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+      else store_part(part, g, o[0], o[1], o[2], o[3]);
+    }
+    if (!whole && wave == 0) store_part_sums(part, m, l);
+    __syncthreads();
+  }
+
+  // ---- stages ----------------------------------------------------------------------------------------------------
+  // part: [2 * GRID][kPart]; slot 2 r: a part that an earlier range began, slot 2 r + 1: one that range r begins
+  static __device__ __forceinline__ void partial(int unit, const T* q, const T* kc, const T* vc, const int* table, const int* qs, const int* cl, T* out, float* part, float scale,
+                                                 char* smem) {
+    // tokens of no sequence: zeros
+    const int inside0 = clamp_int(qs[0], 0, TOKENS), inside1 = clamp_int(qs[SEQS], 0, TOKENS);
+    if (inside0 > 0 || inside1 < TOKENS) {
+      const T zero[8] = {(T)0.0f, (T)0.0f, (T)0.0f, (T)0.0f, (T)0.0f, (T)0.0f, (T)0.0f, (T)0.0f};
+      for (int t = unit; t < TOKENS; t += GRID)
+        if (t < inside0 || t >= inside1)
+          for (int c = thread_id(); c < H * CPR; c += MONONN_BLOCK_SIZE) store_run<COHERENT, T, 8>(out + (long)t * H * D + c * 8, zero);
+    }
+    const int total = total_steps(qs, cl), range = range_of(unit);
+    const int end = range_begin(total, range + 1);
+    int at = range_begin(total, range), turn = 0;
+    const float scale_log2 = scale * 1.44269504088896f;
+    __syncthreads();
+    while (at < end) {
+      int inside;
+      const Item it = locate(qs, cl, at, inside);
+      const int count = it.steps - inside < end - at ? it.steps - inside : end - at;
+      const bool whole = inside == 0 && count == it.steps;
+      float* to = part + (long)(2 * range + (inside == 0 ? 1 : 0)) * kPart;
+      if (it.narrow) narrow(q, kc, vc, table, out, to, it, inside, count, whole, scale_log2, smem);
+      else wide(q, kc, vc, table, out, to, it, inside, count, whole, scale_log2, smem, turn);
+      at += count;
+    }
+    __syncthreads();
+  }
+
+  static __device__ __forceinline__ void join(int unit, const float* part, const int* qs, const int* cl, T* out) {
+    const int total = total_steps(qs, cl), range = range_of(unit);
+    const int begin = range_begin(total, range), end = range_begin(total, range + 1);
+    if (begin >= end) return;
+    int inside;
+    const Item it = locate(qs, cl, end - 1, inside);
+    const int item0 = end - 1 - inside, item1 = item0 + it.steps;
+    if (item0 < begin || item1 <= end) return;   // begun by an earlier range, or finished in this one
+    const int wave = __builtin_amdgcn_readfirstlane(wave_id()), lane = lane_id(), query = lane & 31;
+    // a wide item: every wave its own rows; a narrow one: every wave some groups of the 32 rows
+    const int block = it.narrow ? 0 : wave;
+    Rows r;
+    {
+      const int count = it.s.len * G;
+      int row = it.tile * (it.narrow ? 32 : 32 * NW) + block * 32 + query;
+      r.valid = row < count;
+      if (!r.valid) row = count > 0 ? count - 1 : 0;
+      r.out = row_element(it, row);
+    }
+    const float* sums = part + block * kPartWave + DT * 1024;
+    const int last = [&] {   // the last range that holds a step of the item
+      int x = range;
+      while (x + 1 < GRID && range_begin(total, x + 1) < item1) ++x;
+      return x;
+    }();
+    float m = -1e30f, l = 0.0f;
+    for (int x = range; x <= last; ++x) {
+      if (range_begin(total, x) == range_begin(total, x + 1)) continue;
+      m = fmaxf(m, sums[(long)(2 * x + (x == range ? 1 : 0)) * kPart + query]);
+    }
+    for (int x = range; x <= last; ++x) {
+      if (range_begin(total, x) == range_begin(total, x + 1)) continue;
+      const float* s = sums + (long)(2 * x + (x == range ? 1 : 0)) * kPart;
+      l += s[32 + query] * __builtin_amdgcn_exp2f(s[query] - m);
+    }
+    const float inv = inverse(l);
+    for (int g = it.narrow ? wave : 0; g < DT * 4; g += it.narrow ? NW : 1) {
+      float4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
+      for (int x = range; x <= last; ++x) {
+        if (range_begin(total, x) == range_begin(total, x + 1)) continue;
+        const long slot = (long)(2 * x + (x == range ? 1 : 0)) * kPart;
+        o += __builtin_amdgcn_exp2f(sums[slot + query] - m) * *reinterpret_cast<const float4_t*>(part + slot + block * kPartWave + g * 256 + lane * 4);
+      }
+      store_group(out, r, g, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+    }
+  }
+};
+
+// ---------------------------------------------------------------------------------------------
+// 4-bit weights
+// ---------------------------------------------------------------------------------------------
+// y[m, n] = sum over groups of scale[n, group] * sum over k of (w[n, k] - zero[n, group]) * x[m, k], weights two to a
+// byte along k (the low half is the lower k), zero = 8 without a tensor of zero points.
+//
+// A wave takes 16 weight rows and walks k in chunks of 128: one 16-byte load per lane, lane (r, g) = row r, weights 32 g ..
+// 32 g + 31.  A 4 x 4 transposition of dwords between the four lane groups gives each contraction step of
+// v_mfma_f32_16x16x32 32 consecutive k, so that a step never crosses a group of 32 and a lane's result column is one
+// weight row with one scale.  Weights enter the product as small integers, exactly; scales are applied to its f32 result.
+template <class T>
+struct Nibbles;
+template <>
+struct Nibbles<half_t> {
+  static constexpr int kBias = 8;   // subtracted on the way
+  // 1024 + v in f16 by setting exponent bits, v = (w >> s) & 15 in the last places; elements 0, 4, 1, 5, 2, 6, 3, 7 of the dword
+  static __device__ __forceinline__ half8_t operands(unsigned w) {
+    half8_t r;
+    const half2_t one = {(half_t)1032.0f, (half_t)1032.0f}, sixteenth = {(half_t)0.0625f, (half_t)0.0625f}, high = {(half_t)72.0f, (half_t)72.0f};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const unsigned x = i ? w >> 8 : w;
+      const half2_t lo = __builtin_bit_cast(half2_t, (x & 0x000f000fu) | 0x64006400u) - one;
+      const half2_t hi = __builtin_elementwise_fma(__builtin_bit_cast(half2_t, (x & 0x00f000f0u) | 0x64006400u), sixteenth, -high);
+      r[4 * i] = lo[0], r[4 * i + 1] = lo[1], r[4 * i + 2] = hi[0], r[4 * i + 3] = hi[1];
+    }
+    return r;
+  }
+};
+template <>
+struct Nibbles<__bf16> {
+  static constexpr int kBias = -128;   // 128 + v: there is no packed bf16 subtraction, the sum of x takes it out again
+  static __device__ __forceinline__ half8_t operands(unsigned w) {
+    struct { unsigned d[4]; } r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.d[i] = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+    return __builtin_bit_cast(half8_t, r);
+  }
+};
+
+// 8 consecutive elements in the order of Nibbles::operands
+__device__ __forceinline__ half8_t nibble_order(half8_t x) {
+  return __builtin_shufflevector(x, x, 0, 4, 1, 5, 2, 6, 3, 7);
+}
+
+// exchanges dword i of lane group j with dword j of lane group i (groups of 16 lanes)
+__device__ __forceinline__ void transpose_lane_groups(unsigned (&d)[4]) {
+  auto swap32 = [](unsigned& a, unsigned& b) {   // upper half of a <-> lower half of b
+    const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+    a = r[0], b = r[1];
+  };
+  auto swap16 = [](unsigned& a, unsigned& b) {   // odd groups of a <-> even groups of b
+    const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+    a = r[0], b = r[1];
+  };
+  swap32(d[0], d[2]);
+  swap32(d[1], d[3]);
+  swap16(d[0], d[1]);
+  swap16(d[2], d[3]);
+}
+
+template <class T, int M, int N, int K, int GROUP, bool ZEROS, int WK, bool COHERENT>
+struct MatvecW4 {
+  static constexpr int NW = MONONN_BLOCK_SIZE / kWaveSize;
+  static constexpr int TILES = NW / WK;                       // tiles of 16 weight rows a workgroup takes at once
+  static constexpr int MT = (M + 15) / 16 < 4 ? (M + 15) / 16 : 4;   // blocks of 16 rows of x per pass over the weights
+  static constexpr int CHUNKS = (K + 127) / 128;
+  static constexpr int MINE = (CHUNKS + WK - 1) / WK;         // chunks of a wave (consecutive)
+  static constexpr int DEPTH = MINE < 8 ? MINE : 8;           // chunks in flight
+  static constexpr int GROUPS = K / GROUP;
+  static constexpr int PER_CHUNK = GROUP >= 128 ? 1 : 128 / GROUP;   // scales of a row in a chunk
+  static constexpr int STEPS = 4 / PER_CHUNK;                 // contraction steps per scale
+  static constexpr bool kBf16 = IsBf16<T>::value;
+  static constexpr bool kSums = ZEROS || Nibbles<T>::kBias != 8;
+  static constexpr int ROWS = M < 4 ? M : 4;                  // result rows a lane looks at: row 4 * (lane / 16) + i
+  static constexpr int num_units() { return ((N + 15) / 16 + TILES - 1) / TILES * ((M + 16 * MT - 1) / (16 * MT)); }
+  static constexpr int lds_bytes() { return WK > 1 ? NW * MT * 1024 : 0; }
+
+  struct Chunk {
+    unsigned w[4];
+    T scale[PER_CHUNK];
+    unsigned char zero[PER_CHUNK];
+  };
+  static __device__ __forceinline__ void load(const unsigned char* weight, const T* scale, const unsigned char* zero, long row, int chunk, Chunk& c) {
+    const int g = lane_id() >> 4;
+    int at = chunk * 64 + g * 16;
+    if (K % 128 != 0 && at > K / 2 - 16) at = K / 2 - 16;     // behind the last column: any weights, x is zero there
+    typedef unsigned u4 __attribute__((ext_vector_type(4)));
+    const u4 w = *reinterpret_cast<const u4*>(weight + row * (K / 2) + at);
+    c.w[0] = w[0], c.w[1] = w[1], c.w[2] = w[2], c.w[3] = w[3];
+#pragma unroll
+    for (int i = 0; i < PER_CHUNK; ++i) {
+      int at_group = GROUP >= 128 ? chunk / (GROUP / 128 > 0 ? GROUP / 128 : 1) : chunk * PER_CHUNK + i;
+      if (at_group > GROUPS - 1) at_group = GROUPS - 1;
+      c.scale[i] = scale[row * GROUPS + at_group];
+      if constexpr (ZEROS) c.zero[i] = zero[row * GROUPS + at_group];
+    }
+  }
+
+  static __device__ __forceinline__ void unit(int unit, const T* x, const unsigned char* weight, const T* scale, const unsigned char* zero, T* y, char* smem) {
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), g = lane >> 4, r16 = lane & 15;
+    constexpr int ROW_UNITS = ((N + 15) / 16 + TILES - 1) / TILES;
+    const int pass = unit / ROW_UNITS, tile = unit % ROW_UNITS * TILES + wave / WK, part = wave % WK;
+    const int n = tile * 16 + r16, m0 = pass * 16 * MT;
+    const long row = n < N ? n : N - 1;
+    const int c0 = part * MINE, c1 = c0 + MINE < CHUNKS ? c0 + MINE : CHUNKS;
+    float4_t acc[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[t] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    Chunk ring[DEPTH];
+#pragma unroll
+    for (int i = 0; i < DEPTH; ++i) load(weight, scale, zero, row, c0 + i < CHUNKS ? c0 + i : CHUNKS - 1, ring[i]);
+    for (int base = c0; base < c1; base += DEPTH) {
+#pragma unroll
+      for (int i = 0; i < DEPTH; ++i) {
+        const int c = base + i;
+        if (c >= c1) break;
+        Chunk ch = ring[i];
+        if (c + DEPTH < c1) load(weight, scale, zero, row, c + DEPTH, ring[i]);
+        transpose_lane_groups(ch.w);
+#pragma unroll
+        for (int p = 0; p < PER_CHUNK; ++p) {
+          const float s = (float)ch.scale[p];
+          const float z = ZEROS ? (float)((int)ch.zero[p] - Nibbles<T>::kBias) : (float)(8 - Nibbles<T>::kBias);
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {
+            float4_t dot = {0.0f, 0.0f, 0.0f, 0.0f}, sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int k = 0; k < STEPS; ++k) {
+              const int step = p * STEPS + k, at = c * 128 + step * 32 + g * 8, m = m0 + t * 16 + r16;
+              half8_t a = {0, 0, 0, 0, 0, 0, 0, 0};
+              if (m < M && (K % 128 == 0 || at < K)) a = nibble_order(*reinterpret_cast<const half8_t*>(x + (long)m * K + at));
+              dot = mfma_16x16x32<kBf16>(a, Nibbles<T>::operands(ch.w[step]), dot);
+              if constexpr (kSums) {
+                const T one = (T)1.0f;
+                const half_t o = __builtin_bit_cast(half_t, one);
+                sum = mfma_16x16x32<kBf16>(a, half8_t{o, o, o, o, o, o, o, o}, sum);
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < ROWS; ++i) {
+              if constexpr (kSums) acc[t][i] += s * (dot[i] - z * sum[i]);
+              else acc[t][i] += s * dot[i];
+            }
+          }
+        }
+      }
+    }
+    if constexpr (WK > 1) {
+      float* shares = reinterpret_cast<float*>(smem);
+      __syncthreads();
+#pragma unroll
+      for (int t = 0; t < MT; ++t) *reinterpret_cast<float4_t*>(shares + ((wave * MT + t) * 64 + lane) * 4) = acc[t];
+      __syncthreads();
+      if (part == 0) {
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+          for (int o = 1; o < WK; ++o) acc[t] += *reinterpret_cast<const float4_t*>(shares + (((wave + o) * MT + t) * 64 + lane) * 4);
+      }
+    }
+    if (part == 0 && n < N) {
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) {
+          const int m = m0 + t * 16 + 4 * g + i;
+          if (m < M) {
+            const T v[1] = {(T)acc[t][i]};
+            store_run<COHERENT, T, 1>(y + (long)m * N + n, v);
+          }
+        }
+    }
+  }
+};
+
+}  // namespace mononn_dev

@@ -37,7 +37,7 @@ std::string Program::summary() const {
   std::ostringstream os;
   os << "stages=" << num_stages << " nodes=" << nodes.size() << " temp_bytes=" << temp_bytes << "\n";
   for (auto& n : nodes) {
-    os << "  stage " << n.stage << "  " << (n.kind == NodeKind::kGemm ? "gemm   " : n.kind == NodeKind::kAttention ? "attn   " : (n.row_program ? "rowred " : "elewise")) << " " << n.name;
+    os << "  stage " << n.stage << "  " << (n.kind == NodeKind::kGemm ? "gemm   " : n.kind == NodeKind::kAttention ? "attn   " : n.kind == NodeKind::kOperator ? "oper   " : (n.row_program ? "rowred " : "elewise")) << " " << n.name;
     if (n.kind == NodeKind::kGemm) os << "  [" << n.gemm.problem_hash() << "] members=" << n.members.size() << (n.prologue.empty() ? "" : (n.prologue_stores ? " +row-prologue(stores)" : " +row-prologue"));
     else if (n.kind == NodeKind::kAttention) os << "  [" << n.gemm.problem_hash() << " -> " << n.gemm2.problem_hash() << "] members=" << n.members.size();
     else os << "  members=" << n.members.size() << (n.row_program ? " rows=" + std::to_string(n.rows) + " len=" + std::to_string(n.row_len) : "");
@@ -141,7 +141,9 @@ struct Builder {
       Node n;
       n.name = ins->name;
       n.members.push_back(ins);
-      if (op == "custom-call" || op == "dot") {
+      if (ins->is_operator()) {
+        n.kind = NodeKind::kOperator;
+      } else if (op == "custom-call" || op == "dot") {
         n.kind = NodeKind::kGemm;
         n.gemm = ins->is_conv() ? describe_conv(ins) : describe_gemm(ins);
       } else {
@@ -270,7 +272,7 @@ struct Builder {
 
   // may the kernel keep the right-hand GEMM operand `root` ([.., K, N]) transposed in memory?
   bool can_store_k_contig(const Instr* root, const Instr* operand, int rhs_contracting) const {
-    if (root->opcode == "parameter" || root->opcode == "constant") return false;
+    if (root->opcode == "parameter" || root->opcode == "constant" || defining_member(root)->is_operator()) return false;
     if (root->shape.dims != operand->shape.dims) return false;   // reached through a reshaping alias
     for (auto* u : root->users) {
       if (is_alias_op(u)) return false;
@@ -630,13 +632,17 @@ struct Builder {
     // a use of `operand` as [rows, k] in the given order; `perm_ok`: the root may carry the k-contiguous transposition
     auto use = [&](const Instr* operand, bool fits, int64_t rows, int64_t k, Order order, bool perm_ok) {
       const Instr* root = p.storage_root(operand);
-      fits = fits && rows % 16 == 0 && k % 32 == 0 && p.producer.count(root) && !live.count(root) && (perm_ok || !p.physical_perm.count(root)) &&
+      fits = fits && rows % 16 == 0 && k % 32 == 0 && p.producer.count(root) && !defining_member(root)->is_operator() && !live.count(root) && (perm_ok || !p.physical_perm.count(root)) &&
              hlo::is_half_float(root->shape.dtype) && root->shape.num_elements() == rows * k &&
              (!want.count(root) || (want[root].k == k && want[root].order == order));
       if (fits) want[root] = {k, order};
       else spoiled.insert(root);
     };
     for (auto& n : p.nodes) {
+      if (n.kind == NodeKind::kOperator) {   // operators read and write row-major values
+        spoiled.insert(n.inputs.begin(), n.inputs.end());
+        continue;
+      }
       if (n.kind == NodeKind::kAttention) {
         const GemmDesc& d1 = n.gemm;
         const GemmDesc& d2 = n.gemm2;
@@ -726,6 +732,17 @@ struct Builder {
     }
   }
 
+  // what the buffers of operator nodes need to know
+  void describe_operators() {
+    for (auto& n : p.nodes) {
+      if (n.kind != NodeKind::kOperator) continue;
+      const Instr* ins = n.members[0];
+      if (ins->oper.kind == hlo::OperatorConfig::kKvAppend)
+        for (auto* v : n.outputs) p.in_place[v] = ins->operands[v->tuple_index == 0 ? 2 : 3];
+      if (ins->oper.kind == hlo::OperatorConfig::kPagedAttentionParts) p.temp_size[ins] = codegen::paged_attention_part_bytes(ins, opt.grid, opt.waves);
+    }
+  }
+
   void apply_split_k() {
     // a projection absorbed by an attention node leaves it as one partial sum per head
     for (auto& n : p.nodes)
@@ -796,8 +813,16 @@ struct Builder {
         auto sk = p.split_k.find(v);
         if (sk != p.split_k.end()) b.bytes = v->shape.num_elements() * 4 * sk->second;
         b.def_stage = b.last_use_stage = n.stage;
+        // the stage in front of the join of a paged attention already writes the results that need no joining
+        if (n.kind == NodeKind::kOperator && n.members[0]->oper.kind == hlo::OperatorConfig::kPagedAttention) b.def_stage = n.stage - 1;
+        auto ts = p.temp_size.find(v);
+        if (ts != p.temp_size.end()) b.bytes = ts->second;
         auto li = live_index.find(v);
-        if (li != live_index.end()) {
+        auto ip = p.in_place.find(v);
+        if (ip != p.in_place.end()) {
+          b.kind = Buffer::kParameter;
+          b.index = static_cast<int>(ip->second->parameter_number);
+        } else if (li != live_index.end()) {
           b.kind = Buffer::kLiveOut;
           b.index = li->second;
         } else {
@@ -874,6 +899,7 @@ std::unique_ptr<Program> build_program(std::unique_ptr<hlo::Module> module, cons
   if (!take.empty()) b.fuse_attention_out_proj();
   if (opt.fuse_gemm_prologue && b.enabled("GemmPrologueFusionPass")) b.fuse_gemm_prologues();
   b.finalize();
+  b.describe_operators();
   b.decide_constant_layouts();
   b.fold_layer_norms();
   b.apply_split_k();

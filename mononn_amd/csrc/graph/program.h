@@ -22,7 +22,8 @@ namespace graph {
 
 // kAttention: GEMM -> row program over the GEMM's rows -> GEMM, executed by one wave per 16 rows with
 // the intermediate matrices kept in registers (members: [gemm1, row members..., gemm2, epilogue members...])
-enum class NodeKind { kCluster, kGemm, kAttention };
+// kOperator: one of the custom calls of hlo::OperatorConfig, a stage of its own (one member)
+enum class NodeKind { kCluster, kGemm, kAttention, kOperator };
 
 struct GemmDesc {
   int64_t batch = 1, M = 0, N = 0, K = 0;
@@ -150,6 +151,10 @@ struct Program {
   // hand-over stays inside that XCD's L2
   mutable std::set<const hlo::Instr*> regional_roots;
   std::vector<const hlo::Instr*> live_outs;                        // storage roots, root-tuple order
+  // results of an operator that updates an operand in place -> the entry parameter whose buffer holds them
+  std::map<const hlo::Instr*, const hlo::Instr*> in_place;
+  // bytes of temp values whose size the shape does not tell (the parts of a paged attention)
+  std::map<const hlo::Instr*, int64_t> temp_size;
   std::map<const hlo::Instr*, int> producer;                       // storage root -> node id
   int num_stages = 0;
   int64_t temp_bytes = 0;
@@ -173,6 +178,7 @@ struct BuildOptions {
   // bias / residual epilogue moves into the consuming row program together with the sum over the heads
   bool fuse_attention_out_proj = false;
   std::map<std::string, int> gemm_split_k;   // GEMM instruction (canonical name) -> k split over workgroups
+  int grid = 256, waves = 4;            // workgroups of the launch and waves of a workgroup
   bool reuse_temp_slots = true;         // false: every temp value gets its own address (written once per launch)
   std::set<std::string> disabled_passes;   // MONONN_OPTIMIZATION_DISABLED_PASS (config.cc:82-86)
 };

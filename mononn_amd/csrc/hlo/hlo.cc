@@ -2,6 +2,8 @@
 
 #include <algorithm>
 #include <cctype>
+#include <cmath>
+#include <cstdint>
 #include <cstdlib>
 #include <set>
 #include <sstream>
@@ -351,6 +353,117 @@ void decode_lt_matmul_config(Instr* ins) {
     Shape arr = ins->shape.tuple[0];
     ins->shape = arr;
     ins->lt_tuple_result = true;
+  }
+}
+
+// Shapes and fields of the operators of OperatorConfig.  What a kernel of this package cannot do is refused here, with
+// the operand it is about.
+void decode_operator_config(Instr* ins) {
+  OperatorConfig& c = ins->oper;
+  const std::string& target = ins->custom_call_target;
+  if (target == "mononn$rope") c.kind = OperatorConfig::kRope;
+  else if (target == "mononn$kv_append") c.kind = OperatorConfig::kKvAppend;
+  else if (target == "mononn$paged_attention") c.kind = OperatorConfig::kPagedAttention;
+  else c.kind = OperatorConfig::kMatvecW4;
+  auto refuse_unless = [&](bool ok, const char* what) { MONONN_CHECK(ok, kInvalidArgument) << ins->hlo_name << " (" << target << "): " << what; };
+  auto supported = [&](bool ok, const char* what) { MONONN_CHECK(ok, kUnsupported) << ins->hlo_name << " (" << target << "): " << what; };
+  auto it = ins->attrs.find("backend_config");
+  if (it != ins->attrs.end() && !it->second.empty()) {
+    Json j = Json::parse(it->second);
+    if (j.contains("amplitude")) c.amplitude = j.at("amplitude").as_double();
+    if (j.contains("interleaved")) c.interleaved = j.at("interleaved").as_bool();
+    if (j.contains("scale")) c.scale = j.at("scale").as_double();
+    if (j.contains("window")) c.window = j.at("window").as_int();
+  }
+  refuse_unless(std::isfinite(c.amplitude) && std::isfinite(c.scale), "amplitude and scale must be finite");
+  refuse_unless(c.window >= 0 && c.window <= INT32_MAX, "window must be 0 (all keys) or a positive number of keys");
+  const size_t n = ins->operands.size();
+  for (auto* o : ins->operands) {
+    refuse_unless(!o->shape.is_tuple() && o->shape.num_elements() >= 1, "operands must be arrays of at least one element");
+    supported(!o->is_scalar_constant(), "an operand is a one-element constant written in the text, which has no buffer");
+  }
+  auto dims = [&](size_t i) -> const std::vector<int64_t>& { return ins->operands[i]->shape.dims; };
+  auto type = [&](size_t i) { return ins->operands[i]->shape.dtype; };
+  auto is = [&](size_t i, DType t, size_t rank, const char* what) { refuse_unless(type(i) == t && dims(i).size() == rank, what); };
+  auto float_type = [&](size_t i, bool f32) { supported(hlo::is_half_float(type(i)) || (f32 && type(i) == DType::kF32), f32 ? "elements must be f16, bf16 or f32" : "elements must be f16 or bf16"); };
+  auto result = [&](const Shape& s, DType t, const std::vector<int64_t>& d) { refuse_unless(!s.is_tuple() && s.dtype == t && s.dims == d, "the result's shape does not follow from the operands"); };
+  auto rotary = [&](size_t i, int64_t head) {
+    is(i, DType::kF32, 1, "inv_freq must be f32[rotated / 2]");
+    refuse_unless(2 * dims(i)[0] <= head, "inv_freq has more pairs than a head");
+  };
+  auto small = [&](int64_t v) { return v <= INT32_MAX; };
+  switch (c.kind) {
+    case OperatorConfig::kRope: {
+      refuse_unless(n == 3, "takes (x, positions, inv_freq)");
+      refuse_unless(dims(0).size() == 3, "x must be [tokens, heads, head size]");
+      float_type(0, true);
+      is(1, DType::kS32, 1, "positions must be s32[tokens]");
+      refuse_unless(dims(1)[0] == dims(0)[0], "one position per token");
+      rotary(2, dims(0)[2]);
+      supported(dims(0)[2] <= 1024, "head size above 1024");
+      supported(small(dims(0)[0]), "too many tokens");
+      result(ins->shape, type(0), dims(0));
+      break;
+    }
+    case OperatorConfig::kKvAppend: {
+      refuse_unless(n == 7 || n == 8, "takes (k, v, k_cache, v_cache, page_table, query_start, context_len[, inv_freq])");
+      refuse_unless(dims(0).size() == 3 && dims(1) == dims(0) && type(1) == type(0), "k and v must share a type and a shape [tokens, heads, head size]");
+      float_type(0, true);
+      for (size_t i : {size_t(2), size_t(3)})
+        refuse_unless(type(i) == type(0) && dims(i).size() == 4 && dims(i)[2] == dims(0)[1] && dims(i)[3] == dims(0)[2], "the caches must be [pages, page size, heads, head size] of the type of k");
+      refuse_unless(dims(3) == dims(2), "the caches must share a shape");
+      is(4, DType::kS32, 2, "page_table must be s32[sequences, pages of a sequence]");
+      is(5, DType::kS32, 1, "query_start must be s32[sequences + 1]");
+      is(6, DType::kS32, 1, "context_len must be s32[sequences]");
+      refuse_unless(dims(5)[0] == dims(4)[0] + 1 && dims(6)[0] == dims(4)[0], "page_table, query_start and context_len disagree about the number of sequences");
+      if (n == 8) rotary(7, dims(0)[2]);
+      supported(dims(0)[2] <= 1024, "head size above 1024");
+      supported(small(dims(0)[0]) && small(dims(2)[0]) && small(dims(4)[1] * dims(2)[1]) && small(dims(4)[0]), "too many tokens, pages, sequences or keys of a sequence");
+      refuse_unless(ins->shape.is_tuple() && ins->shape.tuple.size() == 2, "yields (k_cache, v_cache)");
+      result(ins->shape.tuple[0], type(2), dims(2));
+      result(ins->shape.tuple[1], type(3), dims(3));
+      // updated in place: nothing else may look at the values from before the call
+      for (size_t i : {size_t(2), size_t(3)})
+        supported(ins->operands[i]->opcode == "parameter" && ins->operands[i]->shape.minor_to_major == [&] {
+          std::vector<int> m;
+          for (int k = 3; k >= 0; --k) m.push_back(k);
+          return m;
+        }(), "the caches must be entry parameters in row-major order (they are updated in place)");
+      refuse_unless(ins->operands[2] != ins->operands[3], "k_cache and v_cache must be different parameters");
+      break;
+    }
+    case OperatorConfig::kPagedAttention: {
+      refuse_unless(n == 6, "takes (q, k_cache, v_cache, page_table, query_start, context_len)");
+      refuse_unless(dims(0).size() == 3, "q must be [tokens, heads, head size]");
+      float_type(0, false);
+      for (size_t i : {size_t(1), size_t(2)})
+        refuse_unless(type(i) == type(0) && dims(i).size() == 4 && dims(i)[3] == dims(0)[2], "the caches must be [pages, page size, heads, head size] of the type of q");
+      refuse_unless(dims(2) == dims(1), "the caches must share a shape");
+      refuse_unless(dims(0)[1] % dims(1)[2] == 0, "the number of query heads must be a multiple of the key heads");
+      is(3, DType::kS32, 2, "page_table must be s32[sequences, pages of a sequence]");
+      is(4, DType::kS32, 1, "query_start must be s32[sequences + 1]");
+      is(5, DType::kS32, 1, "context_len must be s32[sequences]");
+      refuse_unless(dims(4)[0] == dims(3)[0] + 1 && dims(5)[0] == dims(3)[0], "page_table, query_start and context_len disagree about the number of sequences");
+      supported(dims(0)[2] % 16 == 0 && dims(0)[2] <= 256, "the head size must be a multiple of 16 up to 256");
+      supported(small(dims(0)[0] * dims(0)[1]) && small(dims(1)[0]) && small(dims(3)[1] * dims(1)[1] + 4096), "too many tokens, pages or keys of a sequence");
+      // steps of the whole call are counted in 32 bits: 32 rows and 32 keys at least per step
+      supported((dims(0)[0] * dims(0)[1] / 32 + dims(1)[2] * (dims(3)[0] + 1)) * (dims(3)[1] * dims(1)[1] / 32 + 2) <= INT32_MAX, "too many tokens times keys");
+      result(ins->shape, type(0), dims(0));
+      break;
+    }
+    default: {
+      refuse_unless(n == 3 || n == 4, "takes (x, weight, scales[, zeros])");
+      refuse_unless(dims(0).size() == 2, "x must be [rows, columns]");
+      float_type(0, false);
+      is(1, DType::kU8, 2, "weight must be u8[rows, columns / 2]");
+      refuse_unless(dims(1)[1] * 2 == dims(0)[1], "weight must hold two values to a byte for every column of x");
+      refuse_unless(type(2) == type(0) && dims(2).size() == 2 && dims(2)[0] == dims(1)[0] && dims(0)[1] % dims(2)[1] == 0, "scales must be [weight rows, groups] of the type of x");
+      if (n == 4) refuse_unless(type(3) == DType::kU8 && dims(3) == dims(2), "zeros must be u8 of the shape of scales");
+      const int64_t group = dims(0)[1] / dims(2)[1];
+      supported(group == 32 || group == 64 || group % 128 == 0, "the group size must be 32, 64 or a multiple of 128");
+      supported(small(dims(0)[0]) && small(dims(0)[1]) && small(dims(1)[0]), "too many rows or columns");
+      result(ins->shape, type(0), {dims(0)[0], dims(1)[0]});
+    }
   }
 }
 
@@ -733,6 +846,9 @@ void decode_attrs(Instr* ins, Module* mod) {
       decode_lt_matmul_config(ins);
     } else if (ins->custom_call_target == "__cudnn$convForward") {
       decode_conv_config(ins);
+    } else if (ins->custom_call_target == "mononn$rope" || ins->custom_call_target == "mononn$kv_append" || ins->custom_call_target == "mononn$paged_attention" ||
+               ins->custom_call_target == "mononn$matvec_w4") {
+      decode_operator_config(ins);
     } else {
       // any other target aborts in the reference (core/op/custom_call.cc:96-100)
       MONONN_FAIL(kUnsupported) << ins->hlo_name << ": custom-call target '" << ins->custom_call_target << "' is not supported";
@@ -1101,6 +1217,41 @@ void lower_lt_matmul_epilogues(Module* mod) {
   }
 }
 
+// A paged_attention call becomes two instructions, each a stage of its own: the parts, f32[2 x workgroups, floats of a
+// part] (sized by the code generator, which knows the launch), and the call, which joins them.
+void split_paged_attention(Module* mod) {
+  Computation* comp = mod->entry;
+  for (size_t at = 0; at < comp->instrs.size(); ++at) {
+    Instr* call = comp->instrs[at].get();
+    if (call->oper.kind != OperatorConfig::kPagedAttention) continue;
+    auto up = std::make_unique<Instr>();
+    Instr* parts = up.get();
+    parts->name = call->name + "_parts";
+    parts->hlo_name = call->hlo_name + ".parts";
+    parts->opcode = "custom-call";
+    parts->custom_call_target = call->custom_call_target;
+    parts->oper = call->oper;
+    parts->oper.kind = OperatorConfig::kPagedAttentionParts;
+    parts->shape.dtype = DType::kF32;
+    parts->shape.dims = {1};
+    parts->shape.minor_to_major = {0};
+    parts->parent = comp;
+    parts->operands = call->operands;
+    for (auto* o : call->operands) {
+      auto& u = o->users;
+      u.erase(std::remove(u.begin(), u.end(), call), u.end());
+    }
+    for (auto* o : parts->operands)
+      if (std::find(o->users.begin(), o->users.end(), parts) == o->users.end()) o->users.push_back(parts);
+    call->operands = {parts, parts->operands[4], parts->operands[5]};
+    for (auto* o : call->operands)
+      if (std::find(o->users.begin(), o->users.end(), call) == o->users.end()) o->users.push_back(call);
+    comp->instrs.insert(comp->instrs.begin() + static_cast<long>(at), std::move(up));
+    ++at;
+  }
+  for (size_t i = 0; i < comp->instrs.size(); ++i) comp->instrs[i]->index_in_comp = static_cast<int>(i);
+}
+
 std::unique_ptr<Module> parse_module(const std::string& text) {
   auto mod = std::make_unique<Module>();
   Lexer lx(text);
@@ -1229,6 +1380,19 @@ std::unique_ptr<Module> parse_module(const std::string& text) {
     normalize_layouts(comp.get(), &layout_transposes);
     if (!layout_transposes.empty()) fold_layout_transposes_into_gemms(comp.get(), &layout_transposes);
   }
+  for (auto& comp : mod->computations)
+    for (auto& ins : comp->instrs) {
+      if (!ins->is_operator()) continue;
+      MONONN_CHECK(comp->is_entry, kUnsupported) << ins->hlo_name << ": " << ins->custom_call_target << " must be called from the entry computation";
+      if (ins->oper.kind == OperatorConfig::kKvAppend)
+        for (size_t i : {size_t(2), size_t(3)}) {
+          MONONN_CHECK(ins->operands[i]->opcode == "parameter" && std::count_if(ins->operands[i]->users.begin(), ins->operands[i]->users.end(), [&](Instr* u) { return u != ins.get(); }) == 0 &&
+                           std::count(ins->operands.begin(), ins->operands.end(), ins->operands[i]) == 1,
+                       kUnsupported)
+              << ins->hlo_name << ": the cache " << ins->operands[i]->hlo_name << " is updated in place and may be read by nothing else than this call; read its result instead";
+        }
+    }
+  split_paged_attention(mod.get());
   return mod;
 }
 

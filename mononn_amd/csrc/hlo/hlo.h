@@ -64,6 +64,24 @@ struct ConvConfig {
   double result_scale = 1;
 };
 
+// Operators of a decoding step over a paged key / value cache, custom calls of this package's own (no counterpart in
+// the reference): operands, shapes and backend_config fields are checked by decode_operator_config.
+//   mononn$rope             (x[T,H,D], positions s32[T], inv_freq f32[R/2]) -> [T,H,D]
+//   mononn$kv_append        (k[T,H,D], v[T,H,D], k_cache[P,S,H,D], v_cache[P,S,H,D], page_table s32[B,W],
+//                            query_start s32[B+1], context_len s32[B][, inv_freq f32[R/2]]) -> (k_cache, v_cache), in place
+//   mononn$paged_attention  (q[T,HQ,D], k_cache, v_cache, page_table, query_start, context_len) -> [T,HQ,D]
+//   mononn$matvec_w4        (x[M,K], weight u8[N,K/2], scales[N,K/group][, zeros u8[N,K/group]]) -> [M,N]
+// kPagedAttentionParts is what the parser splits off a paged_attention call: the stage that works through the keys and
+// leaves partial results, which the call itself then joins.
+struct OperatorConfig {
+  enum Kind { kNone, kRope, kKvAppend, kPagedAttention, kPagedAttentionParts, kMatvecW4 };
+  Kind kind = kNone;
+  double amplitude = 1;      // rope, kv_append: factor on cosine and sine
+  bool interleaved = false;  // rope, kv_append: pairs (2i, 2i+1) instead of (i, i + R/2)
+  double scale = 1;          // paged_attention: factor on the scores
+  int64_t window = 0;        // paged_attention: keys a query sees, itself included; 0 = all before it
+};
+
 struct Instr {
   std::string name;            // canonical: '.' and '-' replaced by '_' (string_helpers.cc:22-32)
   std::string hlo_name;        // as written in the text
@@ -96,6 +114,8 @@ struct Instr {
   std::string custom_call_target;
   GemmConfig gemm;
   ConvConfig conv;
+  OperatorConfig oper;
+  bool is_operator() const { return oper.kind != OperatorConfig::kNone; }
   bool is_conv() const { return opcode == "custom-call" && custom_call_target == "__cudnn$convForward"; }
   // a dense contraction with a decoded GemmConfig: the cuBLAS custom call, or a plain `dot` (what a stock XLA
   // prints before its GEMM rewriter has run)

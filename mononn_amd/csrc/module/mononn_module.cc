@@ -405,7 +405,7 @@ void MonoNNModule::launch_static_temp(void* const* device_ptrs, size_t n, void* 
   void* vals[kMaxArgs];
   void* args[kMaxArgs];
   for (size_t i = 0; i < n; ++i) {
-    MONONN_CHECK(device_ptrs[i] != nullptr, kInvalidArgument) << "buffer " << i << " is null";
+    MONONN_CHECK(device_ptrs[i] != nullptr || updated_in_place(i), kInvalidArgument) << "buffer " << i << " is null";
     MONONN_CHECK(reinterpret_cast<uintptr_t>(device_ptrs[i]) % 16 == 0, kInvalidArgument) << "buffer " << i << " is not 16-byte aligned";
     vals[i] = device_ptrs[i];
     args[i] = &vals[i];
@@ -476,10 +476,15 @@ double MonoNNModule::read_stage_clock(std::vector<unsigned long long>* ticks, in
   return dev_.wall_clock_ticks_per_us();
 }
 
+bool MonoNNModule::updated_in_place(size_t argument) const {
+  const size_t np = hip_.param_bytes.size();
+  return argument >= np && argument - np < hip_.liveout_parameter.size() && hip_.liveout_parameter[argument - np] >= 0;
+}
+
 void MonoNNModule::prepare_args(std::vector<void*>& vals) const {
   const size_t n = vals.size();
   for (size_t i = 0; i < n; ++i) {
-    MONONN_CHECK(vals[i] != nullptr || (i + 1 == n && hip_.temp_bytes == 0), kInvalidArgument) << "buffer " << i << " is null";
+    MONONN_CHECK(vals[i] != nullptr || (i + 1 == n && hip_.temp_bytes == 0) || updated_in_place(i), kInvalidArgument) << "buffer " << i << " is null";
     MONONN_CHECK(reinterpret_cast<uintptr_t>(vals[i]) % 16 == 0, kInvalidArgument) << "buffer " << i << " is not 16-byte aligned";
   }
 }

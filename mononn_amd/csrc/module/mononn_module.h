@@ -78,6 +78,8 @@ class MonoNNModule {
   std::string cluster_dir(const std::string& dump_dir) const;
 
  private:
+  // the slot of a live-out whose buffer is an entry parameter's
+  bool updated_in_place(size_t argument) const;
   void prepare_args(std::vector<void*>& vals) const;
   void upload_constant(const codegen::ConstantInfo& ci, const std::vector<char>& payload);
   std::string hlo_text_;

@@ -481,7 +481,10 @@ std::unique_ptr<MonoNNModule> MonoNNModuleTuner::tune(const TuneParams& params) 
         }
       if (clock_len > 0) tu += clock_decl + std::to_string(clock_len) + "];\n";
       for (size_t i : live) tu += "namespace cand_" + std::to_string(i) + " {\n" + trials[i].mod->hip_program().body + "}\n";
-      files["headers.h"] = trials[live[0]].mod->hip_program().files.at("headers.h");
+      for (const char* h : {"headers.h", "operators.h"}) {
+        auto it = trials[live[0]].mod->hip_program().files.find(h);
+        if (it != trials[live[0]].mod->hip_program().files.end()) files[h] = it->second;
+      }
       files["main.hip"] = tu;
       auto res = runtime::compile_hip(files, "main.hip", props.arch);
       runtime::DeviceModule dm;

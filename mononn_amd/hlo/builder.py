@@ -19,7 +19,7 @@ import json
 from dataclasses import dataclass
 from typing import Callable, Dict, List, Optional, Sequence, Tuple
 
-DTYPE_BYTES = {"pred": 1, "s8": 1, "u8": 1, "s16": 2, "u16": 2, "f16": 2, "s32": 4,
+DTYPE_BYTES = {"pred": 1, "s8": 1, "u8": 1, "s16": 2, "u16": 2, "f16": 2, "bf16": 2, "s32": 4,
                "u32": 4, "f32": 4, "s64": 8, "u64": 8, "f64": 8}
 
 
@@ -368,6 +368,58 @@ class Computation:
         self.root = v
         self.root_is_tuple = False
         return v
+
+    # -- operators of a decoding step over a paged cache ----------------------------------------
+    def _operator(self, target: str, dtype: str, dims: Sequence[int], operands: Sequence[Value], config: dict) -> Value:
+        cfg = json.dumps(config, separators=(",", ":")).replace('"', '\\"')
+        return self._emit("custom-call", dtype, dims, operands, attrs=f'custom_call_target="mononn${target}", backend_config="{cfg}"', name_hint="mononn-" + target.replace("_", "-"))
+
+    def rope(self, x: Value, positions: Value, inv_freq: Value, interleaved: bool = False, amplitude: float = 1.0) -> Value:
+        """`mononn$rope`: the first 2 * len(inv_freq) elements of every head of x [tokens, heads, head size] (f16, bf16 or
+        f32) are turned by positions [tokens] (s32): pair i by the angle position * inv_freq[i] (f32), cosine and sine
+        times `amplitude`.  Pairs are (i, i + rotated / 2), or (2 i, 2 i + 1) when `interleaved`; the rest of the head is
+        copied.  Frequencies of a longer context (`models.rope_frequencies`) go into inv_freq."""
+        return self._operator("rope", x.dtype, x.dims, [x, positions, inv_freq], {"interleaved": bool(interleaved), "amplitude": float(amplitude)})
+
+    def kv_append(self, k: Value, v: Value, k_cache: Value, v_cache: Value, page_table: Value, query_start: Value, context_len: Value,
+                  inv_freq: Optional[Value] = None, interleaved: bool = False, amplitude: float = 1.0) -> Tuple[Value, Value]:
+        """`mononn$kv_append`: keys and values [tokens, heads, head size] (f16, bf16 or f32) of new tokens go into the paged
+        caches [pages, page size, heads, head size], which are updated in place: they must be entry parameters, nothing
+        else may read them, and the two values returned are the caches afterwards, in the parameters' buffers.
+        Tokens query_start[b] .. query_start[b + 1] - 1 (s32, ascending) are the last ones of sequence b, which then has
+        context_len[b] keys (s32); position p of it lies in row p % page size of page page_table[b, p // page size]
+        (s32).  With inv_freq the keys are turned by their positions on the way, as by `rope`.  Tokens of no sequence,
+        negative positions, positions behind the table and pages outside the pool are left out; no two tokens of a call
+        may share a row."""
+        cfg = json.dumps({"interleaved": bool(interleaved), "amplitude": float(amplitude)}, separators=(",", ":")).replace('"', '\\"')
+        name = self.module.fresh("mononn-kv-append")
+        tshape = f"({k_cache.shape_str}, {v_cache.shape_str})"
+        operands = [k, v, k_cache, v_cache, page_table, query_start, context_len] + ([inv_freq] if inv_freq is not None else [])
+        self.lines.append(f"%{name} = {tshape} custom-call({', '.join(o.operand_str for o in operands)}), custom_call_target=\"mononn$kv_append\", backend_config=\"{cfg}\"")
+        out = []
+        for i, c in enumerate((k_cache, v_cache)):
+            g = self.module.fresh("get-tuple-element")
+            self.lines.append(f"%{g} = {c.shape_str} get-tuple-element({tshape} %{name}), index={i}")
+            out.append(Value(g, c.dtype, c.dims))
+        self.root = out[-1]
+        self.root_is_tuple = False
+        return out[0], out[1]
+
+    def paged_attention(self, q: Value, k_cache: Value, v_cache: Value, page_table: Value, query_start: Value, context_len: Value,
+                        scale: float, window: int = 0) -> Value:
+        """`mononn$paged_attention`: soft-max attention of new tokens q [tokens, query heads, head size] (f16 or bf16) over
+        paged caches laid out as for `kv_append`, which hold the new tokens already: token i of the n new ones of
+        sequence b sees keys 0 .. context_len[b] - n + i, with `window` > 0 the last `window` of these.  Query head h
+        reads key head h * key heads // query heads; scores are multiplied by `scale`.  Rows that see no key, and tokens
+        of no sequence, are zero.  Cells behind a sequence's last key may hold anything; the cells of its keys must
+        hold finite numbers."""
+        return self._operator("paged_attention", q.dtype, q.dims, [q, k_cache, v_cache, page_table, query_start, context_len], {"scale": float(scale), "window": int(window)})
+
+    def matvec_w4(self, x: Value, weight: Value, scales: Value, zeros: Optional[Value] = None) -> Value:
+        """`mononn$matvec_w4`: x [rows, k] (f16 or bf16) times the transpose of a matrix in 4 bits: weight u8[n, k / 2], two
+        values to a byte, the low half first; scales [n, groups] of x's type and zeros u8[n, groups] (8 without it), one
+        of each for k / groups consecutive columns: w[n, k] = (value - zero) * scale."""
+        return self._operator("matvec_w4", x.dtype, (x.dims[0], weight.dims[0]), [x, weight, scales] + ([zeros] if zeros is not None else []), {})
 
     def set_tuple_root(self, values: Sequence[Value]):
         name = self.module.fresh("tuple")

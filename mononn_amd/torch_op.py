@@ -35,6 +35,7 @@ class MonoNNFunction:
         info = module.buffer_info()
         self._param_bytes = info["parameters"]
         self._out_bytes = info["liveouts"]
+        self._in_place = module.liveout_parameters()   # live-outs that are an input tensor, updated by the call
         assert len(self._out_bytes) == len(self.outputs), "one {dtype, dims} entry per live-out is required"
         self._temp = None if module.owns_temp else torch.zeros(max(info["temp"], 256), dtype=torch.uint8, device=self.device)
         self.handle = id(self)
@@ -47,15 +48,21 @@ class MonoNNFunction:
         assert len(inputs) == len(self._param_bytes), f"expected {len(self._param_bytes)} tensors"
         held = []
         ptrs = []
-        for t, nbytes in zip(inputs, self._param_bytes):
+        for i, (t, nbytes) in enumerate(zip(inputs, self._param_bytes)):
             assert t.is_cuda and t.device == self.device, "inputs must live on the module's GPU"
+            assert t.is_contiguous() or i not in self._in_place, "an input that the call updates in place must be contiguous"
             t = t.contiguous()
             assert t.numel() * t.element_size() == nbytes, f"parameter needs {nbytes} bytes, got {t.numel() * t.element_size()}"
             assert t.data_ptr() % 16 == 0, "buffers must be 16-byte aligned"
             held.append(t)
             ptrs.append(t.data_ptr())
         outs = []
-        for o, nbytes in zip(self.outputs, self._out_bytes):
+        for o, nbytes, param in zip(self.outputs, self._out_bytes, self._in_place):
+            if param >= 0:
+                assert held[param].dtype == _TORCH_DTYPE[o["dtype"]] and list(held[param].shape) == list(o["dims"]), "an input that the call updates in place must have the declared type and shape"
+                outs.append(held[param])
+                ptrs.append(0)
+                continue
             t = torch.empty(o["dims"], dtype=_TORCH_DTYPE[o["dtype"]], device=self.device)
             assert t.numel() * t.element_size() == nbytes
             outs.append(t)
