@@ -51,7 +51,15 @@ class ModelFixture:
         out = {}
         for name, meta in self.constants.items():
             role, dims = meta["role"], meta["dims"]
-            if role.endswith("/bias") or role.endswith("/beta"):
+            if meta["dtype"] == "u8":   # 4-bit weights two to a byte, or their zero points
+                out[name] = rng.integers(0, 256, dims, dtype=np.uint8) if role.endswith("/weight_4bit") else rng.integers(6, 11, dims, dtype=np.uint8)
+                continue
+            if meta["dtype"] == "f32" and role.endswith("/inv_freq"):
+                out[name] = rope_frequencies(2 * dims[0])
+                continue
+            if role.endswith("/scales"):   # weights of about the spread of the others: a uniform 4-bit value deviates by 4.6
+                a = rng.uniform(0.003, 0.006, dims)
+            elif role.endswith("/bias") or role.endswith("/beta"):
                 a = rng.normal(0.0, 0.05, dims) if init == "random" else np.zeros(dims)
             elif role.endswith("/gamma"):
                 a = 1.0 + rng.normal(0.0, 0.1, dims) if init == "random" else np.ones(dims)
@@ -76,6 +84,8 @@ class ModelFixture:
                 a = _host_array(np.zeros(dims), p["dtype"])
             elif kind == "normal":
                 a = _host_array(rng.normal(0.0, 1.0, dims), p["dtype"])
+            elif kind == "values":
+                a = np.array(p["values"], NP_DTYPE[p["dtype"]]).reshape(dims)
             elif kind == "uniform_pm1":
                 a = _host_array(rng.uniform(-1.0, 1.0, dims), p["dtype"])
             else:
@@ -374,6 +384,111 @@ def gpt2(L=12, B=4, S=512, H=768, NH=12, F=3072, vocab=50257, max_pos=1024, eps=
         [{"name": "input_ids", "dtype": "s32", "dims": [B, S], "kind": "token_ids", "vocab": vocab}],
         mb.constants, [{"dtype": _FT, "dims": [B, S, vocab]}],
         dict(B=B, S=S, H=H, NH=NH, F=F, L=L, vocab=vocab, eps=eps))
+
+
+def rope_frequencies(rotary: int, base: float = 10000.0, stretch: float = 1.0, method: str = "linear", original_context: int = 4096,
+                     fast_turns: float = 32.0, slow_turns: float = 1.0) -> np.ndarray:
+    """f32[rotary / 2] angles per position for `Computation.rope` / `kv_append`: base ** (-2 i / rotary), for contexts
+    `stretch` times longer than a model was trained on slowed down by `method`:
+      linear   all frequencies divided by stretch (positions interpolated)
+      base     the base raised so that the lowest frequency is divided by stretch and the highest kept
+      by_turns frequencies that make more than fast_turns turns in original_context kept, those with fewer than
+               slow_turns divided by stretch, linear in the number of turns between (the factor on cosine and sine that
+               goes with it, 0.1 ln(stretch) + 1, is the operator's `amplitude`)"""
+    assert rotary >= 2 and rotary % 2 == 0 and stretch >= 1.0
+    i = np.arange(rotary // 2, dtype=np.float64)
+    if method == "base":
+        assert rotary > 2, "one pair has no range of frequencies"
+        return ((base * stretch ** (rotary / (rotary - 2.0))) ** (-2.0 * i / rotary)).astype(np.float32)
+    f = base ** (-2.0 * i / rotary)
+    if method == "linear":
+        return (f / stretch).astype(np.float32)
+    assert method == "by_turns", method
+    turns = original_context * f / (2.0 * math.pi)
+    keep = np.clip((turns - slow_turns) / (fast_turns - slow_turns), 0.0, 1.0)
+    return (f * (keep + (1.0 - keep) / stretch)).astype(np.float32)
+
+
+def gpt2_step(new_tokens=(1, 1, 1, 1), cached=(100, 37, 200, 5), L=12, H=768, NH=12, NKV=None, F=3072, vocab=50257, max_pos=1024, page=16, width=None,
+              rotary=False, weights_4bit=0, eps=1e-5) -> ModelFixture:
+    """One step of the `gpt2` decoder over a paged key / value cache: new_tokens[b] tokens of every sequence b, packed,
+    behind the cached[b] it already has; a prompt is such a step with nothing cached, decoding one with one token each.
+    Per layer the new keys and values are appended to that layer's caches (parameters, updated in place, and results
+    beside the logits) and the new tokens attend over them: all layers in one kernel.  With learned positions, equal
+    heads and full weights it computes what `gpt2` computes for the same tokens.  NKV < NH shares key heads between
+    query heads; `rotary` turns queries and keys instead of adding learned positions; weights_4bit = 32, 64 or a
+    multiple of 128 keeps the layers' matrices in 4 bits with that group size."""
+    NKV = NKV or NH
+    B, T, D = len(new_tokens), sum(new_tokens), H // NH
+    context = [n + c for n, c in zip(new_tokens, cached)]
+    width = width or max(1, max((c + page - 1) // page for c in context))
+    pages = B * width + 1
+    mb = HloModuleBuilder("cluster_0__XlaCompiledKernel_true__XlaNumConstantArgs_0_.1")
+    e = mb.entry
+    # pages of a sequence lie scattered over the pool
+    order = np.random.default_rng(len(context)).permutation(pages)[:B * width].reshape(B, width)
+    starts = np.concatenate([[0], np.cumsum(new_tokens)])
+    where = np.concatenate([np.arange(c - n, c) for n, c in zip(new_tokens, context)])
+    params = [{"name": "input_ids", "dtype": "s32", "dims": [T], "kind": "token_ids", "vocab": vocab},
+              {"name": "positions", "dtype": "s32", "dims": [T], "kind": "values", "values": where.tolist()},
+              {"name": "page_table", "dtype": "s32", "dims": [B, width], "kind": "values", "values": order.reshape(-1).tolist()},
+              {"name": "query_start", "dtype": "s32", "dims": [B + 1], "kind": "values", "values": starts.tolist()},
+              {"name": "context_len", "dtype": "s32", "dims": [B], "kind": "values", "values": context}]
+    cache_dims = (pages, page, NKV, D)
+    for l in range(L):
+        for n in ("k_cache", "v_cache"):
+            params.append({"name": f"{n}_{l}", "dtype": _FT, "dims": list(cache_dims), "kind": "normal"})
+    ids, positions, table, starts_v, context_v, *caches = [e.parameter(p["dtype"], p["dims"], p["name"]) for p in params]
+    wte = e.elided_constant(_FT, (vocab, H), "gpt2/wte")
+    wpe = None if rotary else e.elided_constant(_FT, (max_pos, H), "gpt2/wpe")
+    freq = e.elided_constant("f32", (D // 2,), "gpt2/inv_freq") if rotary else None
+
+    def emb_body(f, pi, pp, pw, *pe):
+        w = f.gather_rows(pw, pi)
+        if not pe:
+            return w
+        return f.convert(f.add(f.convert(w, "f32"), f.convert(f.gather_rows(pe[0], pp), "f32")), _FT)
+    h = e.fusion("kLoop", [ids, positions, wte] + ([wpe] if wpe is not None else []), emb_body)
+
+    def matrix(x, role, n):
+        """x times a constant [k, n] matrix, f16 or in 4 bits"""
+        k = x.dims[1]
+        if not weights_4bit:
+            return e.gemm(x, e.elided_constant(_FT, (k, n), role + "/kernel"), 1, 0)
+        w = e.elided_constant("u8", (n, k // 2), role + "/weight_4bit")
+        s = e.elided_constant(_FT, (n, k // weights_4bit), role + "/scales")
+        z = e.elided_constant("u8", (n, k // weights_4bit), role + "/zero_points")
+        return e.matvec_w4(x, w, s, z)
+
+    def bias(role, n):
+        return e.elided_constant(_FT, (n,), role + "/bias")
+
+    def heads(x, role, count):
+        g = matrix(x, role, count * D)
+        return e.bitcast(e.fusion("kLoop", [g, bias(role, count * D)], _bias_add_f16), (T, count, D))
+
+    results = []
+    for l in range(L):
+        p = f"gpt2/h_{l}"
+        vec = lambda role: e.elided_constant(_FT, (H,), f"{p}/{role}")
+        a = _layer_norm(e, mb, h, vec("attention/LayerNorm/gamma"), vec("attention/LayerNorm/beta"), eps)
+        q, k, v = heads(a, p + "/attention/query", NH), heads(a, p + "/attention/key", NKV), heads(a, p + "/attention/value", NKV)
+        if rotary:
+            q = e.rope(q, positions, freq)
+        kc, vc = e.kv_append(k, v, caches[2 * l], caches[2 * l + 1], table, starts_v, context_v, inv_freq=freq)
+        results += [kc, vc]
+        ctx = e.bitcast(e.paged_attention(q, kc, vc, table, starts_v, context_v, scale=1.0 / math.sqrt(D)), (T, H))
+        h = _residual_f16(e, matrix(ctx, p + "/attention/output", H), bias(p + "/attention/output", H), h)
+        m = _layer_norm(e, mb, h, vec("output/LayerNorm/gamma"), vec("output/LayerNorm/beta"), eps)
+        act = _ffn_act(e, matrix(m, p + "/intermediate", F), bias(p + "/intermediate", F))
+        h = _residual_f16(e, matrix(act, p + "/output", H), bias(p + "/output", H), h)
+    hf = _layer_norm(e, mb, h, e.elided_constant(_FT, (H,), "gpt2/ln_f/gamma"), e.elided_constant(_FT, (H,), "gpt2/ln_f/beta"), eps)
+    logits = e.gemm(hf, wte, 1, 1)
+    e.set_tuple_root([logits] + results)
+    return ModelFixture(
+        f"gpt2_step_L{L}_H{H}", mb.text(), params, mb.constants,
+        [{"dtype": _FT, "dims": [T, vocab]}] + [{"dtype": _FT, "dims": list(cache_dims)} for _ in results],
+        dict(B=B, T=T, H=H, NH=NH, NKV=NKV, F=F, L=L, vocab=vocab, page=page, pages=pages, eps=eps))
 
 
 def vit(L=12, B=8, image=224, patch=16, H=768, NH=12, F=3072, eps=1e-6) -> ModelFixture:

@@ -59,7 +59,7 @@ def stage_report(hlo_text: str, constants, inputs, outputs, spec_dir=None, launc
 
 def main(argv=None):
     ap = argparse.ArgumentParser(description=__doc__.split("\n\n")[0])
-    ap.add_argument("--model", choices=["bert_layer", "bert_base", "bert_large", "gpt2", "vit"])
+    ap.add_argument("--model", choices=["bert_layer", "bert_base", "bert_large", "gpt2", "gpt2_step", "vit"])
     ap.add_argument("--hlo", help="HLO text file (parameters are fed zeros)")
     ap.add_argument("--spec-dir")
     ap.add_argument("--csv")

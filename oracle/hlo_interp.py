@@ -74,6 +74,8 @@ from typing import Dict, List, Optional, Sequence
 
 import numpy as np
 
+from . import decoding
+
 _NP = {"pred": np.bool_, "s8": np.int8, "u8": np.uint8, "s16": np.int16, "u16": np.uint16,
        "s32": np.int32, "u32": np.uint32, "s64": np.int64, "u64": np.uint64,
        "f16": np.float16, "f32": np.float32, "f64": np.float64,
@@ -490,6 +492,8 @@ class Evaluator:
                 return self._conv_forward(ins, x)
             if target == "__cublas$lt$matmul":
                 return self._lt_matmul(ins, x, dt)
+            if target.startswith("mononn$"):
+                return self._decoding_operator(ins, target[len("mononn$"):], x, dt)
             raise NotImplementedError(f"custom-call target {target}")
         raise NotImplementedError(f"opcode {op}")
 
@@ -586,6 +590,20 @@ class Evaluator:
         with np.errstate(over="ignore"):
             return D.astype(dt, copy=False)
 
+
+    def _decoding_operator(self, ins: Instr, name: str, x, dt):
+        """The package's own custom calls, computed in 64 bits and rounded once to the result type."""
+        cfg = json.loads(ins.attrs["backend_config"][1:-1].replace('\\"', '"'))
+        if name == "rope":
+            return decoding.rope(x[0], x[1], x[2], cfg["interleaved"], cfg["amplitude"]).astype(dt)
+        if name == "kv_append":
+            caches = decoding.kv_append(*x[:7], x[7] if len(x) > 7 else None, cfg["interleaved"], cfg["amplitude"])
+            return tuple(c.astype(self.np_dtype(t.dtype)) for c, t in zip(caches, ins.shape.tuple_shapes))
+        if name == "paged_attention":
+            return decoding.paged_attention(*x, scale=cfg["scale"], window=cfg["window"]).astype(dt)
+        if name == "matvec_w4":
+            return decoding.matvec_w4(*x).astype(dt)
+        raise NotImplementedError(f"custom-call target mononn${name}")
 
     def _lt_matmul(self, ins: Instr, x, dt):
         """__cublas$lt$matmul(a, b[, c][, bias]), the newer spelling of the cuBLAS call.  The reference accepts only
