@@ -127,7 +127,9 @@ NodeFunction generate_operator(const graph::Program& prog, const graph::Node& no
         body << " static_assert(Attention::lds_bytes() == " << f.smem_bytes << ", \"LDS\");";
       } else {
         const std::string pp = input(0), sp = input(1), lp = input(2);
-        body << "Attention::join(unit, " << pp << ", " << sp << ", " << lp << ", " << ptrs.output(ins) << ");";
+        body << "Attention::join(unit, " << pp << ", " << sp << ", " << lp << ", " << ptrs.output(ins) << ", smem);";
+        f.smem_bytes = ls.waves() * 384 * 4;
+        body << " static_assert(Attention::join_lds_bytes() == " << f.smem_bytes << ", \"LDS\");";
       }
       check_units(grid);
       break;

@@ -207,7 +207,21 @@ __device__ __forceinline__ void kv_append_unit(int unit, const T* k, const T* v,
 // ---------------------------------------------------------------------------------------------
 // attention over the paged cache
 // ---------------------------------------------------------------------------------------------
-__device__ __forceinline__ float half_wave_other(float v) { return lane_xor(v, 32); }
+// the larger of, and the sum of, a lane's value and that of the lane 32 further on (one swap of half waves)
+__device__ __forceinline__ void half_waves(float v, float& a, float& b) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+  a = __builtin_bit_cast(float, (unsigned)r[0]), b = __builtin_bit_cast(float, (unsigned)r[1]);
+}
+__device__ __forceinline__ float half_waves_max(float v) {
+  float a, b;
+  half_waves(v, a, b);
+  return fmaxf(a, b);
+}
+__device__ __forceinline__ float half_waves_sum(float v) {
+  float a, b;
+  half_waves(v, a, b);
+  return a + b;
+}
 
 // The query rows of a sequence for one key / value head are its new tokens times the G = H / HKV query heads that
 // share it (row = token * G + head of the group), in tiles: ROWS = 32 per wave in a *wide* item, 32 in all in a
@@ -288,45 +302,55 @@ struct PagedAttention {
   }
   static __device__ __forceinline__ Sequence sequence(const int* qs, const int* cl, int b) { return sequence_at<TOKENS, MAX_KEYS>(qs, cl, b); }
 
-  // Sums over the sequences: lane l of a wave takes sequence l of every 64.
+  // Steps up to and with every sequence: lane l of a wave holds those of sequence l; behind the first 64 sequences
+  // they are added up again where they are needed.
+  struct Plan {
+    int total;          // steps of the call
+    int steps, upto;    // of the lane's sequence; of all sequences up to it
+  };
   static __device__ __forceinline__ int steps_of(const int* qs, const int* cl, int b) { return b < SEQS ? HKV * head_steps(sequence(qs, cl, b)) : 0; }
 #ifndef MONONN_ONE_THREAD
-  // steps of the whole call
-  static __device__ __forceinline__ int total_steps(const int* qs, const int* cl) {
-    int n = 0;
-    for (int base = 0; base < SEQS; base += kWaveSize) n += wave_all_reduce(steps_of(qs, cl, base + lane_id()), [](int a, int c) { return a + c; });
-    return __builtin_amdgcn_readfirstlane(n);
+  static __device__ __forceinline__ int sum_upto(int v) {
+#pragma unroll
+    for (int off = 1; off < kWaveSize; off <<= 1) {
+      const int o = __shfl_up(v, off, kWaveSize);
+      if (lane_id() >= off) v += o;
+    }
+    return v;
+  }
+  static __device__ __forceinline__ Plan plan(const int* qs, const int* cl) {
+    Plan p;
+    p.steps = steps_of(qs, cl, lane_id());
+    p.upto = sum_upto(p.steps);
+    p.total = __builtin_amdgcn_readlane(p.upto, kWaveSize - 1);
+    for (int base = kWaveSize; base < SEQS; base += kWaveSize)
+      p.total += __builtin_amdgcn_readfirstlane(wave_all_reduce(steps_of(qs, cl, base + lane_id()), [](int a, int c) { return a + c; }));
+    return p;
   }
   // the sequence that holds step `rem` of the call; `rem` becomes the step inside it
-  static __device__ __forceinline__ int sequence_with_step(const int* qs, const int* cl, int& rem) {
-    int found = SEQS - 1;
-    for (int base = 0; base < SEQS; base += kWaveSize) {
-      const int v = steps_of(qs, cl, base + lane_id());
-      int upto = v;   // inclusive sum over the lanes
-#pragma unroll
-      for (int off = 1; off < kWaveSize; off <<= 1) {
-        const int o = __shfl_up(upto, off, kWaveSize);
-        if (lane_id() >= off) upto += o;
-      }
+  static __device__ __forceinline__ int sequence_with_step(const Plan& p, const int* qs, const int* cl, int& rem) {
+    int steps = p.steps, upto = p.upto, base = 0;
+    for (;;) {
       const unsigned long long behind = __ballot(upto > rem);
       if (behind != 0) {
         const int l = __builtin_ctzll(behind);
-        found = base + l;
-        rem -= __shfl(upto - v, l, kWaveSize);
-        break;
+        rem -= __builtin_amdgcn_readlane(upto - steps, l);
+        return base + l < SEQS ? base + l : SEQS - 1;
       }
-      rem -= __shfl(upto, kWaveSize - 1, kWaveSize);
+      rem -= __builtin_amdgcn_readlane(upto, kWaveSize - 1);
+      base += kWaveSize;
+      if (base >= SEQS) return SEQS - 1;
+      steps = steps_of(qs, cl, base + lane_id());
+      upto = sum_upto(steps);
     }
-    rem = __builtin_amdgcn_readfirstlane(rem);
-    return __builtin_amdgcn_readfirstlane(clamp_int(found, 0, SEQS - 1));
   }
 #else   // for a host build that runs one thread at a time
-  static __device__ __forceinline__ int total_steps(const int* qs, const int* cl) {
-    int n = 0;
-    for (int b = 0; b < SEQS; ++b) n += steps_of(qs, cl, b);
-    return n;
+  static __device__ __forceinline__ Plan plan(const int* qs, const int* cl) {
+    Plan p = {0, 0, 0};
+    for (int b = 0; b < SEQS; ++b) p.total += steps_of(qs, cl, b);
+    return p;
   }
-  static __device__ __forceinline__ int sequence_with_step(const int* qs, const int* cl, int& rem) {
+  static __device__ __forceinline__ int sequence_with_step(const Plan&, const int* qs, const int* cl, int& rem) {
     for (int b = 0; b < SEQS; ++b) {
       if (rem < steps_of(qs, cl, b)) return b;
       rem -= steps_of(qs, cl, b);
@@ -335,10 +359,10 @@ struct PagedAttention {
   }
 #endif
   // the item that holds step `at` of the call (0 <= at < total_steps) and the step inside it
-  static __device__ __forceinline__ Item locate(const int* qs, const int* cl, int at, int& inside) {
+  static __device__ __forceinline__ Item locate(const Plan& p, const int* qs, const int* cl, int at, int& inside) {
     Item it;
     int rem = at;
-    it.b = sequence_with_step(qs, cl, rem);
+    it.b = sequence_with_step(p, qs, cl, rem);
     it.s = sequence(qs, cl, it.b);
     it.s.start = __builtin_amdgcn_readfirstlane(it.s.start);
     it.s.len = __builtin_amdgcn_readfirstlane(it.s.len);
@@ -359,21 +383,61 @@ struct PagedAttention {
     inside = clamp_int(rem, 0, it.steps - 1);
     return it;
   }
+  // the item behind `it`
+  static __device__ __forceinline__ void next_item(const int* qs, const int* cl, Item& it) {
+    if (it.tile + 1 < tiles_of(it.s.len)) ++it.tile;
+    else {
+      it.tile = 0;
+      if (it.h + 1 < HKV) ++it.h;
+      else {
+        it.h = 0;
+        do {
+          if (it.b + 1 >= SEQS) return;
+          ++it.b;
+          it.s = sequence(qs, cl, it.b);
+        } while (it.s.len == 0);
+        it.s.start = __builtin_amdgcn_readfirstlane(it.s.start);
+        it.s.len = __builtin_amdgcn_readfirstlane(it.s.len);
+        it.s.ctx = __builtin_amdgcn_readfirstlane(it.s.ctx);
+        it.narrow = is_narrow(it.s.len);
+      }
+    }
+    tile_steps(it.s, it.tile, it.first, it.steps);
+  }
   // Ranges follow each other inside an XCD (workgroup u runs on XCD u % 8 of an even deal): the tiles of one key head
   // then read its keys through the same L2.
   static __device__ __forceinline__ int range_of(int unit) { return GRID % kXcds == 0 ? unit % kXcds * (GRID / kXcds) + unit / kXcds : unit; }
   static __device__ __forceinline__ int range_begin(int total, int range) { return (int)((long)total * range / GRID); }
+  static __device__ __forceinline__ int range_with_step(int total, int step) { return (int)((((long)step + 1) * GRID + total - 1) / total) - 1; }
 
   // ---- loads -----------------------------------------------------------------------------------------------------
-  static __device__ __forceinline__ int page_of(const int* table, int b, int key) {
-    key = clamp_int(key, 0, MAX_KEYS - 1);
+  // The pieces of consecutive rows are dealt to the lanes in order.  Lane l fetches the page of row l of a step (one
+  // load, a step ahead); where the 64 / CPR rows of an instruction lie in one page its number is the same for the
+  // whole wave, and the rows' addresses are a scalar base and a lane offset that never changes.
+  static constexpr int kRowsPerRun = kWaveSize / CPR;
+  static constexpr bool kUniformRows = kWaveSize % CPR == 0 && PAGE % (kWaveSize / CPR) == 0;
+  static __device__ __forceinline__ int lane_page(const int* table, int b, int key0) {
+    const int key = clamp_int(key0 + lane_id(), 0, MAX_KEYS - 1);
     return clamp_int(table[(long)b * WIDTH + key / PAGE], 0, PAGES - 1);
   }
-  static __device__ __forceinline__ long row_offset(int page, int key, int h) {
-    key = clamp_int(key, 0, MAX_KEYS - 1);
-    return (((long)page * PAGE + key % PAGE) * HKV + h) * D;
-  }
   static __device__ __forceinline__ half8_t load_piece(const T* p) { return *reinterpret_cast<const half8_t*>(p); }
+  // piece (first_piece + lane) of the keys from key0 on; `pages`: lane_page of key0
+  static __device__ __forceinline__ void load_run_of_rows(const T* kc, const T* vc, int pages, int key0, int first_piece, int h, half8_t& k, half8_t& v) {
+    if constexpr (kUniformRows) {
+      const int row0 = first_piece / CPR, key = key0 + row0;
+      const int page = __builtin_amdgcn_readlane(pages, row0 & (kWaveSize - 1));
+      const long base = (((long)page * PAGE + key % PAGE) * HKV + h) * D;
+      const unsigned at = (unsigned)(lane_id() / CPR) * (HKV * D) + (unsigned)(lane_id() % CPR) * 8;
+      k = load_piece(kc + base + at);
+      v = load_piece(vc + base + at);
+    } else {
+      const int at = first_piece + lane_id(), row = at / CPR, key = key0 + row;
+      const int page = __shfl(pages, row & (kWaveSize - 1), kWaveSize);
+      const long off = (((long)page * PAGE + key % PAGE) * HKV + h) * D + at % CPR * 8;
+      k = load_piece(kc + off);
+      v = load_piece(vc + off);
+    }
+  }
 
   // the lane's query row: operand of the first product, and the keys it sees, [lo, hi]
   struct Rows {
@@ -409,7 +473,7 @@ struct PagedAttention {
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
     }
-    __device__ __forceinline__ void finish() { l += half_wave_other(l); }
+    __device__ __forceinline__ void finish() { l = half_waves_sum(l); }
   };
 
   // BLOCKS x 32 keys from LDS on 32 query rows.  `check`: some row does not see all of these keys.
@@ -439,9 +503,12 @@ struct PagedAttention {
     for (int b = 0; b < BLOCKS; ++b)
 #pragma unroll
       for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
-    top = fmaxf(top, half_wave_other(top)) * scale_log2;
-    const float m = fmaxf(st.m, top);
-    if (__any(m > st.m)) {   // the same for the whole wave
+    top = half_waves_max(top) * scale_log2;
+    // The reference of a query's exponentials only has to stay near its maximum: it moves, and what has been added up
+    // is rescaled, when some query of the wave has outgrown its own by 2^6 (probabilities up to 64 leave f16 and the
+    // sums room), which after the first steps is rare.
+    if (__any(top > st.m + 6.0f)) {
+      const float m = fmaxf(st.m, top);
       const float a = __builtin_amdgcn_exp2f(st.m - m);
       st.l *= a;
 #pragma unroll
@@ -457,7 +524,7 @@ struct PagedAttention {
     for (int b = 0; b < BLOCKS; ++b)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const float e = __builtin_amdgcn_exp2f(s[b][i] * scale_log2 - m);
+        const float e = __builtin_amdgcn_exp2f(s[b][i] * scale_log2 - st.m);
         sum += e;
         p[b][i / 8][i % 8] = __builtin_bit_cast(half_t, (T)e);
       }
@@ -498,26 +565,19 @@ struct PagedAttention {
 
   // ---- wide items ------------------------------------------------------------------------------------------------
   static constexpr int kRuns = (kWideKeys * CPR + MONONN_BLOCK_SIZE - 1) / MONONN_BLOCK_SIZE;   // pieces of K (and of V) a thread moves per step
-  static __device__ __forceinline__ void wide_pages(const int* table, const Item& it, int key0, int (&page)[kRuns]) {
+  static __device__ __forceinline__ int wide_piece(int run) { return (run * NW + __builtin_amdgcn_readfirstlane(wave_id())) * kWaveSize; }
+  static __device__ __forceinline__ void wide_load(const T* kc, const T* vc, int pages, int key0, int h, half8_t (&k)[kRuns], half8_t (&v)[kRuns]) {
 #pragma unroll
-    for (int i = 0; i < kRuns; ++i) page[i] = page_of(table, it.b, key0 + (thread_id() + i * MONONN_BLOCK_SIZE) / CPR);
+    for (int i = 0; i < kRuns; ++i) load_run_of_rows(kc, vc, pages, key0, wide_piece(i), h, k[i], v[i]);
   }
-  static __device__ __forceinline__ void wide_load(const T* kc, const T* vc, const Item& it, int key0, const int (&page)[kRuns], half8_t (&k)[kRuns], half8_t (&v)[kRuns]) {
-#pragma unroll
-    for (int i = 0; i < kRuns; ++i) {
-      const int at = thread_id() + i * MONONN_BLOCK_SIZE;
-      const long off = row_offset(page[i], key0 + at / CPR, it.h) + at % CPR * 8;
-      k[i] = load_piece(kc + off);
-      v[i] = load_piece(vc + off);
-    }
-  }
-  // rows behind the sequence's last key become zeros: whatever those cells hold, NaN included, must not reach 0 * v
+  // Rows behind the sequence's last key become zeros: whatever those cells hold, NaN included, must not reach 0 * v.
   static __device__ __forceinline__ void wide_store(char* buf, int key0, int ctx, const half8_t (&k)[kRuns], const half8_t (&v)[kRuns]) {
+    const bool all = key0 + kWideKeys <= ctx;
 #pragma unroll
     for (int i = 0; i < kRuns; ++i) {
-      const int at = thread_id() + i * MONONN_BLOCK_SIZE, row = at / CPR, c = at % CPR;
+      const int at = wide_piece(i) + lane_id(), row = at / CPR, c = at % CPR;
       if (kWideKeys * CPR % MONONN_BLOCK_SIZE != 0 && row >= kWideKeys) break;
-      const bool in = key0 + row < ctx;
+      const bool in = all || key0 + row < ctx;
       const half8_t zero = {0, 0, 0, 0, 0, 0, 0, 0};
       *reinterpret_cast<half8_t*>(buf + row * KP + c * 16) = in ? k[i] : zero;
       *reinterpret_cast<half8_t*>(buf + kWideKeys * KP + row * VP + c * 16) = in ? v[i] : zero;
@@ -536,11 +596,9 @@ struct PagedAttention {
     State st;
     st.clear();
     half8_t k[kRuns], v[kRuns];
-    int page[kRuns];
     const int begin = (it.first + from) * kWideKeys;
-    wide_pages(table, it, begin, page);
-    wide_load(kc, vc, it, begin, page, k, v);
-    wide_pages(table, it, begin + kWideKeys, page);
+    wide_load(kc, vc, lane_page(table, it.b, begin), begin, it.h, k, v);
+    int pages = lane_page(table, it.b, begin + kWideKeys);
     for (int i = 0; i < count; ++i) {
       const int key0 = begin + i * kWideKeys;
       char* buf = smem + turn * kWideBuffer;
@@ -548,8 +606,8 @@ struct PagedAttention {
       wide_store(buf, key0, it.s.ctx, k, v);
       __syncthreads();
       if (i + 1 < count) {
-        wide_load(kc, vc, it, key0 + kWideKeys, page, k, v);
-        wide_pages(table, it, key0 + 2 * kWideKeys, page);
+        wide_load(kc, vc, pages, key0 + kWideKeys, it.h, k, v);
+        pages = lane_page(table, it.b, key0 + 2 * kWideKeys);
       }
       const bool none = !live || key0 > p_last || (WINDOW > 0 && key0 + kWideKeys - 1 < p_first - WINDOW + 1);
       if (!none) {
@@ -573,14 +631,9 @@ struct PagedAttention {
 
   // ---- narrow items ----------------------------------------------------------------------------------------------
   static constexpr int kMine = CPR / 2;   // pieces of K (and of V) a lane moves per step: 32 rows over 64 lanes
-  static __device__ __forceinline__ void narrow_load(const T* kc, const T* vc, const int* table, const Item& it, int key0, half8_t (&k)[kMine], half8_t (&v)[kMine]) {
+  static __device__ __forceinline__ void narrow_load(const T* kc, const T* vc, int pages, int key0, int h, half8_t (&k)[kMine], half8_t (&v)[kMine]) {
 #pragma unroll
-    for (int i = 0; i < kMine; ++i) {
-      const int at = lane_id() + i * kWaveSize, key = key0 + at / CPR;
-      const long off = row_offset(page_of(table, it.b, key), key, it.h) + at % CPR * 8;
-      k[i] = load_piece(kc + off);
-      v[i] = load_piece(vc + off);
-    }
+    for (int i = 0; i < kMine; ++i) load_run_of_rows(kc, vc, pages, key0, i * kWaveSize, h, k[i], v[i]);
   }
   static __device__ __forceinline__ void narrow(const T* q, const T* kc, const T* vc, const int* table, T* out, float* part, const Item& it, int from, int count, bool whole,
                                                 float scale_log2, char* smem) {
@@ -597,18 +650,23 @@ struct PagedAttention {
       const int p_first = it.s.ctx - it.s.len, p_last = it.s.ctx - 1;
       half8_t k[kMine], v[kMine];
       const int begin = (it.first + from) * kNarrowKeys + wave * 32;
-      narrow_load(kc, vc, table, it, begin, k, v);
+      narrow_load(kc, vc, lane_page(table, it.b, begin), begin, it.h, k, v);
+      int pages = lane_page(table, it.b, begin + kNarrowKeys);
       for (int i = 0; i < count; ++i) {
         const int key0 = begin + i * kNarrowKeys;
+        const bool all = key0 + 32 <= it.s.ctx;
 #pragma unroll
         for (int j = 0; j < kMine; ++j) {
           const int at = lane_id() + j * kWaveSize, row = at / CPR, c = at % CPR;
-          const bool in = key0 + row < it.s.ctx;
+          const bool in = all || key0 + row < it.s.ctx;
           const half8_t zero = {0, 0, 0, 0, 0, 0, 0, 0};
           *reinterpret_cast<half8_t*>(kbuf + row * KP + c * 16) = in ? k[j] : zero;
           *reinterpret_cast<half8_t*>(vbuf + row * VP + c * 16) = in ? v[j] : zero;
         }
-        if (i + 1 < count) narrow_load(kc, vc, table, it, key0 + kNarrowKeys, k, v);
+        if (i + 1 < count) {
+          narrow_load(kc, vc, pages, key0 + kNarrowKeys, it.h, k, v);
+          pages = lane_page(table, it.b, key0 + 2 * kNarrowKeys);
+        }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();   // the wave's own rows: written above, read below
         const bool none = key0 > p_last || (WINDOW > 0 && key0 + 31 < p_first - WINDOW + 1);
@@ -667,68 +725,99 @@ struct PagedAttention {
         if (t < inside0 || t >= inside1)
           for (int c = thread_id(); c < H * CPR; c += MONONN_BLOCK_SIZE) store_run<COHERENT, T, 8>(out + (long)t * H * D + c * 8, zero);
     }
-    const int total = total_steps(qs, cl), range = range_of(unit);
-    const int end = range_begin(total, range + 1);
-    int at = range_begin(total, range), turn = 0;
+    const Plan p = plan(qs, cl);
+    const int range = range_of(unit), end = range_begin(p.total, range + 1);
+    int at = range_begin(p.total, range), turn = 0;
     const float scale_log2 = scale * 1.44269504088896f;
+    if (at >= end) return;
+    int inside;
+    Item it = locate(p, qs, cl, at, inside);
     __syncthreads();
     while (at < end) {
-      int inside;
-      const Item it = locate(qs, cl, at, inside);
       const int count = it.steps - inside < end - at ? it.steps - inside : end - at;
       const bool whole = inside == 0 && count == it.steps;
       float* to = part + (long)(2 * range + (inside == 0 ? 1 : 0)) * kPart;
       if (it.narrow) narrow(q, kc, vc, table, out, to, it, inside, count, whole, scale_log2, smem);
       else wide(q, kc, vc, table, out, to, it, inside, count, whole, scale_log2, smem, turn);
       at += count;
+      inside = 0;
+      next_item(qs, cl, it);
     }
     __syncthreads();
   }
 
-  static __device__ __forceinline__ void join(int unit, const float* part, const int* qs, const int* cl, T* out) {
-    const int total = total_steps(qs, cl), range = range_of(unit);
-    const int begin = range_begin(total, range), end = range_begin(total, range + 1);
-    if (begin >= end) return;
-    int inside;
-    const Item it = locate(qs, cl, end - 1, inside);
-    const int item0 = end - 1 - inside, item1 = item0 + it.steps;
-    if (item0 < begin || item1 <= end) return;   // begun by an earlier range, or finished in this one
+  // Adds up the parts of the items that were split.  The workgroups whose ranges hold a part of an item share its
+  // output groups among them: `rank` of `count` is this workgroup's.  With many parts the waves of a workgroup take the
+  // parts of a group between them, with few every wave its own groups.
+  static __device__ __forceinline__ void join_item(const float* part, const Plan& p, const Item& it, int item0, int rank, int count, T* out, char* smem) {
     const int wave = __builtin_amdgcn_readfirstlane(wave_id()), lane = lane_id(), query = lane & 31;
-    // a wide item: every wave its own rows; a narrow one: every wave some groups of the 32 rows
-    const int block = it.narrow ? 0 : wave;
-    Rows r;
-    {
-      const int count = it.s.len * G;
-      int row = it.tile * (it.narrow ? 32 : 32 * NW) + block * 32 + query;
-      r.valid = row < count;
-      if (!r.valid) row = count > 0 ? count - 1 : 0;
-      r.out = row_element(it, row);
-    }
-    const float* sums = part + block * kPartWave + DT * 1024;
-    const int last = [&] {   // the last range that holds a step of the item
-      int x = range;
-      while (x + 1 < GRID && range_begin(total, x + 1) < item1) ++x;
-      return x;
-    }();
-    float m = -1e30f, l = 0.0f;
-    for (int x = range; x <= last; ++x) {
-      if (range_begin(total, x) == range_begin(total, x + 1)) continue;
-      m = fmaxf(m, sums[(long)(2 * x + (x == range ? 1 : 0)) * kPart + query]);
-    }
-    for (int x = range; x <= last; ++x) {
-      if (range_begin(total, x) == range_begin(total, x + 1)) continue;
-      const float* s = sums + (long)(2 * x + (x == range ? 1 : 0)) * kPart;
-      l += s[32 + query] * __builtin_amdgcn_exp2f(s[query] - m);
-    }
-    const float inv = inverse(l);
-    for (int g = it.narrow ? wave : 0; g < DT * 4; g += it.narrow ? NW : 1) {
+    const int rows = it.s.len * G, row0 = it.tile * (it.narrow ? 32 : 32 * NW);
+    const int blocks = it.narrow ? 1 : clamp_int((rows - row0 + 31) / 32, 1, NW), groups = blocks * DT * 4;
+    const int first = range_with_step(p.total, item0);
+    // part i: ranges follow each other, unless there are fewer steps than ranges; then every step is a part
+    auto slot = [&](int i) { return (long)(i == 0 ? 2 * first + 1 : 2 * (p.total >= GRID ? first + i : range_with_step(p.total, item0 + i))) * kPart; };
+    const bool shared = count >= NW;
+    float* share = reinterpret_cast<float*>(smem);   // [NW][64][4] outputs, [NW][64] maxima, [NW][64] sums
+    for (int e = shared ? rank : rank * NW + wave; e < groups; e += shared ? count : count * NW) {
+      const int block = e / (DT * 4), g = e % (DT * 4);
+      const float* tile = part + block * kPartWave;
       float4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
-      for (int x = range; x <= last; ++x) {
-        if (range_begin(total, x) == range_begin(total, x + 1)) continue;
-        const long slot = (long)(2 * x + (x == range ? 1 : 0)) * kPart;
-        o += __builtin_amdgcn_exp2f(sums[slot + query] - m) * *reinterpret_cast<const float4_t*>(part + slot + block * kPartWave + g * 256 + lane * 4);
+      float m = -1e30f, l = 0.0f;
+      const int step = shared ? NW : 1;
+      int i = shared ? wave : 0;
+      auto add = [&](float pm, float pl, float4_t po) {
+        const float top = fmaxf(m, pm), a = __builtin_amdgcn_exp2f(m - top), b = __builtin_amdgcn_exp2f(pm - top);
+        m = top;
+        l = l * a + pl * b;
+        o = o * a + po * b;
+      };
+      for (; i + 3 * step < count; i += 4 * step) {   // four parts in flight
+        float pm[4], pl[4];
+        float4_t po[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float* t = tile + slot(i + k * step);
+          pm[k] = t[DT * 1024 + query], pl[k] = t[DT * 1024 + 32 + query];
+          po[k] = *reinterpret_cast<const float4_t*>(t + g * 256 + lane * 4);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) add(pm[k], pl[k], po[k]);
       }
+      for (; i < count; i += step) {
+        const float* t = tile + slot(i);
+        add(t[DT * 1024 + query], t[DT * 1024 + 32 + query], *reinterpret_cast<const float4_t*>(t + g * 256 + lane * 4));
+      }
+      if (shared) {
+        __syncthreads();
+        *reinterpret_cast<float4_t*>(share + (wave * 64 + lane) * 4) = o;
+        share[NW * 256 + wave * 64 + lane] = m;
+        share[NW * 320 + wave * 64 + lane] = l;
+        __syncthreads();
+        if (wave != 0) continue;
+        for (int w = 1; w < NW; ++w) add(share[NW * 256 + w * 64 + lane], share[NW * 320 + w * 64 + lane], *reinterpret_cast<const float4_t*>(share + (w * 64 + lane) * 4));
+      }
+      Rows r;
+      const int row = row0 + block * 32 + query;
+      r.valid = row < rows;
+      r.out = row_element(it, r.valid ? row : 0);
+      const float inv = inverse(l);
       store_group(out, r, g, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+    }
+  }
+  static constexpr int join_lds_bytes() { return NW * 384 * 4; }
+  static __device__ __forceinline__ void join(int unit, const float* part, const int* qs, const int* cl, T* out, char* smem) {
+    const Plan p = plan(qs, cl);
+    const int range = range_of(unit), begin = range_begin(p.total, range), end = range_begin(p.total, range + 1);
+    if (begin >= end) return;
+    // the item that an earlier range began, if there is one, and the one that this range leaves unfinished
+    for (int k = 0; k < 2; ++k) {
+      int inside;
+      const Item it = locate(p, qs, cl, k == 0 ? begin : end - 1, inside);
+      const int item0 = (k == 0 ? begin : end - 1) - inside, item1 = item0 + it.steps;
+      if (k == 0 ? inside == 0 : (item0 < begin || item1 <= end)) continue;
+      const int first = range_with_step(p.total, item0), last = range_with_step(p.total, item1 - 1);
+      const bool dense = p.total >= GRID;
+      join_item(part, p, it, item0, dense ? range - first : begin - item0, dense ? last - first + 1 : it.steps, out, smem);
     }
   }
 };

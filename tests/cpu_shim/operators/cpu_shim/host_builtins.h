@@ -15,6 +15,7 @@ inline void sincospif(float x, float* s, float* c) { *s = sinf(3.14159265f * x),
 #define __any(x) (x)
 #define __ballot(x) ((x) ? 1ull : 0ull)
 #define __shfl(v, ...) (v)
+#define __builtin_amdgcn_readlane(v, l) (v)
 #define __shfl_up(v, ...) (v)
 struct HostPair {
   unsigned v[2];
