@@ -50,8 +50,8 @@ bool read_in_kernel(const graph::Program& prog, const Instr* root) {
 int64_t paged_attention_part_bytes(const Instr* parts, int grid, int waves) {
   const auto& q = parts->operands[0]->shape.dims;
   const int64_t group = q[1] / parts->operands[1]->shape.dims[2];
-  const int64_t blocks = q[0] * group <= 32 ? 1 : waves;   // all sequences have at most 32 query rows
-  return 2 * int64_t(grid) * blocks * ((q[2] + 31) / 32 * 1024 + 64) * 4;
+  const int64_t D = q[2], narrow = D / 16 * 256 + 32, wide = waves * ((D + 31) / 32 * 1024 + 64);   // floats
+  return 2 * int64_t(grid) * (q[0] * group <= 16 ? narrow : wide) * 4;   // at most 16 query rows in all: no wide item
 }
 
 NodeFunction generate_operator(const graph::Program& prog, const graph::Node& node, const LaunchShape& ls, int grid) {
@@ -118,12 +118,13 @@ NodeFunction generate_operator(const graph::Program& prog, const graph::Node& no
         const std::string qp = input(0), kp = input(1), vp = input(2), tp = input(3), sp = input(4), lp = input(5);
         const std::string out = ptrs.output(result), pp = ptrs.output(ins);
         body << "Attention::partial(unit, " << qp << ", " << kp << ", " << vp << ", " << tp << ", " << sp << ", " << lp << ", " << out << ", " << pp << ", " << float_literal(c.scale) << ", smem);";
-        const int64_t D = q[2], waves = ls.waves();
-        const int64_t kp_bytes = D * 2 + 16, vp_bytes = (D * 2 + 63) / 128 * 128 + 64, tiles = (D + 31) / 32;
         // mirrors PagedAttention::lds_bytes
+        const int64_t D = q[2], waves = ls.waves(), limit = 160 * 1024;
+        const int64_t krow = D * 2 + 16, vrow = (D * 2 + 63) / 128 * 128 + 64, vpn = (D / 16 | 1) * 32, merge = D / 16 * 1024 + 128;
         int64_t nn = waves;
-        while (nn > 1 && (nn * 32 * (kp_bytes + vp_bytes) > 160 * 1024 || nn * D * 128 + nn * 256 > 160 * 1024)) nn /= 2;
-        f.smem_bytes = static_cast<int>(std::max({2 * 64 * (kp_bytes + vp_bytes), nn * 32 * (kp_bytes + vp_bytes), nn * (tiles * 4096 + 256)}));
+        while (nn > 1 && (nn * 32 * (krow + vpn) > limit || nn * merge > limit)) nn /= 2;
+        const int64_t wide = q[0] * (q[1] / kc[2]) <= 16 ? 0 : 2 * 64 * (krow + vrow);
+        f.smem_bytes = static_cast<int>(std::max({wide, nn * 32 * (krow + vpn), nn * merge}));
         body << " static_assert(Attention::lds_bytes() == " << f.smem_bytes << ", \"LDS\");";
       } else {
         const std::string pp = input(0), sp = input(1), lp = input(2);

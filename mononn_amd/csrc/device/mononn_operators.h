@@ -222,10 +222,25 @@ __device__ __forceinline__ float half_waves_sum(float v) {
   half_waves(v, a, b);
   return a + b;
 }
+// the same for the lane 16 further on or back
+__device__ __forceinline__ void quarter_waves(float v, float& a, float& b) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+  a = __builtin_bit_cast(float, (unsigned)r[0]), b = __builtin_bit_cast(float, (unsigned)r[1]);
+}
+__device__ __forceinline__ float quarter_waves_max(float v) {
+  float a, b;
+  quarter_waves(v, a, b);
+  return fmaxf(a, b);
+}
+__device__ __forceinline__ float quarter_waves_sum(float v) {
+  float a, b;
+  quarter_waves(v, a, b);
+  return a + b;
+}
 
 // The query rows of a sequence for one key / value head are its new tokens times the G = H / HKV query heads that
-// share it (row = token * G + head of the group), in tiles: ROWS = 32 per wave in a *wide* item, 32 in all in a
-// *narrow* one (a sequence with at most 32 rows: decoding).  An item (sequence, key head, tile) works through its
+// share it (row = token * G + head of the group), in tiles: 32 rows per wave in a *wide* item, 16 in all in a
+// *narrow* one (a sequence with at most 16 rows: decoding).  An item (sequence, key head, tile) works through its
 // keys in steps: 64 keys that all waves share in a wide item, 32 keys per wave in a narrow one.
 //
 // The steps of all items, in order, are dealt to the workgroups in equal contiguous ranges, whatever the lengths of
@@ -233,8 +248,8 @@ __device__ __forceinline__ float half_waves_sum(float v) {
 // a range that begins or ends inside an item leaves the running maximum, sum and output of its part in memory, and
 // the next stage (`join`) adds those up: the range in which an item begins owns it.
 //
-// Per step, with S^T = K Q^T and O^T += V^T P^T on v_mfma_f32_32x32x16: queries lie along the lanes in both products, so
-// the maximum, the sum and the rescaling of a query stay in its lane (and the lane 32 further on), and the
+// Per step, with S^T = K Q^T and O^T += V^T P^T on v_mfma_f32_32x32x16 (narrow: 16x16x32): queries lie along the lanes in both products, so
+// the maximum, the sum and the rescaling of a query stay in its lane (and those 32, or 16, further on), and the
 // probabilities leave the first product in the lanes that feed the second (a lane's 8 accumulator rows are the 8 keys
 // of one contraction step, in an order that the transposed reads of V follow).
 template <class T, int TOKENS, int SEQS, int H, int HKV, int D, int PAGE, int PAGES, int WIDTH, int WINDOW, int GRID, bool COHERENT>
@@ -254,16 +269,22 @@ struct PagedAttention {
   static_assert(VP >= D * 2 && VP >= DT * 64, "value rows");
   static constexpr int kWideKeys = 64;
   static constexpr int kWideBuffer = kWideKeys * (KP + VP);
-  static constexpr int kWaveBuffer = 32 * (KP + VP);
+  // narrow items: values are read 32 bytes of 8 rows per 32 lanes; an odd multiple of 32 bytes keeps 8 rows apart
+  static constexpr int VPN = (D / 16 | 1) * 32;
+  static constexpr int kWaveBuffer = 32 * (KP + VPN);
+  static constexpr int kTiles = D / 16;          // tiles of 16 output elements of a narrow item
+  static constexpr int QN = (D + 31) / 32;       // its contraction steps of the first product
   static constexpr int kLdsLimit = 160 * 1024;
-  static constexpr int narrow_waves(int n) { return n * kWaveBuffer <= kLdsLimit && n * D * 128 + n * 256 <= kLdsLimit ? n : narrow_waves(n / 2); }
+  static constexpr int narrow_waves(int n) { return n * kWaveBuffer <= kLdsLimit && n * (kTiles * 1024 + 128) <= kLdsLimit ? n : narrow_waves(n / 2); }
   static constexpr int NN = narrow_waves(NW);    // waves that take part in a narrow item
   static constexpr int kNarrowKeys = 32 * NN;
+  static constexpr bool kAllNarrow = TOKENS * G <= 16;      // no sequence can have more rows
   static constexpr int kPartWave = DT * 1024 + 64;          // floats: output tiles as they lie in the registers, maxima, sums
-  static constexpr int kPart = (TOKENS * G <= 32 ? 1 : NW) * kPartWave;   // floats of one partial result; two per workgroup
-  static constexpr int kMergeBytes = NN * (DT * 4096 + 256);
+  static constexpr int kPartNarrow = kTiles * 256 + 32;
+  static constexpr int kPart = kAllNarrow ? kPartNarrow : NW * kPartWave;   // floats of one partial result; two per workgroup
+  static constexpr int kMergeBytes = NN * (kTiles * 1024 + 128);
   static constexpr int lds_bytes() {
-    int n = 2 * kWideBuffer;
+    int n = kAllNarrow ? 0 : 2 * kWideBuffer;
     if (NN * kWaveBuffer > n) n = NN * kWaveBuffer;
     return kMergeBytes > n ? kMergeBytes : n;
   }
@@ -271,16 +292,16 @@ struct PagedAttention {
   struct Item {
     int b, h, tile;
     Sequence s;
-    bool narrow;
+    int narrow;
     int first, steps;   // first step (a multiple of the step's keys) and how many
   };
 
-  static __device__ __forceinline__ bool is_narrow(int len) { return len * G <= 32; }
+  static __device__ __forceinline__ bool is_narrow(int len) { return kAllNarrow || len * G <= 16; }
   static __device__ __forceinline__ int tiles_of(int len) { return is_narrow(len) ? (len > 0 ? 1 : 0) : (len * G + 32 * NW - 1) / (32 * NW); }
   // keys [lo, hi) that some row of the tile sees, as steps; at least one step, so that empty rows are written too
   static __device__ __forceinline__ void tile_steps(const Sequence& s, int tile, int& first, int& steps) {
     const bool narrow = is_narrow(s.len);
-    const int rows = narrow ? 32 : 32 * NW, keys = narrow ? kNarrowKeys : kWideKeys;
+    const int rows = narrow ? 16 : 32 * NW, keys = narrow ? kNarrowKeys : kWideKeys;
     const int t0 = tile * rows / G;
     int t1 = ((tile + 1) * rows - 1) / G;
     if (t1 > s.len - 1) t1 = s.len - 1;
@@ -418,21 +439,21 @@ struct PagedAttention {
   static constexpr bool kUniformRows = kWaveSize % CPR == 0 && PAGE % (kWaveSize / CPR) == 0;
   static __device__ __forceinline__ int lane_page(const int* table, int b, int key0) {
     const int key = clamp_int(key0 + lane_id(), 0, MAX_KEYS - 1);
-    return clamp_int(table[(long)b * WIDTH + key / PAGE], 0, PAGES - 1);
+    return table[(long)b * WIDTH + key / PAGE];   // clamped to the pool where it is used: nothing waits for it here
   }
   static __device__ __forceinline__ half8_t load_piece(const T* p) { return *reinterpret_cast<const half8_t*>(p); }
   // piece (first_piece + lane) of the keys from key0 on; `pages`: lane_page of key0
   static __device__ __forceinline__ void load_run_of_rows(const T* kc, const T* vc, int pages, int key0, int first_piece, int h, half8_t& k, half8_t& v) {
     if constexpr (kUniformRows) {
       const int row0 = first_piece / CPR, key = key0 + row0;
-      const int page = __builtin_amdgcn_readlane(pages, row0 & (kWaveSize - 1));
+      const int page = clamp_int(__builtin_amdgcn_readlane(pages, row0 & (kWaveSize - 1)), 0, PAGES - 1);
       const long base = (((long)page * PAGE + key % PAGE) * HKV + h) * D;
       const unsigned at = (unsigned)(lane_id() / CPR) * (HKV * D) + (unsigned)(lane_id() % CPR) * 8;
       k = load_piece(kc + base + at);
       v = load_piece(vc + base + at);
     } else {
       const int at = first_piece + lane_id(), row = at / CPR, key = key0 + row;
-      const int page = __shfl(pages, row & (kWaveSize - 1), kWaveSize);
+      const int page = clamp_int(__shfl(pages, row & (kWaveSize - 1), kWaveSize), 0, PAGES - 1);
       const long off = (((long)page * PAGE + key % PAGE) * HKV + h) * D + at % CPR * 8;
       k = load_piece(kc + off);
       v = load_piece(vc + off);
@@ -571,16 +592,20 @@ struct PagedAttention {
     for (int i = 0; i < kRuns; ++i) load_run_of_rows(kc, vc, pages, key0, wide_piece(i), h, k[i], v[i]);
   }
   // Rows behind the sequence's last key become zeros: whatever those cells hold, NaN included, must not reach 0 * v.
-  static __device__ __forceinline__ void wide_store(char* buf, int key0, int ctx, const half8_t (&k)[kRuns], const half8_t (&v)[kRuns]) {
-    const bool all = key0 + kWideKeys <= ctx;
+  static __device__ __forceinline__ void wide_store(char* buf, int key0, int ctx, half8_t (&k)[kRuns], half8_t (&v)[kRuns]) {
+    if (key0 + kWideKeys > ctx) {
+#pragma unroll
+      for (int i = 0; i < kRuns; ++i) {
+        const half8_t zero = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (key0 + (wide_piece(i) + lane_id()) / CPR >= ctx) k[i] = zero, v[i] = zero;
+      }
+    }
 #pragma unroll
     for (int i = 0; i < kRuns; ++i) {
       const int at = wide_piece(i) + lane_id(), row = at / CPR, c = at % CPR;
       if (kWideKeys * CPR % MONONN_BLOCK_SIZE != 0 && row >= kWideKeys) break;
-      const bool in = all || key0 + row < ctx;
-      const half8_t zero = {0, 0, 0, 0, 0, 0, 0, 0};
-      *reinterpret_cast<half8_t*>(buf + row * KP + c * 16) = in ? k[i] : zero;
-      *reinterpret_cast<half8_t*>(buf + kWideKeys * KP + row * VP + c * 16) = in ? v[i] : zero;
+      *reinterpret_cast<half8_t*>(buf + row * KP + c * 16) = k[i];
+      *reinterpret_cast<half8_t*>(buf + kWideKeys * KP + row * VP + c * 16) = v[i];
     }
   }
   static __device__ __forceinline__ void wide(const T* q, const T* kc, const T* vc, const int* table, T* out, float* part, const Item& it, int from, int count, bool whole,
@@ -630,87 +655,215 @@ struct PagedAttention {
   }
 
   // ---- narrow items ----------------------------------------------------------------------------------------------
+  // Bound by the reads of keys and values.  Every wave streams its own 32 keys of a step: requested a step ahead into
+  // registers, through the wave's own LDS rows (no workgroup barrier) into the products.  The next step may belong to
+  // the next item: its keys, and that item's queries, are on their way while the waves' shares of the last one are added up.
   static constexpr int kMine = CPR / 2;   // pieces of K (and of V) a lane moves per step: 32 rows over 64 lanes
-  static __device__ __forceinline__ void narrow_load(const T* kc, const T* vc, int pages, int key0, int h, half8_t (&k)[kMine], half8_t (&v)[kMine]) {
+  struct Cursor {
+    Item it;
+    int step;   // inside the item
+    __device__ __forceinline__ int key0() const { return (it.first + step) * kNarrowKeys + __builtin_amdgcn_readfirstlane(wave_id()) * 32; }
+  };
+  struct NarrowRows {
+    half8_t q[QN];
+    int lo, hi;
+    bool valid;
+    long out;
+  };
+  static __device__ __forceinline__ void narrow_rows(const T* q, const Item& it, NarrowRows& r) {
+    const int lane = lane_id(), count = it.s.len * G, g = lane >> 4;
+    int row = lane & 15;
+    r.valid = row < count;
+    if (!r.valid) row = count > 0 ? count - 1 : 0;
+    r.out = row_element(it, row);
 #pragma unroll
-    for (int i = 0; i < kMine; ++i) load_run_of_rows(kc, vc, pages, key0, i * kWaveSize, h, k[i], v[i]);
+    for (int i = 0; i < QN; ++i) {
+      const half8_t zero = {0, 0, 0, 0, 0, 0, 0, 0};
+      r.q[i] = D % 32 != 0 && i == QN - 1 && g >= 2 ? zero : load_piece(q + r.out + i * 32 + g * 8);
+    }
+    r.hi = it.s.ctx - it.s.len + row / G;
+    r.lo = WINDOW > 0 ? r.hi - WINDOW + 1 : 0;
   }
-  static __device__ __forceinline__ void narrow(const T* q, const T* kc, const T* vc, const int* table, T* out, float* part, const Item& it, int from, int count, bool whole,
-                                                float scale_log2, char* smem) {
-    const int wave = __builtin_amdgcn_readfirstlane(wave_id());
+  static __device__ __forceinline__ void narrow_load(const T* kc, const T* vc, int pages, const Cursor& c, half8_t (&k)[kMine], half8_t (&v)[kMine]) {
+    if (c.key0() >= c.it.s.ctx) return;   // the wave has no key in this step
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) load_run_of_rows(kc, vc, pages, c.key0(), i * kWaveSize, c.it.h, k[i], v[i]);
+  }
+  struct NarrowState {
+    float4_t o[kTiles];
+    float m, l;   // of the lane's query; l of the lane's keys until finish()
+    __device__ __forceinline__ void clear() {
+      m = -1e30f;
+      l = 0.0f;
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) o[t] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    __device__ __forceinline__ void finish() { l = quarter_waves_sum(half_waves_sum(l)); }
+  };
+  // 32 keys on 16 query rows
+  static __device__ __forceinline__ void narrow_step(const char* kbuf, const char* vbuf, int key0, const NarrowRows& r, NarrowState& st, float scale_log2, bool check) {
+    const int lane = lane_id(), g = lane >> 4, i16 = lane & 15;
+    float4_t s[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      s[b] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+      const char* row = kbuf + (b * 16 + i16) * KP + g * 16;
+#pragma unroll
+      for (int i = 0; i < QN; ++i) {
+        // half a step at the end of the head: the queries are zero there, any elements of the row will do
+        const int back = D % 32 != 0 && i == QN - 1 && g >= 2 ? 32 : 0;
+        s[b] = mfma_16x16x32<kBf16>(*reinterpret_cast<const half8_t*>(row + i * 64 - back), r.q[i], s[b]);
+      }
+    }
+    if (check) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = key0 + b * 16 + 4 * g + i;
+          s[b][i] = key >= r.lo && key <= r.hi ? s[b][i] : -__builtin_inff();
+        }
+    }
+    float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+    top = quarter_waves_max(half_waves_max(top)) * scale_log2;
+    if (__any(top > st.m + 6.0f)) {   // as in step()
+      const float m = fmaxf(st.m, top);
+      const float a = __builtin_amdgcn_exp2f(st.m - m);
+      st.l *= a;
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) st.o[t] *= a;
+      st.m = m;
+    }
+    half8_t p;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float e = __builtin_amdgcn_exp2f(s[b][i] * scale_log2 - st.m);
+        st.l += e;
+        p[b * 4 + i] = __builtin_bit_cast(half_t, (T)e);
+      }
+    const char* vrow = vbuf + (4 * g + i16 / 4) * VPN + (i16 & 3) * 8;
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) {
+      struct { mononn_short4 lo, hi; } v;
+      v.lo = MONONN_LDS_READ_TR16(vrow + t * 32);
+      v.hi = MONONN_LDS_READ_TR16(vrow + 16 * VPN + t * 32);
+      st.o[t] = mfma_16x16x32<kBf16>(__builtin_bit_cast(half8_t, v), p, st.o[t]);
+    }
+  }
+  static __device__ __forceinline__ void narrow_out(T* out, long row, bool valid, int tile, float4_t o, float inv) {
+    if (!valid) return;
+    const T v[4] = {(T)(o[0] * inv), (T)(o[1] * inv), (T)(o[2] * inv), (T)(o[3] * inv)};
+    store_run<COHERENT, T, 4>(out + row + tile * 16 + (lane_id() >> 4) * 4, v);
+  }
+  // Works from step `inside` of `it` to the end of the range or of the run of narrow items; `it` and `inside` become
+  // where it stopped.  Returns the steps done.
+  static __device__ __forceinline__ int narrow(const T* q, const T* kc, const T* vc, const int* table, const int* qs, const int* cl, T* out, float* part, int range, Item& it, int& inside,
+                                               int left, float scale_log2, char* smem) {
+    const int wave = __builtin_amdgcn_readfirstlane(wave_id()), lane = lane_id(), query = lane & 15;
     const bool live = wave < NN;
-    Rows r;
-    load_rows(q, it, 0, r);
-    State st;
+    char* kbuf = smem + (live ? wave : 0) * kWaveBuffer;
+    char* vbuf = kbuf + 32 * KP;
+    Cursor cur = {it, inside};
+    // the step behind `c`; false when the range ends before it or it is a wide item's (`c` is that item then)
+    auto advance = [&](Cursor& c, int remaining) {
+      if (remaining <= 0) return false;
+      if (++c.step < c.it.steps) return true;
+      next_item(qs, cl, c.it);
+      c.step = 0;
+      return c.it.narrow != 0;
+    };
+    half8_t k[kMine], v[kMine];
+    int done = 0, begun = inside;   // step of the item at which this part begins
+    NarrowRows r, rn;
+    narrow_rows(q, cur.it, r);
+    if (live) narrow_load(kc, vc, lane_page(table, cur.it.b, cur.key0()), cur, k, v);
+    Cursor nxt = cur;
+    bool more = advance(nxt, left - 1);
+    int pages = more ? lane_page(table, nxt.it.b, nxt.key0()) : 0;
+    NarrowState st;
     st.clear();
     __syncthreads();   // the buffers may still be read by a wide item's last step
-    if (live) {
-      char* kbuf = smem + wave * kWaveBuffer;
-      char* vbuf = kbuf + 32 * KP;
-      const int p_first = it.s.ctx - it.s.len, p_last = it.s.ctx - 1;
-      half8_t k[kMine], v[kMine];
-      const int begin = (it.first + from) * kNarrowKeys + wave * 32;
-      narrow_load(kc, vc, lane_page(table, it.b, begin), begin, it.h, k, v);
-      int pages = lane_page(table, it.b, begin + kNarrowKeys);
-      for (int i = 0; i < count; ++i) {
-        const int key0 = begin + i * kNarrowKeys;
-        const bool all = key0 + 32 <= it.s.ctx;
+    for (;;) {
+      const int key0 = cur.key0();
+      const bool some = live && key0 < cur.it.s.ctx;
+      if (some) {
+        if (key0 + 32 > cur.it.s.ctx) {   // rows behind the last key: zeros, as in wide_store()
+#pragma unroll
+          for (int j = 0; j < kMine; ++j) {
+            const half8_t zero = {0, 0, 0, 0, 0, 0, 0, 0};
+            if (key0 + (lane + j * kWaveSize) / CPR >= cur.it.s.ctx) k[j] = zero, v[j] = zero;
+          }
+        }
 #pragma unroll
         for (int j = 0; j < kMine; ++j) {
-          const int at = lane_id() + j * kWaveSize, row = at / CPR, c = at % CPR;
-          const bool in = all || key0 + row < it.s.ctx;
-          const half8_t zero = {0, 0, 0, 0, 0, 0, 0, 0};
-          *reinterpret_cast<half8_t*>(kbuf + row * KP + c * 16) = in ? k[j] : zero;
-          *reinterpret_cast<half8_t*>(vbuf + row * VP + c * 16) = in ? v[j] : zero;
+          const int at = lane + j * kWaveSize, row = at / CPR, c = at % CPR;
+          *reinterpret_cast<half8_t*>(kbuf + row * KP + c * 16) = k[j];
+          *reinterpret_cast<half8_t*>(vbuf + row * VPN + c * 16) = v[j];
         }
-        if (i + 1 < count) {
-          narrow_load(kc, vc, pages, key0 + kNarrowKeys, it.h, k, v);
-          pages = lane_page(table, it.b, key0 + 2 * kNarrowKeys);
-        }
+      }
+      Cursor behind = nxt;
+      bool more_behind = false;
+      if (more) {
+        if (live) narrow_load(kc, vc, pages, nxt, k, v);
+        more_behind = advance(behind, left - done - 2);
+        if (more_behind) pages = lane_page(table, behind.it.b, behind.key0());
+      }
+      if (some) {
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();   // the wave's own rows: written above, read below
-        const bool none = key0 > p_last || (WINDOW > 0 && key0 + 31 < p_first - WINDOW + 1);
-        if (!none) {
+        const int p_first = cur.it.s.ctx - cur.it.s.len, p_last = cur.it.s.ctx - 1;
+        if (!(WINDOW > 0 && key0 + 31 < p_first - WINDOW + 1)) {
           const bool check = key0 + 31 > p_first || (WINDOW > 0 && key0 < p_last - WINDOW + 1);
-          step<1>(kbuf, vbuf, key0, r, st, scale_log2, check);
+          narrow_step(kbuf, vbuf, key0, r, st, scale_log2, check);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
         __builtin_amdgcn_wave_barrier();
       }
-    }
-    st.finish();
-    // the waves' shares of the keys meet in LDS; every wave then adds up some of the output groups
-    __syncthreads();
-    float* sums = reinterpret_cast<float*>(smem);             // [NN][64]: maxima, sums
-    float* tiles = sums + NN * 64;                            // [NN][DT * 4][64][4]
-    if (live) {
-      sums[wave * 64 + lane_id()] = lane_id() < 32 ? st.m : st.l;
+      ++done;
+      if (cur.step + 1 == cur.it.steps || done == left) {
+        // the end of the item, or of the range: the waves' shares of the keys meet in LDS, every wave adds up some tiles
+        const bool whole = begun == 0 && cur.step + 1 == cur.it.steps;
+        if (more) narrow_rows(q, nxt.it, rn);
+        st.finish();
+        __syncthreads();
+        float* sums = reinterpret_cast<float*>(smem);             // [NN][32]: maxima, sums
+        float* tiles = sums + NN * 32;                            // [NN][kTiles][64][4]
+        if (live) {
+          if (lane < 32) sums[wave * 32 + lane] = lane < 16 ? st.m : st.l;
 #pragma unroll
-      for (int g = 0; g < DT * 4; ++g) {
-        const float4_t o = {st.o[g / 4][g % 4 * 4], st.o[g / 4][g % 4 * 4 + 1], st.o[g / 4][g % 4 * 4 + 2], st.o[g / 4][g % 4 * 4 + 3]};
-        *reinterpret_cast<float4_t*>(tiles + (wave * DT * 4 + g) * 256 + lane_id() * 4) = o;
+          for (int t = 0; t < kTiles; ++t) *reinterpret_cast<float4_t*>(tiles + (wave * kTiles + t) * 256 + lane * 4) = st.o[t];
+        }
+        __syncthreads();
+        float m = -1e30f, l = 0.0f, w[NN];
+#pragma unroll
+        for (int i = 0; i < NN; ++i) m = fmaxf(m, sums[i * 32 + query]);
+#pragma unroll
+        for (int i = 0; i < NN; ++i) {
+          w[i] = __builtin_amdgcn_exp2f(sums[i * 32 + query] - m);
+          l += w[i] * sums[i * 32 + 16 + query];
+        }
+        float* to = part + (long)(2 * range + (begun == 0 ? 1 : 0)) * kPart;
+        const float inv = inverse(l);
+        for (int t = wave; t < kTiles; t += NW) {
+          float4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int i = 0; i < NN; ++i) o += w[i] * *reinterpret_cast<const float4_t*>(tiles + (i * kTiles + t) * 256 + lane * 4);
+          if (whole) narrow_out(out, r.out, r.valid, t, o, inv);
+          else store_part(to, t, o[0], o[1], o[2], o[3]);
+        }
+        if (!whole && wave == 0 && lane < 32) st1(to + kTiles * 256 + lane, lane < 16 ? m : l);
+        __syncthreads();
+        begun = 0;
+        st.clear();
+        r = rn;
       }
+      if (!more) break;
+      cur = nxt, nxt = behind, more = more_behind;
     }
-    __syncthreads();
-    const int query = lane_id() & 31;
-    float m = -1e30f, l = 0.0f, w[NN];
-#pragma unroll
-    for (int i = 0; i < NN; ++i) m = fmaxf(m, sums[i * 64 + query]);
-#pragma unroll
-    for (int i = 0; i < NN; ++i) {
-      w[i] = __builtin_amdgcn_exp2f(sums[i * 64 + query] - m);
-      l += w[i] * sums[i * 64 + 32 + query];
-    }
-    const float inv = whole ? inverse(l) : 1.0f;
-    for (int g = wave; g < DT * 4; g += NW) {
-      float4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int i = 0; i < NN; ++i) o += w[i] * *reinterpret_cast<const float4_t*>(tiles + (i * DT * 4 + g) * 256 + lane_id() * 4);
-      if (whole) store_group(out, r, g, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
-      else store_part(part, g, o[0], o[1], o[2], o[3]);
-    }
-    if (!whole && wave == 0) store_part_sums(part, m, l);
-    __syncthreads();
+    it = nxt.it, inside = nxt.step;
+    return done;
   }
 
   // ---- stages ----------------------------------------------------------------------------------------------------
@@ -734,14 +887,18 @@ struct PagedAttention {
     Item it = locate(p, qs, cl, at, inside);
     __syncthreads();
     while (at < end) {
-      const int count = it.steps - inside < end - at ? it.steps - inside : end - at;
-      const bool whole = inside == 0 && count == it.steps;
-      float* to = part + (long)(2 * range + (inside == 0 ? 1 : 0)) * kPart;
-      if (it.narrow) narrow(q, kc, vc, table, out, to, it, inside, count, whole, scale_log2, smem);
-      else wide(q, kc, vc, table, out, to, it, inside, count, whole, scale_log2, smem, turn);
-      at += count;
-      inside = 0;
-      next_item(qs, cl, it);
+      if (it.narrow) {
+        at += narrow(q, kc, vc, table, qs, cl, out, part, range, it, inside, end - at, scale_log2, smem);
+        continue;
+      }
+      if constexpr (!kAllNarrow) {
+        const int count = it.steps - inside < end - at ? it.steps - inside : end - at;
+        const bool whole = inside == 0 && count == it.steps;
+        wide(q, kc, vc, table, out, part + (long)(2 * range + (inside == 0 ? 1 : 0)) * kPart, it, inside, count, whole, scale_log2, smem, turn);
+        at += count;
+        inside = 0;
+        next_item(qs, cl, it);
+      }
     }
     __syncthreads();
   }
@@ -750,16 +907,17 @@ struct PagedAttention {
   // output groups among them: `rank` of `count` is this workgroup's.  With many parts the waves of a workgroup take the
   // parts of a group between them, with few every wave its own groups.
   static __device__ __forceinline__ void join_item(const float* part, const Plan& p, const Item& it, int item0, int rank, int count, T* out, char* smem) {
-    const int wave = __builtin_amdgcn_readfirstlane(wave_id()), lane = lane_id(), query = lane & 31;
-    const int rows = it.s.len * G, row0 = it.tile * (it.narrow ? 32 : 32 * NW);
-    const int blocks = it.narrow ? 1 : clamp_int((rows - row0 + 31) / 32, 1, NW), groups = blocks * DT * 4;
+    const int wave = __builtin_amdgcn_readfirstlane(wave_id()), lane = lane_id(), queries = it.narrow ? 16 : 32, query = lane & (queries - 1);
+    const int rows = it.s.len * G, row0 = it.tile * (it.narrow ? 16 : 32 * NW);
+    const int per_block = it.narrow ? kTiles : DT * 4, sums = per_block * 256;   // groups of four elements per lane; maxima and sums lie behind
+    const int blocks = it.narrow ? 1 : clamp_int((rows - row0 + 31) / 32, 1, NW), groups = blocks * per_block;
     const int first = range_with_step(p.total, item0);
     // part i: ranges follow each other, unless there are fewer steps than ranges; then every step is a part
     auto slot = [&](int i) { return (long)(i == 0 ? 2 * first + 1 : 2 * (p.total >= GRID ? first + i : range_with_step(p.total, item0 + i))) * kPart; };
     const bool shared = count >= NW;
     float* share = reinterpret_cast<float*>(smem);   // [NW][64][4] outputs, [NW][64] maxima, [NW][64] sums
     for (int e = shared ? rank : rank * NW + wave; e < groups; e += shared ? count : count * NW) {
-      const int block = e / (DT * 4), g = e % (DT * 4);
+      const int block = e / per_block, g = e % per_block;
       const float* tile = part + block * kPartWave;
       float4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
       float m = -1e30f, l = 0.0f;
@@ -777,7 +935,7 @@ struct PagedAttention {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const float* t = tile + slot(i + k * step);
-          pm[k] = t[DT * 1024 + query], pl[k] = t[DT * 1024 + 32 + query];
+          pm[k] = t[sums + query], pl[k] = t[sums + queries + query];
           po[k] = *reinterpret_cast<const float4_t*>(t + g * 256 + lane * 4);
         }
 #pragma unroll
@@ -785,7 +943,7 @@ struct PagedAttention {
       }
       for (; i < count; i += step) {
         const float* t = tile + slot(i);
-        add(t[DT * 1024 + query], t[DT * 1024 + 32 + query], *reinterpret_cast<const float4_t*>(t + g * 256 + lane * 4));
+        add(t[sums + query], t[sums + queries + query], *reinterpret_cast<const float4_t*>(t + g * 256 + lane * 4));
       }
       if (shared) {
         __syncthreads();
@@ -801,7 +959,8 @@ struct PagedAttention {
       r.valid = row < rows;
       r.out = row_element(it, r.valid ? row : 0);
       const float inv = inverse(l);
-      store_group(out, r, g, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+      if (it.narrow) narrow_out(out, r.out, r.valid, g, o, inv);
+      else store_group(out, r, g, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
     }
   }
   static constexpr int join_lds_bytes() { return NW * 384 * 4; }
