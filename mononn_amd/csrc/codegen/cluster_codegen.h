@@ -124,8 +124,8 @@ bool gemm_uses_mfma(const graph::GemmDesc& g);
 
 // one of the custom calls of hlo::OperatorConfig (device/mononn_operators.h); grid: workgroups of the launch
 NodeFunction generate_operator(const graph::Program& prog, const graph::Node& node, const LaunchShape& ls, int grid);
-// temp bytes of a paged attention's partial results
-int64_t paged_attention_part_bytes(const hlo::Instr* parts, int grid, int waves);
+// temp bytes of the partial results of a call that the parser has split
+int64_t operator_part_bytes(const hlo::Instr* parts, int grid, int waves);
 
 // dry runs used by the merge passes
 bool can_merge_clusters(const graph::Program& prog, const std::vector<const hlo::Instr*>& producer,

@@ -47,8 +47,52 @@ bool read_in_kernel(const graph::Program& prog, const Instr* root) {
 
 }  // namespace
 
-int64_t paged_attention_part_bytes(const Instr* parts, int grid, int waves) {
+namespace {
+// How matvec_w4 is dealt to the launch: `wk` waves share a tile of 16 weight rows, `sk` workgroups do, a wave reads
+// blocks of 128 `p` columns.
+struct MatvecPlan {
+  int64_t M, N, K, group;
+  int64_t wk = 1, sk = 1, p = 1;
+  int64_t row_blocks() const { return std::min<int64_t>((M + 15) / 16, 4); }
+  int64_t x_rows() const { return std::min(M, 16 * row_blocks()); }
+  int64_t blocks_per_workgroup() const { return ((K + 128 * p - 1) / (128 * p) + sk - 1) / sk; }
+  int64_t x_bytes() const { return blocks_per_workgroup() * p * 256 * (x_rows() | 1); }   // an odd pitch
+};
+// The plan whose busiest workgroup reads the fewest columns times tiles; among equals larger blocks (fewer loads of
+// scales), then fewer slices, then fewer shares (fewer starts of a workgroup's loads).
+MatvecPlan plan_matvec(const Instr* call, int64_t grid, int64_t waves) {
+  const auto &x = call->operands[0]->shape.dims, &w = call->operands[1]->shape.dims, &s = call->operands[2]->shape.dims;
+  MatvecPlan best{x[0], w[0], x[1], x[1] / s[1]};
+  const bool split = hlo::matvec_w4_in_parts(best.M, best.K);
+  const int64_t tiles = (best.N + 15) / 16, passes = (best.M + 16 * best.row_blocks() - 1) / (16 * best.row_blocks());
+  int64_t least = -1;
+  for (int64_t p : {4, 2, 1}) {
+    if (p > 1 && best.M > 4 && (best.group >= 128 || p > 2)) continue;   // MatvecW4::kWhole, and the scales of kSwap
+    for (int64_t sk = 1; sk <= (split ? 64 : 1); ++sk)
+      for (int64_t wk = 1; wk <= waves; wk *= 2) {
+        if (waves % wk != 0) break;
+        MatvecPlan c = best;
+        c.p = p, c.sk = sk, c.wk = wk;
+        if (c.x_bytes() > 128 * 1024) continue;
+        const int64_t at_once = waves / wk, units = (tiles + at_once - 1) / at_once * sk * passes;
+        const int64_t busiest = (units + grid - 1) / grid * ((c.blocks_per_workgroup() + wk - 1) / wk) * p;
+        if (least < 0 || busiest < least) {
+          least = busiest;
+          best.p = p, best.sk = sk, best.wk = wk;
+        }
+      }
+  }
+  MONONN_CHECK(least >= 0, kInternal) << call->hlo_name << ": no arrangement of the 4-bit product fits the LDS";
+  return best;
+}
+}  // namespace
+
+int64_t operator_part_bytes(const Instr* parts, int grid, int waves) {
   const auto& q = parts->operands[0]->shape.dims;
+  if (parts->oper.kind == OperatorConfig::kMatvecW4Parts) {
+    const MatvecPlan p = plan_matvec(parts, grid, waves);
+    return p.sk * p.M * p.N * 4;
+  }
   const int64_t group = q[1] / parts->operands[1]->shape.dims[2];
   const int64_t D = q[2], narrow = D / 16 * 256 + 32, wide = waves * ((D + 31) / 32 * 1024 + 64);   // floats
   return 2 * int64_t(grid) * (q[0] * group <= 16 ? narrow : wide) * 4;   // at most 16 query rows in all: no wide item
@@ -135,25 +179,26 @@ NodeFunction generate_operator(const graph::Program& prog, const graph::Node& no
       check_units(grid);
       break;
     }
-    case OperatorConfig::kMatvecW4: {
-      const int64_t M = dims(0)[0], K = dims(0)[1], N = dims(1)[0], group = K / dims(2)[1];
-      const bool zeros = ins->operands.size() == 4;
-      // Waves that share a tile of 16 weight rows by splitting the columns: the arrangement with the shortest longest
-      // wave over the whole launch, the fewest shares among equals.
-      const int64_t tiles = (N + 15) / 16, chunks = (K + 127) / 128, passes = (M + 63) / 64;
-      int64_t wk = 1, best = -1;
-      for (int64_t w = 1; w <= ls.waves(); w *= 2) {
-        if (ls.waves() % w != 0) break;
-        const int64_t units = (tiles + ls.waves() / w - 1) / (ls.waves() / w) * passes;
-        const int64_t longest = (units + grid - 1) / grid * ((chunks + w - 1) / w);
-        if (best < 0 || longest < best) best = longest, wk = w;
+    case OperatorConfig::kMatvecW4:
+    case OperatorConfig::kMatvecW4Parts: {
+      const bool parts_stage = c.kind == OperatorConfig::kMatvecW4Parts;
+      const Instr* call = parts_stage || ins->operands[0]->oper.kind != OperatorConfig::kMatvecW4Parts ? ins : ins->operands[0];
+      const MatvecPlan p = plan_matvec(call, grid, ls.waves());
+      const bool zeros = call->operands.size() == 4, join = call != ins;
+      body << "typedef mononn_dev::MatvecW4<" << hlo::dtype_ctype(call->operands[0]->shape.dtype) << ", " << p.M << ", " << p.N << ", " << p.K << ", " << p.group << ", " << flag(zeros) << ", "
+           << p.wk << ", " << p.sk << ", " << p.p << ", " << flag(!parts_stage && read_in_kernel(prog, ins)) << "> Matvec; ";
+      if (join) {
+        const std::string pp = input(0);
+        body << "Matvec::join(unit, " << pp << ", " << ptrs.output(ins) << ");";
+        check_units((p.M * p.N + block - 1) / block);
+        break;
       }
-      const int64_t mt = std::min<int64_t>((M + 15) / 16, 4), per = ls.waves() / wk;
       const std::string x = input(0), w = input(1), s = input(2), z = zeros ? input(3) : "nullptr", out = ptrs.output(ins);
-      body << "mononn_dev::MatvecW4<" << ctype(0) << ", " << M << ", " << N << ", " << K << ", " << group << ", " << flag(zeros) << ", " << wk << ", " << flag(read_in_kernel(prog, ins))
-           << ">::unit(unit, " << x << ", " << w << ", " << s << ", " << z << ", " << out << ", smem);";
-      f.smem_bytes = wk > 1 ? static_cast<int>(ls.waves() * mt * 1024) : 0;
-      check_units((tiles + per - 1) / per * ((M + 16 * mt - 1) / (16 * mt)));
+      body << "Matvec::unit(unit, " << x << ", " << w << ", " << s << ", " << z << ", " << (parts_stage ? "nullptr, " + out : out + ", nullptr") << ", smem);";
+      const int64_t at_once = ls.waves() / p.wk, row_blocks = p.row_blocks();
+      f.smem_bytes = static_cast<int>((p.wk > 1 ? ls.waves() * row_blocks * 1024 : 0) + p.x_bytes());
+      check_units(((p.N + 15) / 16 + at_once - 1) / at_once * p.sk * ((p.M + 16 * row_blocks - 1) / (16 * row_blocks)));
+      body << " static_assert(Matvec::lds_bytes() == " << f.smem_bytes << " && Matvec::num_units() == " << f.num_units << ", \"launch\");";
       break;
     }
     default: MONONN_FAIL(kInternal) << node.name << " is not an operator";

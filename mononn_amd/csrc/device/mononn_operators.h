@@ -15,6 +15,11 @@ typedef short mononn_short4 __attribute__((ext_vector_type(4)));
 #define MONONN_LDS_READ_TR16(p) __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) mononn_short4*)(p))
 #endif
 
+// an empty statement after which the compiler has the constant `v` in a vector register (and may still share or move it)
+#ifndef MONONN_KEEP_IN_VGPR
+#define MONONN_KEEP_IN_VGPR(v) asm("" : "+v"(v))
+#endif
+
 namespace mononn_dev {
 
 template <class T>
@@ -987,24 +992,32 @@ struct PagedAttention {
 // y[m, n] = sum over groups of scale[n, group] * sum over k of (w[n, k] - zero[n, group]) * x[m, k], weights two to a
 // byte along k (the low half is the lower k), zero = 8 without a tensor of zero points.
 //
-// A wave takes 16 weight rows and walks k in chunks of 128: one 16-byte load per lane, lane (r, g) = row r, weights 32 g ..
-// 32 g + 31.  A 4 x 4 transposition of dwords between the four lane groups gives each contraction step of
-// v_mfma_f32_16x16x32 32 consecutive k, so that a step never crosses a group of 32 and a lane's result column is one
-// weight row with one scale.  Weights enter the product as small integers, exactly; scales are applied to its f32 result.
+// Bound by the reads of the weights as long as a byte of them costs few instructions.  A wave takes 16 weight rows; lane
+// (r, g) = (lane % 16, lane / 16) reads row r, of every 128 P columns the 32 P that belong to its lane group g, in P
+// pieces of 16 bytes.  The products run on v_mfma_f32_16x16x32 with x as the left operand and the weights, small
+// integers and so exact, as the right one: a lane's result column is one weight row, scales are applied to f32 results.
+// A contraction step takes 8 columns from each lane group, so the groups' scales must not meet in it:
+//   kSpread  M <= 4: the 16 rows of the left operand hold x once per lane group, with zeros for the other groups'
+//            columns.  Result row 4 g + m then is lane group g's share of row m, in the lanes that hold its scales.
+//   kWhole   groups of 128 columns or more, P = 1: all four lane groups share a scale.
+//   kSwap    otherwise: a 4 x 4 transposition of dwords between the lane groups gives every step 32 consecutive columns.
 template <class T>
 struct Nibbles;
 template <>
 struct Nibbles<half_t> {
   static constexpr int kBias = 8;   // subtracted on the way
-  // 1024 + v in f16 by setting exponent bits, v = (w >> s) & 15 in the last places; elements 0, 4, 1, 5, 2, 6, 3, 7 of the dword
+  // (w >> s) & 15 in f16 by setting exponent bits: 1024 + v where the four bits are the last of the mantissa, 64 + v where
+  // they stand four places higher; elements 0, 4, 1, 5, 2, 6, 3, 7 of the dword
   static __device__ __forceinline__ half8_t operands(unsigned w) {
     half8_t r;
-    const half2_t one = {(half_t)1032.0f, (half_t)1032.0f}, sixteenth = {(half_t)0.0625f, (half_t)0.0625f}, high = {(half_t)72.0f, (half_t)72.0f};
+    unsigned low = 0x64006400u, high = 0x54005400u;   // in vector registers: one instruction then masks and sets (two constants would need two)
+    MONONN_KEEP_IN_VGPR(low);
+    MONONN_KEEP_IN_VGPR(high);
+    const half2_t l8 = {(half_t)1032.0f, (half_t)1032.0f}, h8 = {(half_t)72.0f, (half_t)72.0f};
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const unsigned x = i ? w >> 8 : w;
-      const half2_t lo = __builtin_bit_cast(half2_t, (x & 0x000f000fu) | 0x64006400u) - one;
-      const half2_t hi = __builtin_elementwise_fma(__builtin_bit_cast(half2_t, (x & 0x00f000f0u) | 0x64006400u), sixteenth, -high);
+      const half2_t lo = __builtin_bit_cast(half2_t, (x & 0x000f000fu) | low) - l8, hi = __builtin_bit_cast(half2_t, (x & 0x00f000f0u) | high) - h8;
       r[4 * i] = lo[0], r[4 * i + 1] = lo[1], r[4 * i + 2] = hi[0], r[4 * i + 3] = hi[1];
     }
     return r;
@@ -1015,8 +1028,10 @@ struct Nibbles<__bf16> {
   static constexpr int kBias = -128;   // 128 + v: there is no packed bf16 subtraction, the sum of x takes it out again
   static __device__ __forceinline__ half8_t operands(unsigned w) {
     struct { unsigned d[4]; } r;
+    unsigned bits = 0x43004300u;
+    MONONN_KEEP_IN_VGPR(bits);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r.d[i] = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+    for (int i = 0; i < 4; ++i) r.d[i] = ((w >> (4 * i)) & 0x000f000fu) | bits;
     return __builtin_bit_cast(half8_t, r);
   }
 };
@@ -1042,96 +1057,179 @@ __device__ __forceinline__ void transpose_lane_groups(unsigned (&d)[4]) {
   swap16(d[2], d[3]);
 }
 
-template <class T, int M, int N, int K, int GROUP, bool ZEROS, int WK, bool COHERENT>
+// WK waves of a workgroup share a tile of 16 weight rows by splitting the columns; SK workgroups do where x does not fit
+// one's LDS (`parts`, added up by `join`)
+template <class T, int M, int N, int K, int GROUP, bool ZEROS, int WK, int SK, int P, bool COHERENT>
 struct MatvecW4 {
   static constexpr int NW = MONONN_BLOCK_SIZE / kWaveSize;
   static constexpr int TILES = NW / WK;                       // tiles of 16 weight rows a workgroup takes at once
   static constexpr int MT = (M + 15) / 16 < 4 ? (M + 15) / 16 : 4;   // blocks of 16 rows of x per pass over the weights
-  static constexpr int CHUNKS = (K + 127) / 128;
-  static constexpr int MINE = (CHUNKS + WK - 1) / WK;         // chunks of a wave (consecutive)
-  static constexpr int DEPTH = MINE < 8 ? MINE : 8;           // chunks in flight
+  static constexpr int XROWS = M < 16 * MT ? M : 16 * MT;     // rows of x in a pass
+  static constexpr bool kSpread = M <= 4, kWhole = !kSpread && GROUP >= 128, kSwap = !kSpread && !kWhole;
+  static_assert(!kWhole || P == 1, "the lane groups of a step share a scale");
+  static constexpr int BLOCK = 128 * P;                       // columns a wave reads at a time
+  static constexpr int BLOCKS = (K + BLOCK - 1) / BLOCK;
+  static constexpr int PER_GROUP = (BLOCKS + SK - 1) / SK;    // blocks of a workgroup
+  static constexpr int MINE = (PER_GROUP + WK - 1) / WK;      // blocks of a wave (consecutive)
   static constexpr int GROUPS = K / GROUP;
-  static constexpr int PER_CHUNK = GROUP >= 128 ? 1 : 128 / GROUP;   // scales of a row in a chunk
-  static constexpr int STEPS = 4 / PER_CHUNK;                 // contraction steps per scale
+  static constexpr int SCALES = kSwap ? BLOCK / GROUP : (kSpread && 32 * P > GROUP ? 32 * P / GROUP : 1);   // scales of a block that a lane needs
+  static constexpr int AHEAD = 8 / P;
+  static constexpr int DEPTH = MINE < AHEAD ? MINE : AHEAD;   // blocks in flight
   static constexpr bool kBf16 = IsBf16<T>::value;
   static constexpr bool kSums = ZEROS || Nibbles<T>::kBias != 8;
-  static constexpr int ROWS = M < 4 ? M : 4;                  // result rows a lane looks at: row 4 * (lane / 16) + i
-  static constexpr int num_units() { return ((N + 15) / 16 + TILES - 1) / TILES * ((M + 16 * MT - 1) / (16 * MT)); }
-  static constexpr int lds_bytes() { return WK > 1 ? NW * MT * 1024 : 0; }
+  static constexpr int ROWS = M < 4 ? M : 4;                  // result rows a lane looks at
+  static constexpr int kShareBytes = WK > 1 ? NW * MT * 1024 : 0;
+  static constexpr int kPieces = PER_GROUP * BLOCK / 8;       // x in LDS: [piece of 8 columns][row][8], elements in the operands' order
+  static constexpr int ROW_UNITS = ((N + 15) / 16 + TILES - 1) / TILES;
+  static constexpr int num_units() { return ROW_UNITS * SK * ((M + 16 * MT - 1) / (16 * MT)); }
+  static constexpr int XPITCH = XROWS % 2 == 0 ? XROWS + 1 : XROWS;   // an odd number of 16-byte cells per piece: columns of cells fall on different banks
+  static constexpr int lds_bytes() { return kShareBytes + kPieces * XPITCH * 16; }
 
-  struct Chunk {
-    unsigned w[4];
-    T scale[PER_CHUNK];
-    unsigned char zero[PER_CHUNK];
+  struct Scales { T v[SCALES]; };
+  struct Zeros { unsigned char v[SCALES]; };
+  struct Weights {
+    int4_t w[P];
+    Scales scale;
+    Zeros zero;
   };
-  static __device__ __forceinline__ void load(const unsigned char* weight, const T* scale, const unsigned char* zero, long row, int chunk, Chunk& c) {
-    const int g = lane_id() >> 4;
-    int at = chunk * 64 + g * 16;
-    if (K % 128 != 0 && at > K / 2 - 16) at = K / 2 - 16;     // behind the last column: any weights, x is zero there
-    typedef unsigned u4 __attribute__((ext_vector_type(4)));
-    const u4 w = *reinterpret_cast<const u4*>(weight + row * (K / 2) + at);
-    c.w[0] = w[0], c.w[1] = w[1], c.w[2] = w[2], c.w[3] = w[3];
+  // what a lane needs of `E`[N, GROUPS] for a block
+  template <class V, class E>
+  static __device__ __forceinline__ V load_groups(const E* p, long row, int block) {
+    const int first = kSpread ? (block * BLOCK + (lane_id() >> 4) * 32 * P) / GROUP : block * BLOCK / GROUP;
+    V r;
+    if constexpr (K % BLOCK == 0) {
+      struct alignas(sizeof(V)) Run { V v; };
+      r = reinterpret_cast<const Run*>(p + row * GROUPS + first)->v;
+    } else {
 #pragma unroll
-    for (int i = 0; i < PER_CHUNK; ++i) {
-      int at_group = GROUP >= 128 ? chunk / (GROUP / 128 > 0 ? GROUP / 128 : 1) : chunk * PER_CHUNK + i;
-      if (at_group > GROUPS - 1) at_group = GROUPS - 1;
-      c.scale[i] = scale[row * GROUPS + at_group];
-      if constexpr (ZEROS) c.zero[i] = zero[row * GROUPS + at_group];
+      for (int i = 0; i < SCALES; ++i) r.v[i] = p[row * GROUPS + (first + i < GROUPS ? first + i : GROUPS - 1)];
+    }
+    return r;
+  }
+  static __device__ __forceinline__ void load(const unsigned char* weight, const T* scale, const unsigned char* zero, long row, int block, Weights& c) {
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      int at = block * (BLOCK / 2) + (lane_id() >> 4) * 16 * P + i * 16;
+      if (K % BLOCK != 0 && at > K / 2 - 16) at = K / 2 - 16;     // behind the last column: any weights, x is zero there
+      c.w[i] = *reinterpret_cast<const int4_t*>(weight + row * (K / 2) + at);
+    }
+    c.scale = load_groups<Scales>(scale, row, block);
+    if constexpr (ZEROS) c.zero = load_groups<Zeros>(zero, row, block);
+  }
+  static __device__ __forceinline__ void stage_x(const T* x, int m0, int piece0, half8_t* xs) {
+    for (int i = thread_id(); i < kPieces * XROWS; i += MONONN_BLOCK_SIZE) {
+      const int piece = i % kPieces, m = i / kPieces;   // neighbouring threads read along a row
+      half8_t v = {0, 0, 0, 0, 0, 0, 0, 0};
+      if (m0 + m < M && (piece0 + piece) * 8 < K) v = nibble_order(*reinterpret_cast<const half8_t*>(x + (long)(m0 + m) * K + (piece0 + piece) * 8));
+      xs[piece * XPITCH + m] = v;
     }
   }
+  // left operands of piece i of a block, for its four steps; `a` keeps its zeros in the lanes that hold no x
+  static __device__ __forceinline__ void x_operands(const half8_t* xs, int block, int i, half8_t (&a)[MT][4]) {
+    const int g = lane_id() >> 4, r16 = lane_id() & 15;
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        // first column of the lane's 8: of its own lane group's, or of the 32 that step k holds after the transposition
+        const int piece = block * (BLOCK / 8) + (kSwap ? k * 4 * P + i * 4 + g : g * 4 * P + i * 4 + k);
+        if constexpr (kSpread) {
+          if (r16 >> 2 == g && (r16 & 3) < M) a[t][k] = xs[piece * XPITCH + (r16 & 3)];
+        } else {
+          const int m = t * 16 + r16 < XROWS ? t * 16 + r16 : XROWS - 1;   // rows behind the last: some row, the results are not stored
+          a[t][k] = xs[piece * XPITCH + m];
+        }
+      }
+  }
 
-  static __device__ __forceinline__ void unit(int unit, const T* x, const unsigned char* weight, const T* scale, const unsigned char* zero, T* y, char* smem) {
+  // result: y, or with SK > 1 the f32 partial sums [SK][M][N]
+  static __device__ __forceinline__ void unit(int unit, const T* x, const unsigned char* weight, const T* scale, const unsigned char* zero, T* y, float* parts, char* smem) {
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), g = lane >> 4, r16 = lane & 15;
-    constexpr int ROW_UNITS = ((N + 15) / 16 + TILES - 1) / TILES;
-    const int pass = unit / ROW_UNITS, tile = unit % ROW_UNITS * TILES + wave / WK, part = wave % WK;
+    const int pass = unit / (ROW_UNITS * SK), slice = unit / ROW_UNITS % SK, tile = unit % ROW_UNITS * TILES + wave / WK, part = wave % WK;
     const int n = tile * 16 + r16, m0 = pass * 16 * MT;
     const long row = n < N ? n : N - 1;
-    const int c0 = part * MINE, c1 = c0 + MINE < CHUNKS ? c0 + MINE : CHUNKS;
+    const int first = slice * PER_GROUP, b0 = first + part * MINE;
+    const int behind = first + PER_GROUP < BLOCKS ? first + PER_GROUP : BLOCKS, count = clamp_int(behind - b0, 0, MINE);
+    half8_t* xs = reinterpret_cast<half8_t*>(smem + kShareBytes);
+    __syncthreads();   // the rows of the unit before
+    Weights ring[DEPTH];
+    auto block_at = [&](int i) { return clamp_int(b0 + (i < count ? i : count - 1), 0, BLOCKS - 1); };   // the last one again behind the end
+    stage_x(x, m0, first * (BLOCK / 8), xs);
+#pragma unroll
+    for (int i = 0; i < DEPTH; ++i) load(weight, scale, zero, row, block_at(i), ring[i]);
     float4_t acc[MT];
+    half8_t a[2][MT][4];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) acc[t] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    Chunk ring[DEPTH];
+    for (int t = 0; t < MT; ++t) {
+      acc[t] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < DEPTH; ++i) load(weight, scale, zero, row, c0 + i < CHUNKS ? c0 + i : CHUNKS - 1, ring[i]);
-    for (int base = c0; base < c1; base += DEPTH) {
+      for (int k = 0; k < 4; ++k) a[0][t][k] = a[1][t][k] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
+    }
+    __syncthreads();
+    x_operands(xs, block_at(0) - first, 0, a[0]);
+    for (int base = 0; base < count; base += DEPTH) {
 #pragma unroll
       for (int i = 0; i < DEPTH; ++i) {
-        const int c = base + i;
-        if (c >= c1) break;
-        Chunk ch = ring[i];
-        if (c + DEPTH < c1) load(weight, scale, zero, row, c + DEPTH, ring[i]);
-        transpose_lane_groups(ch.w);
+        if (base + i >= count) break;
+        const Weights c = ring[i];
+        load(weight, scale, zero, row, block_at(base + i + DEPTH), ring[i]);
+        constexpr int SETS = kSwap ? 4 : 1;   // results with scales of their own
+        float4_t dot[MT][SETS], sum[MT][SETS];
 #pragma unroll
-        for (int p = 0; p < PER_CHUNK; ++p) {
-          const float s = (float)ch.scale[p];
-          const float z = ZEROS ? (float)((int)ch.zero[p] - Nibbles<T>::kBias) : (float)(8 - Nibbles<T>::kBias);
+        for (int j = 0; j < P; ++j) {
+          constexpr bool kAlternate = (DEPTH * P) % 2 == 0;   // operands one piece ahead, in the other set of registers
+          half8_t(&now)[MT][4] = a[kAlternate ? (i * P + j) % 2 : 0];
+          half8_t(&ahead)[MT][4] = a[kAlternate ? (i * P + j + 1) % 2 : 1];
+          x_operands(xs, (j + 1 < P ? block_at(base + i) : block_at(base + i + 1)) - first, (j + 1) % P, ahead);
+          unsigned w[4] = {(unsigned)c.w[j][0], (unsigned)c.w[j][1], (unsigned)c.w[j][2], (unsigned)c.w[j][3]};
+          if constexpr (kSwap) transpose_lane_groups(w);
+          // the first product of a set starts from zero; a set ends where its columns end a group, or with the block
+          const bool fresh = j == 0 || (32 * j) % GROUP == 0, done = (32 * (j + 1)) % GROUP == 0 || j + 1 == P;
 #pragma unroll
-          for (int t = 0; t < MT; ++t) {
-            float4_t dot = {0.0f, 0.0f, 0.0f, 0.0f}, sum = {0.0f, 0.0f, 0.0f, 0.0f};
+          for (int k = 0; k < 4; ++k) {
+            const half8_t b = Nibbles<T>::operands(w[k]);
+            constexpr float4_t kZero = {0.0f, 0.0f, 0.0f, 0.0f};
+            const int set = kSwap ? k : 0;
+            const bool start = fresh && (kSwap || k == 0);
 #pragma unroll
-            for (int k = 0; k < STEPS; ++k) {
-              const int step = p * STEPS + k, at = c * 128 + step * 32 + g * 8, m = m0 + t * 16 + r16;
-              half8_t a = {0, 0, 0, 0, 0, 0, 0, 0};
-              if (m < M && (K % 128 == 0 || at < K)) a = nibble_order(*reinterpret_cast<const half8_t*>(x + (long)m * K + at));
-              dot = mfma_16x16x32<kBf16>(a, Nibbles<T>::operands(ch.w[step]), dot);
+            for (int t = 0; t < MT; ++t) {
+              dot[t][set] = mfma_16x16x32<kBf16>(now[t][k], b, start ? kZero : dot[t][set]);
               if constexpr (kSums) {
-                const T one = (T)1.0f;
-                const half_t o = __builtin_bit_cast(half_t, one);
-                sum = mfma_16x16x32<kBf16>(a, half8_t{o, o, o, o, o, o, o, o}, sum);
+                const half_t o = __builtin_bit_cast(half_t, (T)1.0f);
+                sum[t][set] = mfma_16x16x32<kBf16>(now[t][k], half8_t{o, o, o, o, o, o, o, o}, start ? kZero : sum[t][set]);
               }
             }
+          }
+          if (done) {
 #pragma unroll
-            for (int i = 0; i < ROWS; ++i) {
-              if constexpr (kSums) acc[t][i] += s * (dot[i] - z * sum[i]);
-              else acc[t][i] += s * dot[i];
+            for (int q = 0; q < SETS; ++q) {
+              const int at = kSwap ? (q * 32 * P + 32 * j) / GROUP : (kSpread ? 32 * j / GROUP : 0);
+              const float s = (float)c.scale.v[at];
+              const float z = ZEROS ? (float)((int)c.zero.v[at] - Nibbles<T>::kBias) : (float)(8 - Nibbles<T>::kBias);
+#pragma unroll
+              for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int e = 0; e < ROWS; ++e) {
+                  if constexpr (kSums) acc[t][e] += s * (dot[t][q][e] - z * sum[t][q][e]);
+                  else acc[t][e] += s * dot[t][q][e];
+                }
             }
+          }
+          if constexpr (!kAlternate) {
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+              for (int k = 0; k < 4; ++k) a[0][t][k] = a[1][t][k];
           }
         }
       }
     }
+    if constexpr (kSpread) {   // the lane groups' shares
+#pragma unroll
+      for (int e = 0; e < ROWS; ++e) acc[0][e] = quarter_waves_sum(half_waves_sum(acc[0][e]));
+    }
     if constexpr (WK > 1) {
       float* shares = reinterpret_cast<float*>(smem);
-      __syncthreads();
 #pragma unroll
       for (int t = 0; t < MT; ++t) *reinterpret_cast<float4_t*>(shares + ((wave * MT + t) * 64 + lane) * 4) = acc[t];
       __syncthreads();
@@ -1146,14 +1244,28 @@ struct MatvecW4 {
 #pragma unroll
       for (int t = 0; t < MT; ++t)
 #pragma unroll
-        for (int i = 0; i < ROWS; ++i) {
-          const int m = m0 + t * 16 + 4 * g + i;
-          if (m < M) {
-            const T v[1] = {(T)acc[t][i]};
+        for (int e = 0; e < ROWS; ++e) {
+          const int m = kSpread ? e : m0 + t * 16 + 4 * g + e;
+          if (m >= M || (kSpread && g != 0)) continue;
+          if constexpr (SK > 1) {
+            st1(parts + ((long)slice * M + m) * N + n, acc[t][e]);
+          } else {
+            const T v[1] = {(T)acc[t][e]};
             store_run<COHERENT, T, 1>(y + (long)m * N + n, v);
           }
         }
     }
+  }
+
+  static constexpr int join_units() { return (M * N + MONONN_BLOCK_SIZE - 1) / MONONN_BLOCK_SIZE; }
+  static __device__ __forceinline__ void join(int unit, const float* parts, T* y) {
+    const long i = (long)unit * MONONN_BLOCK_SIZE + thread_id();
+    if (i >= (long)M * N) return;
+    float v = parts[i];
+#pragma unroll
+    for (int s = 1; s < SK; ++s) v += parts[(long)s * M * N + i];
+    const T r[1] = {(T)v};
+    store_run<COHERENT, T, 1>(y + i, r);
   }
 };
 

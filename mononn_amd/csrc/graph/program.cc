@@ -739,7 +739,8 @@ struct Builder {
       const Instr* ins = n.members[0];
       if (ins->oper.kind == hlo::OperatorConfig::kKvAppend)
         for (auto* v : n.outputs) p.in_place[v] = ins->operands[v->tuple_index == 0 ? 2 : 3];
-      if (ins->oper.kind == hlo::OperatorConfig::kPagedAttentionParts) p.temp_size[ins] = codegen::paged_attention_part_bytes(ins, opt.grid, opt.waves);
+      if (ins->oper.kind == hlo::OperatorConfig::kPagedAttentionParts || ins->oper.kind == hlo::OperatorConfig::kMatvecW4Parts)
+        p.temp_size[ins] = codegen::operator_part_bytes(ins, opt.grid, opt.waves);
     }
   }
 

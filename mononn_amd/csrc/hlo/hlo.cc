@@ -1217,13 +1217,15 @@ void lower_lt_matmul_epilogues(Module* mod) {
   }
 }
 
-// A paged_attention call becomes two instructions, each a stage of its own: the parts, f32[2 x workgroups, floats of a
-// part] (sized by the code generator, which knows the launch), and the call, which joins them.
-void split_paged_attention(Module* mod) {
+// Calls that become two instructions, each a stage of its own: the parts (partial results in memory, sized by the code
+// generator, which knows the launch), and the call, which joins them.
+void split_operators(Module* mod) {
   Computation* comp = mod->entry;
   for (size_t at = 0; at < comp->instrs.size(); ++at) {
     Instr* call = comp->instrs[at].get();
-    if (call->oper.kind != OperatorConfig::kPagedAttention) continue;
+    const bool attention = call->oper.kind == OperatorConfig::kPagedAttention;
+    const bool matvec = call->oper.kind == OperatorConfig::kMatvecW4 && matvec_w4_in_parts(call->operands[0]->shape.dims[0], call->operands[0]->shape.dims[1]);
+    if (!attention && !matvec) continue;
     auto up = std::make_unique<Instr>();
     Instr* parts = up.get();
     parts->name = call->name + "_parts";
@@ -1231,7 +1233,7 @@ void split_paged_attention(Module* mod) {
     parts->opcode = "custom-call";
     parts->custom_call_target = call->custom_call_target;
     parts->oper = call->oper;
-    parts->oper.kind = OperatorConfig::kPagedAttentionParts;
+    parts->oper.kind = attention ? OperatorConfig::kPagedAttentionParts : OperatorConfig::kMatvecW4Parts;
     parts->shape.dtype = DType::kF32;
     parts->shape.dims = {1};
     parts->shape.minor_to_major = {0};
@@ -1243,7 +1245,8 @@ void split_paged_attention(Module* mod) {
     }
     for (auto* o : parts->operands)
       if (std::find(o->users.begin(), o->users.end(), parts) == o->users.end()) o->users.push_back(parts);
-    call->operands = {parts, parts->operands[4], parts->operands[5]};
+    call->operands = {parts};
+    if (attention) call->operands.insert(call->operands.end(), {parts->operands[4], parts->operands[5]});
     for (auto* o : call->operands)
       if (std::find(o->users.begin(), o->users.end(), call) == o->users.end()) o->users.push_back(call);
     comp->instrs.insert(comp->instrs.begin() + static_cast<long>(at), std::move(up));
@@ -1251,6 +1254,8 @@ void split_paged_attention(Module* mod) {
   }
   for (size_t i = 0; i < comp->instrs.size(); ++i) comp->instrs[i]->index_in_comp = static_cast<int>(i);
 }
+
+bool matvec_w4_in_parts(int64_t rows, int64_t columns) { return (columns + 127) / 128 * 256 * std::min<int64_t>(rows, 64) > kMatvecW4RowBytes; }
 
 std::unique_ptr<Module> parse_module(const std::string& text) {
   auto mod = std::make_unique<Module>();
@@ -1392,7 +1397,7 @@ std::unique_ptr<Module> parse_module(const std::string& text) {
               << ins->hlo_name << ": the cache " << ins->operands[i]->hlo_name << " is updated in place and may be read by nothing else than this call; read its result instead";
         }
     }
-  split_paged_attention(mod.get());
+  split_operators(mod.get());
   return mod;
 }
 

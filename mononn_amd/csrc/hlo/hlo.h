@@ -72,15 +72,20 @@ struct ConvConfig {
 //   mononn$paged_attention  (q[T,HQ,D], k_cache, v_cache, page_table, query_start, context_len) -> [T,HQ,D]
 //   mononn$matvec_w4        (x[M,K], weight u8[N,K/2], scales[N,K/group][, zeros u8[N,K/group]]) -> [M,N]
 // kPagedAttentionParts is what the parser splits off a paged_attention call: the stage that works through the keys and
-// leaves partial results, which the call itself then joins.
+// leaves partial results, which the call itself then joins.  kMatvecW4Parts likewise, for matvec_w4 calls whose x does
+// not fit a workgroup's LDS.
 struct OperatorConfig {
-  enum Kind { kNone, kRope, kKvAppend, kPagedAttention, kPagedAttentionParts, kMatvecW4 };
+  enum Kind { kNone, kRope, kKvAppend, kPagedAttention, kPagedAttentionParts, kMatvecW4, kMatvecW4Parts };
   Kind kind = kNone;
   double amplitude = 1;      // rope, kv_append: factor on cosine and sine
   bool interleaved = false;  // rope, kv_append: pairs (2i, 2i+1) instead of (i, i + R/2)
   double scale = 1;          // paged_attention: factor on the scores
   int64_t window = 0;        // paged_attention: keys a query sees, itself included; 0 = all before it
 };
+
+// LDS that a workgroup of matvec_w4 gives to x: its rows for all columns, or a slice of the columns
+constexpr int64_t kMatvecW4RowBytes = 96 * 1024;
+bool matvec_w4_in_parts(int64_t rows, int64_t columns);
 
 struct Instr {
   std::string name;            // canonical: '.' and '-' replaced by '_' (string_helpers.cc:22-32)

@@ -3,6 +3,7 @@
 #pragma once
 #include "../../host_builtins.h"
 #define MONONN_ONE_THREAD
+#define MONONN_KEEP_IN_VGPR(v) ((void)0)
 typedef short mononn_short4 __attribute__((ext_vector_type(4)));
 inline mononn_short4 host_lds_read8(const char* p) {
   mononn_short4 v;
