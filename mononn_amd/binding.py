@@ -234,6 +234,10 @@ class MonoNNModule:
         arr = (ctypes.c_void_p * len(device_ptrs))(*device_ptrs)
         _check(_lib.mononn_launch(self._h, arr, len(device_ptrs), ctypes.c_void_p(stream)))
 
+    def launch_arguments(self, arguments: "ctypes.Array", stream: int = 0):
+        """launch_raw with the pointers in a ctypes array of c_void_p that the caller keeps."""
+        _check(_lib.mononn_launch(self._h, arguments, len(arguments), stream))
+
     def launch_static_temp(self, device_ptrs: Sequence[int], stream: int = 0):
         """mononn_launch_static_temp: parameters and live-outs only; the temp arena is the library's static device array."""
         arr = (ctypes.c_void_p * len(device_ptrs))(*device_ptrs)

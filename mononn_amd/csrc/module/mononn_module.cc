@@ -73,6 +73,19 @@ void MonoNNModule::generate_code() {
     }
     kernel_name_ = "mononn_" + shortn;
   }
+  if (!spec_given_) {
+    // Default launch: four waves per compute unit, eight when every node is an operator call.  Their kernels hide the
+    // memory's latency and the soft-max behind a second wave per SIMD (256 -> 512 threads: attention of prompt chunks
+    // 900 -> 533 us, of one token over 131071 keys 116 -> 106); GEMM tiles want the registers of one (the 12-layer
+    // decoder step of four tokens 445 -> 795 us).
+    bool operators = false, others = false;
+    for (auto& up : mod->entry->instrs) {
+      const hlo::Instr& i = *up;
+      if (i.is_operator()) operators = true;
+      else if (i.opcode != "parameter" && i.opcode != "constant" && i.opcode != "tuple" && i.opcode != "get-tuple-element" && !graph::is_alias_op(&i)) others = true;
+    }
+    if (operators && !others) spec_.runtime.block_dim.x = 512;
+  }
   // MONONN_CODEGEN_ALLOW_LIST_OVERRIDE (mononn_module.cc:62-89)
   auto override_list = env::allow_list_override();
   if (!override_list.empty()) spec_.codegen_allow_list = override_list;

@@ -10,6 +10,7 @@ torch is used for device memory and the stream only; all arithmetic happens in t
 """
 from __future__ import annotations
 
+import ctypes
 from typing import Dict, List, Sequence
 
 import torch
@@ -38,38 +39,53 @@ class MonoNNFunction:
         self._in_place = module.liveout_parameters()   # live-outs that are an input tensor, updated by the call
         assert len(self._out_bytes) == len(self.outputs), "one {dtype, dims} entry per live-out is required"
         self._temp = None if module.owns_temp else torch.zeros(max(info["temp"], 256), dtype=torch.uint8, device=self.device)
+        # what a call fills in: the kernel's arguments, in order (parameters, live-outs, temp)
+        self._args = (ctypes.c_void_p * (len(self._param_bytes) + len(self._out_bytes) + 1))()
+        self._args[len(self._args) - 1] = 0 if self._temp is None else self._temp.data_ptr()
+        self._results = [(tuple(o["dims"]), _TORCH_DTYPE[o["dtype"]], p) for o, p in zip(self.outputs, self._in_place)]
+        for (dims, dtype, _), nbytes in zip(self._results, self._out_bytes):
+            assert torch.empty(dims, dtype=dtype, device="meta").nbytes == nbytes
         self.handle = id(self)
         _REGISTRY[self.handle] = self
 
     def close(self):
         _REGISTRY.pop(self.handle, None)
 
+    def _input(self, i: int, t: torch.Tensor) -> torch.Tensor:
+        """Parameter i from a tensor that is not simply the parameter's bytes: made contiguous, or refused."""
+        assert t.is_cuda and t.device == self.device, "inputs must live on the module's GPU"
+        assert t.is_contiguous() or i not in self._in_place, "an input that the call updates in place must be contiguous"
+        t = t.contiguous()
+        nbytes = self._param_bytes[i]
+        assert t.numel() * t.element_size() == nbytes, f"parameter needs {nbytes} bytes, got {t.numel() * t.element_size()}"
+        assert t.data_ptr() % 16 == 0, "buffers must be 16-byte aligned"
+        return t
+
     def __call__(self, *inputs: torch.Tensor) -> List[torch.Tensor]:
+        # A call is a few microseconds of GPU work for the smallest modules, so the common case (tensors that can be
+        # handed over as they are) does nothing twice.
         assert len(inputs) == len(self._param_bytes), f"expected {len(self._param_bytes)} tensors"
-        held = []
-        ptrs = []
+        args, device, held = self._args, self.device, list(inputs)
         for i, (t, nbytes) in enumerate(zip(inputs, self._param_bytes)):
-            assert t.is_cuda and t.device == self.device, "inputs must live on the module's GPU"
-            assert t.is_contiguous() or i not in self._in_place, "an input that the call updates in place must be contiguous"
-            t = t.contiguous()
-            assert t.numel() * t.element_size() == nbytes, f"parameter needs {nbytes} bytes, got {t.numel() * t.element_size()}"
-            assert t.data_ptr() % 16 == 0, "buffers must be 16-byte aligned"
-            held.append(t)
-            ptrs.append(t.data_ptr())
+            ptr = t.data_ptr()
+            if ptr % 16 or t.nbytes != nbytes or t.device != device or not t.is_contiguous():
+                held[i] = t = self._input(i, t)
+                ptr = t.data_ptr()
+            args[i] = ptr
         outs = []
-        for o, nbytes, param in zip(self.outputs, self._out_bytes, self._in_place):
+        at = len(inputs)
+        for dims, dtype, param in self._results:
             if param >= 0:
-                assert held[param].dtype == _TORCH_DTYPE[o["dtype"]] and list(held[param].shape) == list(o["dims"]), "an input that the call updates in place must have the declared type and shape"
-                outs.append(held[param])
-                ptrs.append(0)
-                continue
-            t = torch.empty(o["dims"], dtype=_TORCH_DTYPE[o["dtype"]], device=self.device)
-            assert t.numel() * t.element_size() == nbytes
+                t = held[param]
+                assert t.dtype == dtype and t.shape == dims, "an input that the call updates in place must have the declared type and shape"
+                args[at] = None
+            else:
+                t = torch.empty(dims, dtype=dtype, device=device)
+                args[at] = t.data_ptr()
             outs.append(t)
-            ptrs.append(t.data_ptr())
-        ptrs.append(0 if self._temp is None else self._temp.data_ptr())
-        stream = torch.cuda.current_stream(self.device).cuda_stream
-        self.module.launch_raw(ptrs, stream)
+            at += 1
+        stream = torch._C._cuda_getCurrentRawStream(device.index)   # what torch.cuda.current_stream(device).cuda_stream says, without the stream object
+        self.module.launch_arguments(args, stream)
         if self.checked:
             self.module.synchronize(stream)
         return outs

@@ -329,5 +329,5 @@ def test_bounds_harness_sees_the_operators(monkeypatch, tmp_path):
     ok, message = check(monkeypatch, tmp_path, text, {4: [[8] * 4, [0] * 4], 5: [0, 1, 5], 6: [6, 4]}, shrink=("parameter 2", 16))
     assert not ok and "parameter 2" in message
     text, _ = dc.attention_module(4, 12, 12, 64, 30, 16, 4, 8, "f16", 0.1)
-    ok, message = check(monkeypatch, tmp_path, text, {3: [[29] * 8] * 4, 4: [0, 1, 2, 3, 4], 5: [1, 128, 77, 0]}, grid=8, shrink=("LDS", 4096))
+    ok, message = check(monkeypatch, tmp_path, text, {3: [[29] * 8] * 4, 4: [0, 1, 2, 3, 4], 5: [1, 128, 77, 0]}, grid=8, block=256, shrink=("LDS", 4096))
     assert not ok and "LDS" in message
