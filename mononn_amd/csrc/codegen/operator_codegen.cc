@@ -167,7 +167,7 @@ NodeFunction generate_operator(const graph::Program& prog, const graph::Node& no
         const int64_t krow = D * 2 + 16, vrow = (D * 2 + 63) / 128 * 128 + 64, vpn = (D / 16 | 1) * 32, merge = D / 16 * 1024 + 128;
         int64_t nn = waves;
         while (nn > 1 && (nn * 32 * (krow + vpn) > limit || nn * merge > limit)) nn /= 2;
-        const int64_t wide = q[0] * (q[1] / kc[2]) <= 16 ? 0 : 2 * 64 * (krow + vrow);
+        const int64_t wide = q[0] * (q[1] / kc[2]) <= 16 ? 0 : 64 * (2 * krow + (waves >= 8 && 64 * (2 * krow + 3 * vrow) <= 160 * 1024 ? 3 : 2) * vrow);
         f.smem_bytes = static_cast<int>(std::max({wide, nn * 32 * (krow + vpn), nn * merge}));
         body << " static_assert(Attention::lds_bytes() == " << f.smem_bytes << ", \"LDS\");";
       } else {

@@ -273,13 +273,14 @@ struct PagedAttention {
   static constexpr int VP = (D * 2 + 63) / 128 * 128 + 64;
   static_assert(VP >= D * 2 && VP >= DT * 64, "value rows");
   static constexpr int kWideKeys = 64;
-  static constexpr int kWideBuffer = kWideKeys * (KP + VP);
   // narrow items: values are read 32 bytes of 8 rows per 32 lanes; an odd multiple of 32 bytes keeps 8 rows apart
   static constexpr int VPN = (D / 16 | 1) * 32;
   static constexpr int kWaveBuffer = 32 * (KP + VPN);
   static constexpr int kTiles = D / 16;          // tiles of 16 output elements of a narrow item
   static constexpr int QN = (D + 31) / 32;       // its contraction steps of the first product
   static constexpr int kLdsLimit = 160 * 1024;
+  static constexpr bool kSkew = NW >= 8 && kWideKeys * (2 * KP + 3 * VP) <= kLdsLimit;   // two waves per SIMD, and room: see wide()
+  static constexpr int kValueBuffers = kSkew ? 3 : 2;
   static constexpr int narrow_waves(int n) { return n * kWaveBuffer <= kLdsLimit && n * (kTiles * 1024 + 128) <= kLdsLimit ? n : narrow_waves(n / 2); }
   static constexpr int NN = narrow_waves(NW);    // waves that take part in a narrow item
   static constexpr int kNarrowKeys = 32 * NN;
@@ -289,7 +290,7 @@ struct PagedAttention {
   static constexpr int kPart = kAllNarrow ? kPartNarrow : NW * kPartWave;   // floats of one partial result; two per workgroup
   static constexpr int kMergeBytes = NN * (kTiles * 1024 + 128);
   static constexpr int lds_bytes() {
-    int n = kAllNarrow ? 0 : 2 * kWideBuffer;
+    int n = kAllNarrow ? 0 : kWideKeys * (2 * KP + kValueBuffers * VP);
     if (NN * kWaveBuffer > n) n = NN * kWaveBuffer;
     return kMergeBytes > n ? kMergeBytes : n;
   }
@@ -440,30 +441,57 @@ struct PagedAttention {
   // The pieces of consecutive rows are dealt to the lanes in order.  Lane l fetches the page of row l of a step (one
   // load, a step ahead); where the 64 / CPR rows of an instruction lie in one page its number is the same for the
   // whole wave, and the rows' addresses are a scalar base and a lane offset that never changes.
-  static constexpr int kRowsPerRun = kWaveSize / CPR;
-  static constexpr bool kUniformRows = kWaveSize % CPR == 0 && PAGE % (kWaveSize / CPR) == 0;
-  static __device__ __forceinline__ int lane_page(const int* table, int b, int key0) {
-    const int key = clamp_int(key0 + lane_id(), 0, MAX_KEYS - 1);
-    return table[(long)b * WIDTH + key / PAGE];   // clamped to the pool where it is used: nothing waits for it here
+  // What a lane's part in that comes to is worked out once per item, not per step (Lane).
+  static constexpr bool kWholeRows = kWaveSize % CPR == 0;
+  static constexpr bool kUniformRows = kWholeRows && PAGE % (kWholeRows ? kWaveSize / CPR : 1) == 0;
+  struct Lane {
+    int lane, wave;
+    unsigned cell;   // element offset of the lane's piece from its run's first row in the cache
+    int row, piece;  // row and piece of the lane in a run that begins with a row
+    __device__ __forceinline__ Lane() {
+      lane = lane_id();
+      wave = __builtin_amdgcn_readfirstlane(wave_id());
+      row = lane / CPR, piece = lane % CPR;
+      cell = (unsigned)row * (HKV * D) + (unsigned)piece * 8;
+    }
+    // LDS byte offset of piece (first + lane) in rows of `pitch` bytes; `mine`: row * pitch + piece * 16
+    __device__ __forceinline__ int lds(int first, int pitch, int mine) const {
+      if constexpr (kWholeRows) return first / CPR * pitch + mine;
+      else return (first + lane) / CPR * pitch + (first + lane) % CPR * 16;
+    }
+    __device__ __forceinline__ int row_of(int first) const {
+      if constexpr (kWholeRows) return first / CPR + row;
+      else return (first + lane) / CPR;
+    }
+  };
+  static __device__ __forceinline__ int lane_page(const Lane& l, const int* table, int b, int key0) {
+    const int key = clamp_int(key0 + l.lane, 0, MAX_KEYS - 1);
+    return table[(long)b * WIDTH + (unsigned)key / PAGE];   // clamped to the pool where it is used: nothing waits for it here
   }
   static __device__ __forceinline__ half8_t load_piece(const T* p) { return *reinterpret_cast<const half8_t*>(p); }
-  // piece (first_piece + lane) of the keys from key0 on; `pages`: lane_page of key0
-  static __device__ __forceinline__ void load_run_of_rows(const T* kc, const T* vc, int pages, int key0, int first_piece, int h, half8_t& k, half8_t& v) {
+  static __device__ __forceinline__ int in_pool(int pages) { return clamp_int(pages, 0, PAGES - 1); }
+  // Element offset, in either cache, of piece (first + lane) of the cells from key0 on: a scalar part, and the lane's.
+  // `pages`: in_pool(lane_page of key0).
+  struct Cell {
+    unsigned long base;
+    unsigned mine;
+  };
+  static __device__ __forceinline__ Cell cell_of(const Lane& l, int pages, int key0, int first, int h) {
+    Cell c;
     if constexpr (kUniformRows) {
-      const int row0 = first_piece / CPR, key = key0 + row0;
-      const int page = clamp_int(__builtin_amdgcn_readlane(pages, row0 & (kWaveSize - 1)), 0, PAGES - 1);
-      const long base = (((long)page * PAGE + key % PAGE) * HKV + h) * D;
-      const unsigned at = (unsigned)(lane_id() / CPR) * (HKV * D) + (unsigned)(lane_id() % CPR) * 8;
-      k = load_piece(kc + base + at);
-      v = load_piece(vc + base + at);
+      const int row0 = first / CPR;
+      const unsigned page = __builtin_amdgcn_readlane(pages, row0 & (kWaveSize - 1));
+      c.base = (unsigned long)page * ((unsigned)PAGE * HKV * D) + ((unsigned)(key0 + row0) % PAGE * (HKV * D) + (unsigned)h * D);
+      c.mine = l.cell;
     } else {
-      const int at = first_piece + lane_id(), row = at / CPR, key = key0 + row;
-      const int page = clamp_int(__shfl(pages, row & (kWaveSize - 1), kWaveSize), 0, PAGES - 1);
-      const long off = (((long)page * PAGE + key % PAGE) * HKV + h) * D + at % CPR * 8;
-      k = load_piece(kc + off);
-      v = load_piece(vc + off);
+      const int row = l.row_of(first);
+      const unsigned page = __shfl(pages, row & (kWaveSize - 1), kWaveSize);
+      c.base = (unsigned long)page * ((unsigned)PAGE * HKV * D);
+      c.mine = (unsigned)(key0 + row) % PAGE * (HKV * D) + (unsigned)h * D + (kWholeRows ? l.piece : (first + l.lane) % CPR) * 8;
     }
+    return c;
   }
+  static __device__ __forceinline__ half8_t load_cell(const T* cache, const Cell& c) { return load_piece(cache + c.base + c.mine); }
 
   // the lane's query row: operand of the first product, and the keys it sees, [lo, hi]
   struct Rows {
@@ -502,31 +530,60 @@ struct PagedAttention {
     __device__ __forceinline__ void finish() { l = half_waves_sum(l); }
   };
 
-  // BLOCKS x 32 keys from LDS on 32 query rows.  `check`: some row does not see all of these keys.
-  template <int BLOCKS>
-  static __device__ __forceinline__ void step(const char* kbuf, const char* vbuf, int key0, const Rows& r, State& st, float scale_log2, bool check) {
-    const int lane = lane_id(), half = lane >> 5;
-    float16_t s[BLOCKS];
+  // The three parts of a step: 64 keys on the wave's 32 query rows.  Left to itself the compiler reads every operand of a
+  // product right in front of it and waits; here operands are read in batches of four products, a batch ahead, and nothing
+  // moves across the marks between them.
+  static constexpr int kBatch = 4;
+  typedef float16_t Scores[2];
+  typedef half8_t Probabilities[4];   // 16 keys each
+  // row: the lane's first operand; before(): work done while the first operands are on their way
+  template <class F>
+  static __device__ __forceinline__ void score(const char* row, const Rows& r, Scores& s, F before) {
+    constexpr int kProducts = 2 * QS, kBatches = (kProducts + kBatch - 1) / kBatch;   // numbered block by block of 32 keys
+    half8_t k[2][kBatch];
+    auto read = [&](int batch) {
 #pragma unroll
-    for (int b = 0; b < BLOCKS; ++b) {
+      for (int j = 0; j < kBatch; ++j) {
+        const int at = batch * kBatch + j;
+        if (at < kProducts) k[batch & 1][j] = *reinterpret_cast<const half8_t*>(row + at / QS * 32 * KP + at % QS * 32);
+      }
+    };
+    __builtin_amdgcn_s_setprio(1);
+    read(0);
+    __builtin_amdgcn_sched_barrier(0);
+    before();
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[b][i] = 0.0f;
-      const char* row = kbuf + (b * 32 + (lane & 31)) * KP + half * 16;
 #pragma unroll
-      for (int i = 0; i < QS; ++i) s[b] = mfma_32x32x16<kBf16>(*reinterpret_cast<const half8_t*>(row + i * 32), r.q[i], s[b]);
+    for (int batch = 0; batch < kBatches; ++batch) {
+      if (batch + 1 < kBatches) read(batch + 1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const int at = batch * kBatch + j;
+        if (at < kProducts) s[at / QS] = mfma_32x32x16<kBf16>(k[batch & 1][j], r.q[at % QS], s[at / QS]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
+  }
+  // `check`: some row does not see all of these keys
+  static __device__ __forceinline__ void soft_max(int key0, const Rows& r, State& st, float scale_log2, bool check, Scores& s, Probabilities& p) {
     if (check) {
 #pragma unroll
-      for (int b = 0; b < BLOCKS; ++b)
+      for (int b = 0; b < 2; ++b)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const int key = key0 + b * 32 + 8 * (i / 4) + 4 * half + i % 4;
+          const int key = key0 + b * 32 + 8 * (i / 4) + 4 * (lane_id() >> 5) + i % 4;
           s[b][i] = key >= r.lo && key <= r.hi ? s[b][i] : -__builtin_inff();
         }
     }
+    __builtin_amdgcn_s_setprio(0);
     float top = s[0][0];
 #pragma unroll
-    for (int b = 0; b < BLOCKS; ++b)
+    for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
     top = half_waves_max(top) * scale_log2;
@@ -545,29 +602,38 @@ struct PagedAttention {
     }
     // probabilities are rounded to the element type for the second product; the sum takes the unrounded ones
     float sum = 0.0f;
-    half8_t p[BLOCKS][2];
 #pragma unroll
-    for (int b = 0; b < BLOCKS; ++b)
+    for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const float e = __builtin_amdgcn_exp2f(s[b][i] * scale_log2 - st.m);
         sum += e;
-        p[b][i / 8][i % 8] = __builtin_bit_cast(half_t, (T)e);
+        p[b * 2 + i / 8][i % 8] = __builtin_bit_cast(half_t, (T)e);
       }
     st.l += sum;
-    const int i16 = lane & 15;
-    const char* vrow = vbuf + (4 * half + i16 / 4) * VP + ((lane >> 4) & 1) * 32 + (i16 & 3) * 8;
+  }
+  static __device__ __forceinline__ void weigh(const char* row, const Probabilities& p, State& st) {   // row: likewise
+    constexpr int kProducts = DT * 4, kBatches = DT;   // numbered tile by tile of 32 output elements
+    struct Pair { mononn_short4 lo, hi; };
+    Pair v[2][kBatch];
+    auto read = [&](int t) {
 #pragma unroll
-    for (int t = 0; t < DT; ++t)
+      for (int k = 0; k < 4; ++k) {
+        v[t & 1][k].lo = MONONN_LDS_READ_TR16(row + k * 16 * VP + t * 64);
+        v[t & 1][k].hi = MONONN_LDS_READ_TR16(row + (k * 16 + 8) * VP + t * 64);
+      }
+    };
+    __builtin_amdgcn_s_setprio(1);
+    read(0);
 #pragma unroll
-      for (int b = 0; b < BLOCKS; ++b)
+    for (int t = 0; t < kBatches; ++t) {
+      if (t + 1 < kBatches) read(t + 1);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          struct { mononn_short4 lo, hi; } v;
-          v.lo = MONONN_LDS_READ_TR16(vrow + (b * 32 + k * 16) * VP + t * 64);
-          v.hi = MONONN_LDS_READ_TR16(vrow + (b * 32 + k * 16 + 8) * VP + t * 64);
-          st.o[t] = mfma_32x32x16<kBf16>(__builtin_bit_cast(half8_t, v), p[b][k], st.o[t]);
-        }
+      for (int k = 0; k < 4; ++k) st.o[t] = mfma_32x32x16<kBf16>(__builtin_bit_cast(half8_t, v[t & 1][k]), p[k], st.o[t]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    static_assert(kProducts == kBatches * kBatch, "a batch per tile");
   }
 
   // ---- results ---------------------------------------------------------------------------------------------------
@@ -590,34 +656,58 @@ struct PagedAttention {
   static __device__ __forceinline__ float inverse(float l) { return l > 0.0f || l != l ? 1.0f / l : 0.0f; }   // a row without keys: zeros
 
   // ---- wide items ------------------------------------------------------------------------------------------------
+  // Bound by how well two waves per SIMD overlap: of the 5000 clocks of a step the matrix units are busy for 2050 (two
+  // waves), the vector units for 2000 (an exponential per score takes a quarter of that), the LDS reads of K and V for
+  // about as long; leaving out any one of them saves no more than 8 %.  One barrier per step: it ends the stores of the
+  // step's tile, while the next one is on its way in registers.  So that a SIMD's two waves are not at the same part at
+  // the same time, the later one runs half a step behind: it begins with the products of the last step's values, which
+  // therefore stay a step longer (three buffers).  Waves at their products go first where both could issue.
+  // At 5 prompts of 6405 tokens in all on 32 / 8 heads of 128 elements in bf16: 500 us, 880 TFLOP/s; 515 without the
+  // shift, 510 without the priority, 530 with a workgroup barrier per half step that forces the waves to take turns.
   static constexpr int kRuns = (kWideKeys * CPR + MONONN_BLOCK_SIZE - 1) / MONONN_BLOCK_SIZE;   // pieces of K (and of V) a thread moves per step
-  static __device__ __forceinline__ int wide_piece(int run) { return (run * NW + __builtin_amdgcn_readfirstlane(wave_id())) * kWaveSize; }
-  static __device__ __forceinline__ void wide_load(const T* kc, const T* vc, int pages, int key0, int h, half8_t (&k)[kRuns], half8_t (&v)[kRuns]) {
-#pragma unroll
-    for (int i = 0; i < kRuns; ++i) load_run_of_rows(kc, vc, pages, key0, wide_piece(i), h, k[i], v[i]);
-  }
+  static __device__ __forceinline__ int wide_piece(const Lane& l, int run) { return (run * NW + l.wave) * kWaveSize; }
   // Rows behind the sequence's last key become zeros: whatever those cells hold, NaN included, must not reach 0 * v.
-  static __device__ __forceinline__ void wide_store(char* buf, int key0, int ctx, half8_t (&k)[kRuns], half8_t (&v)[kRuns]) {
+  static __device__ __forceinline__ void wide_store(const Lane& l, char* buf, int pitch, int mine, int key0, int ctx, half8_t (&x)[kRuns]) {
     if (key0 + kWideKeys > ctx) {
 #pragma unroll
-      for (int i = 0; i < kRuns; ++i) {
-        const half8_t zero = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (key0 + (wide_piece(i) + lane_id()) / CPR >= ctx) k[i] = zero, v[i] = zero;
-      }
+      for (int i = 0; i < kRuns; ++i)
+        if (key0 + l.row_of(wide_piece(l, i)) >= ctx) x[i] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
     }
 #pragma unroll
     for (int i = 0; i < kRuns; ++i) {
-      const int at = wide_piece(i) + lane_id(), row = at / CPR, c = at % CPR;
-      if (kWideKeys * CPR % MONONN_BLOCK_SIZE != 0 && row >= kWideKeys) break;
-      *reinterpret_cast<half8_t*>(buf + row * KP + c * 16) = k[i];
-      *reinterpret_cast<half8_t*>(buf + kWideKeys * KP + row * VP + c * 16) = v[i];
+      if (kWideKeys * CPR % MONONN_BLOCK_SIZE != 0 && l.row_of(wide_piece(l, i)) >= kWideKeys) break;
+      *reinterpret_cast<half8_t*>(buf + l.lds(wide_piece(l, i), pitch, mine)) = x[i];
     }
   }
   static __device__ __forceinline__ void wide(const T* q, const T* kc, const T* vc, const int* table, T* out, float* part, const Item& it, int from, int count, bool whole,
-                                              float scale_log2, char* smem, int& turn) {
-    const int wave = __builtin_amdgcn_readfirstlane(wave_id());
+                                              float scale_log2, char* smem) {
+    const Lane l;
+    const int k_mine = l.row * KP + l.piece * 16, v_mine = l.row * VP + l.piece * 16;
+    const int k_read = (l.lane & 31) * KP + (l.lane >> 5) * 16, v_read = (4 * (l.lane >> 5) + (l.lane & 15) / 4) * VP + ((l.lane >> 4) & 1) * 32 + (l.lane & 3) * 8;
+    const int wave = l.wave;
     const int rows = it.s.len * G, row0 = it.tile * 32 * NW + wave * 32;
-    const bool live = row0 < rows;
+    const bool live = row0 < rows, later = kSkew && (wave / 4) % 2 == 1;   // wave w runs on SIMD w % 4
+    char* const kbuf = smem;                                   // [2][64][KP]
+    char* const vbuf = smem + 2 * kWideKeys * KP;              // [kValueBuffers][64][VP]
+    const int begin = (it.first + from) * kWideKeys;
+    half8_t k[kRuns], v[kRuns];   // the next tile, on its way
+    int pages_next = lane_page(l, table, it.b, begin);
+    // Behind the last step the same again, stored where nothing reads it any more: without branches around them the
+    // compiler knows how many loads are on their way, and waits for no more than it needs.  The pages of the next tile
+    // are asked for before this one's rows: loads return in order.
+    auto load_tile = [&](int j) {
+      const int pages = in_pool(pages_next);
+      pages_next = lane_page(l, table, it.b, begin + (j + 1) * kWideKeys);
+#pragma unroll
+      for (int i = 0; i < kRuns; ++i) {
+        const Cell cell = cell_of(l, pages, begin + j * kWideKeys, wide_piece(l, i), it.h);
+        k[i] = load_cell(kc, cell);
+        v[i] = load_cell(vc, cell);
+      }
+    };
+    int v_at = 0;   // the buffer of this step's values, in bytes
+    auto next_buffer = [](int at) { return at == (kValueBuffers - 1) * kWideKeys * VP ? 0 : at + kWideKeys * VP; };
+    load_tile(0);
     Rows r;
     load_rows(q, it, row0, r);
     // keys that the wave's first and last row see
@@ -625,26 +715,34 @@ struct PagedAttention {
     const int p_first = it.s.ctx - it.s.len + t_first, p_last = it.s.ctx - it.s.len + t_last;
     State st;
     st.clear();
-    half8_t k[kRuns], v[kRuns];
-    const int begin = (it.first + from) * kWideKeys;
-    wide_load(kc, vc, lane_page(table, it.b, begin), begin, it.h, k, v);
-    int pages = lane_page(table, it.b, begin + kWideKeys);
+    wide_store(l, kbuf, KP, k_mine, begin, it.s.ctx, k);
+    wide_store(l, vbuf, VP, v_mine, begin, it.s.ctx, v);
+    load_tile(1);
+    Scores s;
+    Probabilities p;
+    bool weighing = false;   // the last step left probabilities to a later wave
+    int v_last = 0;
     for (int i = 0; i < count; ++i) {
       const int key0 = begin + i * kWideKeys;
-      char* buf = smem + turn * kWideBuffer;
-      turn ^= 1;
-      wide_store(buf, key0, it.s.ctx, k, v);
+      const bool some = live && key0 <= p_last && !(WINDOW > 0 && key0 + kWideKeys - 1 < p_first - WINDOW + 1);
+      const int v_next = next_buffer(v_at);
+      auto move = [&] {
+        wide_store(l, kbuf + ((i + 1) & 1) * kWideKeys * KP, KP, k_mine, key0 + kWideKeys, it.s.ctx, k);
+        wide_store(l, vbuf + v_next, VP, v_mine, key0 + kWideKeys, it.s.ctx, v);
+        load_tile(i + 2);
+      };
       __syncthreads();
-      if (i + 1 < count) {
-        wide_load(kc, vc, pages, key0 + kWideKeys, it.h, k, v);
-        pages = lane_page(table, it.b, key0 + 2 * kWideKeys);
-      }
-      const bool none = !live || key0 > p_last || (WINDOW > 0 && key0 + kWideKeys - 1 < p_first - WINDOW + 1);
-      if (!none) {
-        const bool check = key0 + kWideKeys - 1 > p_first || (WINDOW > 0 && key0 < p_last - WINDOW + 1);
-        step<2>(buf, buf + kWideKeys * KP, key0, r, st, scale_log2, check);
-      }
+      if (later && weighing) weigh(vbuf + v_last + v_read, p, st);
+      if (some) score(kbuf + (i & 1) * kWideKeys * KP + k_read, r, s, move);
+      else move();
+      if (some) soft_max(key0, r, st, scale_log2, key0 + kWideKeys - 1 > p_first || (WINDOW > 0 && key0 < p_last - WINDOW + 1), s, p);
+      if (!later && some) weigh(vbuf + v_at + v_read, p, st);
+      weighing = some;
+      v_last = v_at;
+      v_at = v_next;
     }
+    if (later && weighing) weigh(vbuf + v_last + v_read, p, st);   // stored behind it: the next buffer
+    __syncthreads();
     st.finish();
     if (!live) return;
     if (whole) {
@@ -667,7 +765,7 @@ struct PagedAttention {
   struct Cursor {
     Item it;
     int step;   // inside the item
-    __device__ __forceinline__ int key0() const { return (it.first + step) * kNarrowKeys + __builtin_amdgcn_readfirstlane(wave_id()) * 32; }
+    __device__ __forceinline__ int key0(const Lane& l) const { return (it.first + step) * kNarrowKeys + l.wave * 32; }
   };
   struct NarrowRows {
     half8_t q[QN];
@@ -689,10 +787,18 @@ struct PagedAttention {
     r.hi = it.s.ctx - it.s.len + row / G;
     r.lo = WINDOW > 0 ? r.hi - WINDOW + 1 : 0;
   }
-  static __device__ __forceinline__ void narrow_load(const T* kc, const T* vc, int pages, const Cursor& c, half8_t (&k)[kMine], half8_t (&v)[kMine]) {
-    if (c.key0() >= c.it.s.ctx) return;   // the wave has no key in this step
+  static __device__ __forceinline__ void narrow_load(const Lane& l, const T* kc, const T* vc, int pages, const Cursor& c, half8_t (&k)[kMine], half8_t (&v)[kMine]) {
+    const int key0 = c.key0(l);
+    if (key0 >= c.it.s.ctx) return;   // the wave has no key in this step
+    pages = in_pool(pages);
+    Cell cell[kMine];
 #pragma unroll
-    for (int i = 0; i < kMine; ++i) load_run_of_rows(kc, vc, pages, c.key0(), i * kWaveSize, c.it.h, k[i], v[i]);
+    for (int i = 0; i < kMine; ++i) {
+      cell[i] = cell_of(l, pages, key0, i * kWaveSize, c.it.h);
+      k[i] = load_cell(kc, cell[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) v[i] = load_cell(vc, cell[i]);
   }
   struct NarrowState {
     float4_t o[kTiles];
@@ -706,13 +812,13 @@ struct PagedAttention {
     __device__ __forceinline__ void finish() { l = quarter_waves_sum(half_waves_sum(l)); }
   };
   // 32 keys on 16 query rows
-  static __device__ __forceinline__ void narrow_step(const char* kbuf, const char* vbuf, int key0, const NarrowRows& r, NarrowState& st, float scale_log2, bool check) {
-    const int lane = lane_id(), g = lane >> 4, i16 = lane & 15;
+  static __device__ __forceinline__ void narrow_step(const Lane& l, const char* krow, const char* vrow, int key0, const NarrowRows& r, NarrowState& st, float scale_log2, bool check) {
+    const int g = l.lane >> 4;
     float4_t s[2];
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       s[b] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-      const char* row = kbuf + (b * 16 + i16) * KP + g * 16;
+      const char* row = krow + b * 16 * KP;
 #pragma unroll
       for (int i = 0; i < QN; ++i) {
         // half a step at the end of the head: the queries are zero there, any elements of the row will do
@@ -731,7 +837,7 @@ struct PagedAttention {
     }
     float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
     top = quarter_waves_max(half_waves_max(top)) * scale_log2;
-    if (__any(top > st.m + 6.0f)) {   // as in step()
+    if (__any(top > st.m + 6.0f)) {   // as in soft_max()
       const float m = fmaxf(st.m, top);
       const float a = __builtin_amdgcn_exp2f(st.m - m);
       st.l *= a;
@@ -748,7 +854,6 @@ struct PagedAttention {
         st.l += e;
         p[b * 4 + i] = __builtin_bit_cast(half_t, (T)e);
       }
-    const char* vrow = vbuf + (4 * g + i16 / 4) * VPN + (i16 & 3) * 8;
 #pragma unroll
     for (int t = 0; t < kTiles; ++t) {
       struct { mononn_short4 lo, hi; } v;
@@ -766,10 +871,13 @@ struct PagedAttention {
   // where it stopped.  Returns the steps done.
   static __device__ __forceinline__ int narrow(const T* q, const T* kc, const T* vc, const int* table, const int* qs, const int* cl, T* out, float* part, int range, Item& it, int& inside,
                                                int left, float scale_log2, char* smem) {
-    const int wave = __builtin_amdgcn_readfirstlane(wave_id()), lane = lane_id(), query = lane & 15;
+    const Lane l;
+    const int wave = l.wave, lane = l.lane, query = lane & 15;
     const bool live = wave < NN;
-    char* kbuf = smem + (live ? wave : 0) * kWaveBuffer;
-    char* vbuf = kbuf + 32 * KP;
+    char* const kbuf = smem + (live ? wave : 0) * kWaveBuffer;
+    char* const vbuf = kbuf + 32 * KP;
+    const int k_mine = l.row * KP + l.piece * 16, v_mine = l.row * VPN + l.piece * 16;
+    const int k_read = (lane & 15) * KP + (lane >> 4) * 16, v_read = (4 * (lane >> 4) + (lane & 15) / 4) * VPN + (lane & 3) * 8;
     Cursor cur = {it, inside};
     // the step behind `c`; false when the range ends before it or it is a wide item's (`c` is that item then)
     auto advance = [&](Cursor& c, int remaining) {
@@ -783,37 +891,36 @@ struct PagedAttention {
     int done = 0, begun = inside;   // step of the item at which this part begins
     NarrowRows r, rn;
     narrow_rows(q, cur.it, r);
-    if (live) narrow_load(kc, vc, lane_page(table, cur.it.b, cur.key0()), cur, k, v);
+    if (live) narrow_load(l, kc, vc, lane_page(l, table, cur.it.b, cur.key0(l)), cur, k, v);
     Cursor nxt = cur;
     bool more = advance(nxt, left - 1);
-    int pages = more ? lane_page(table, nxt.it.b, nxt.key0()) : 0;
+    int pages = more ? lane_page(l, table, nxt.it.b, nxt.key0(l)) : 0;
     NarrowState st;
     st.clear();
     __syncthreads();   // the buffers may still be read by a wide item's last step
     for (;;) {
-      const int key0 = cur.key0();
+      const int key0 = cur.key0(l);
       const bool some = live && key0 < cur.it.s.ctx;
       if (some) {
         if (key0 + 32 > cur.it.s.ctx) {   // rows behind the last key: zeros, as in wide_store()
 #pragma unroll
           for (int j = 0; j < kMine; ++j) {
             const half8_t zero = {0, 0, 0, 0, 0, 0, 0, 0};
-            if (key0 + (lane + j * kWaveSize) / CPR >= cur.it.s.ctx) k[j] = zero, v[j] = zero;
+            if (key0 + l.row_of(j * kWaveSize) >= cur.it.s.ctx) k[j] = zero, v[j] = zero;
           }
         }
 #pragma unroll
         for (int j = 0; j < kMine; ++j) {
-          const int at = lane + j * kWaveSize, row = at / CPR, c = at % CPR;
-          *reinterpret_cast<half8_t*>(kbuf + row * KP + c * 16) = k[j];
-          *reinterpret_cast<half8_t*>(vbuf + row * VPN + c * 16) = v[j];
+          *reinterpret_cast<half8_t*>(kbuf + l.lds(j * kWaveSize, KP, k_mine)) = k[j];
+          *reinterpret_cast<half8_t*>(vbuf + l.lds(j * kWaveSize, VPN, v_mine)) = v[j];
         }
       }
       Cursor behind = nxt;
       bool more_behind = false;
       if (more) {
-        if (live) narrow_load(kc, vc, pages, nxt, k, v);
+        if (live) narrow_load(l, kc, vc, pages, nxt, k, v);
         more_behind = advance(behind, left - done - 2);
-        if (more_behind) pages = lane_page(table, behind.it.b, behind.key0());
+        if (more_behind) pages = lane_page(l, table, behind.it.b, behind.key0(l));
       }
       if (some) {
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -821,7 +928,7 @@ struct PagedAttention {
         const int p_first = cur.it.s.ctx - cur.it.s.len, p_last = cur.it.s.ctx - 1;
         if (!(WINDOW > 0 && key0 + 31 < p_first - WINDOW + 1)) {
           const bool check = key0 + 31 > p_first || (WINDOW > 0 && key0 < p_last - WINDOW + 1);
-          narrow_step(kbuf, vbuf, key0, r, st, scale_log2, check);
+          narrow_step(l, kbuf + k_read, vbuf + v_read, key0, r, st, scale_log2, check);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -885,7 +992,7 @@ struct PagedAttention {
     }
     const Plan p = plan(qs, cl);
     const int range = range_of(unit), end = range_begin(p.total, range + 1);
-    int at = range_begin(p.total, range), turn = 0;
+    int at = range_begin(p.total, range);
     const float scale_log2 = scale * 1.44269504088896f;
     if (at >= end) return;
     int inside;
@@ -899,7 +1006,7 @@ struct PagedAttention {
       if constexpr (!kAllNarrow) {
         const int count = it.steps - inside < end - at ? it.steps - inside : end - at;
         const bool whole = inside == 0 && count == it.steps;
-        wide(q, kc, vc, table, out, part + (long)(2 * range + (inside == 0 ? 1 : 0)) * kPart, it, inside, count, whole, scale_log2, smem, turn);
+        wide(q, kc, vc, table, out, part + (long)(2 * range + (inside == 0 ? 1 : 0)) * kPart, it, inside, count, whole, scale_log2, smem);
         at += count;
         inside = 0;
         next_item(qs, cl, it);

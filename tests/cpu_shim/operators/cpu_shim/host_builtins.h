@@ -13,6 +13,7 @@ inline mononn_short4 host_lds_read8(const char* p) {
 #define MONONN_LDS_READ_TR16(p) host_lds_read8(p)
 inline void sincospif(float x, float* s, float* c) { *s = sinf(3.14159265f * x), *c = cosf(3.14159265f * x); }
 #define __builtin_amdgcn_exp2f(x) exp2f(x)
+#define __builtin_amdgcn_s_setprio(p) ((void)0)
 #define __any(x) (x)
 #define __ballot(x) ((x) ? 1ull : 0ull)
 #define __shfl(v, ...) (v)
