@@ -1223,12 +1223,23 @@ struct MatvecW4 {
     c.scale = load_groups<Scales>(scale, row, block);
     if constexpr (ZEROS) c.zero = load_groups<Zeros>(zero, row, block);
   }
-  static __device__ __forceinline__ void stage_x(const T* x, int m0, int piece0, half8_t* xs) {
-    for (int i = thread_id(); i < kPieces * XROWS; i += MONONN_BLOCK_SIZE) {
+  // x goes to the LDS through registers, kRun pieces of a thread at a time.  The last of these rounds is split in two, so
+  // that the first weights can be asked for between its loads and its stores: loads return in order.
+  static constexpr int kCells = kPieces * XROWS, kRounds = (kCells + MONONN_BLOCK_SIZE - 1) / MONONN_BLOCK_SIZE, kRun = kRounds < 8 ? kRounds : 8;
+  static __device__ __forceinline__ void request_x(const T* x, int m0, int piece0, int round, half8_t (&v)[kRun]) {
+#pragma unroll
+    for (int j = 0; j < kRun; ++j) {
+      const int i = (round + j) * MONONN_BLOCK_SIZE + thread_id();
       const int piece = i % kPieces, m = i / kPieces;   // neighbouring threads read along a row
-      half8_t v = {0, 0, 0, 0, 0, 0, 0, 0};
-      if (m0 + m < M && (piece0 + piece) * 8 < K) v = nibble_order(*reinterpret_cast<const half8_t*>(x + (long)(m0 + m) * K + (piece0 + piece) * 8));
-      xs[piece * XPITCH + m] = v;
+      v[j] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
+      if (m < XROWS && m0 + m < M && (piece0 + piece) * 8 < K) v[j] = *reinterpret_cast<const half8_t*>(x + (long)(m0 + m) * K + (piece0 + piece) * 8);
+    }
+  }
+  static __device__ __forceinline__ void keep_x(int round, const half8_t (&v)[kRun], half8_t* xs) {
+#pragma unroll
+    for (int j = 0; j < kRun; ++j) {
+      const int i = (round + j) * MONONN_BLOCK_SIZE + thread_id();
+      if (i < kCells) xs[i % kPieces * XPITCH + i / kPieces] = nibble_order(v[j]);
     }
   }
   // left operands of piece i of a block, for its four steps; `a` keeps its zeros in the lanes that hold no x
@@ -1261,9 +1272,16 @@ struct MatvecW4 {
     __syncthreads();   // the rows of the unit before
     Weights ring[DEPTH];
     auto block_at = [&](int i) { return clamp_int(b0 + (i < count ? i : count - 1), 0, BLOCKS - 1); };   // the last one again behind the end
-    stage_x(x, m0, first * (BLOCK / 8), xs);
+    half8_t staged[kRun];
+    int round = 0;
+    for (; round + kRun < kRounds; round += kRun) {
+      request_x(x, m0, first * (BLOCK / 8), round, staged);
+      keep_x(round, staged, xs);
+    }
+    request_x(x, m0, first * (BLOCK / 8), round, staged);
 #pragma unroll
     for (int i = 0; i < DEPTH; ++i) load(weight, scale, zero, row, block_at(i), ring[i]);
+    keep_x(round, staged, xs);
     float4_t acc[MT];
     half8_t a[2][MT][4];
 #pragma unroll
