@@ -159,7 +159,7 @@ NodeFunction generate_operator(const graph::Program& prog, const graph::Node& no
       MONONN_CHECK(result != nullptr && parts->oper.kind == OperatorConfig::kPagedAttentionParts, kInternal) << node.name << ": a paged attention without its other stage";
       const auto &q = parts->operands[0]->shape.dims, &kc = parts->operands[1]->shape.dims, &table = parts->operands[3]->shape.dims;
       body << "typedef mononn_dev::PagedAttention<" << hlo::dtype_ctype(result->shape.dtype) << ", " << q[0] << ", " << table[0] << ", " << q[1] << ", " << kc[2] << ", " << q[2] << ", " << kc[1]
-           << ", " << kc[0] << ", " << table[1] << ", " << c.window << ", " << grid << ", " << flag(read_in_kernel(prog, result)) << "> Attention; ";
+           << ", " << kc[0] << ", " << table[1] << ", " << (c.window < table[1] * kc[1] ? c.window : 0) << ", " << grid << ", " << flag(read_in_kernel(prog, result)) << "> Attention; ";
       if (parts_stage) {
         const std::string qp = input(0), kp = input(1), vp = input(2), tp = input(3), sp = input(4), lp = input(5);
         const std::string out = ptrs.output(result), pp = ptrs.output(ins);

@@ -295,6 +295,8 @@ struct PagedAttention {
     return kMergeBytes > n ? kMergeBytes : n;
   }
 
+  static constexpr float kNothing = -3e38f;   // running maximum before the first key: below any finite score
+
   struct Item {
     int b, h, tile;
     Sequence s;
@@ -304,16 +306,21 @@ struct PagedAttention {
 
   static __device__ __forceinline__ bool is_narrow(int len) { return kAllNarrow || len * G <= 16; }
   static __device__ __forceinline__ int tiles_of(int len) { return is_narrow(len) ? (len > 0 ? 1 : 0) : (len * G + 32 * NW - 1) / (32 * NW); }
-  // keys [lo, hi) that some row of the tile sees, as steps; at least one step, so that empty rows are written too
-  static __device__ __forceinline__ void tile_steps(const Sequence& s, int tile, int& first, int& steps) {
-    const bool narrow = is_narrow(s.len);
-    const int rows = narrow ? 16 : 32 * NW, keys = narrow ? kNarrowKeys : kWideKeys;
+  // keys [lo, hi) that some row of the tile sees
+  static __device__ __forceinline__ void tile_keys(const Sequence& s, int tile, int& lo, int& hi) {
+    const int rows = is_narrow(s.len) ? 16 : 32 * NW;
     const int t0 = tile * rows / G;
     int t1 = ((tile + 1) * rows - 1) / G;
     if (t1 > s.len - 1) t1 = s.len - 1;
     const int p0 = s.ctx - s.len + t0, p1 = s.ctx - s.len + t1;
-    const int lo = WINDOW > 0 && p0 - WINDOW + 1 > 0 ? p0 - WINDOW + 1 : 0;
-    const int hi = p1 + 1;   // <= ctx
+    lo = WINDOW > 0 && p0 - WINDOW + 1 > 0 ? p0 - WINDOW + 1 : 0;
+    hi = p1 + 1;   // <= ctx
+  }
+  // ... as steps; at least one step, so that empty rows are written too
+  static __device__ __forceinline__ void tile_steps(const Sequence& s, int tile, int& first, int& steps) {
+    const int keys = is_narrow(s.len) ? kNarrowKeys : kWideKeys;
+    int lo, hi;
+    tile_keys(s, tile, lo, hi);
     first = lo / keys;
     steps = hi > lo ? (hi + keys - 1) / keys - first : 0;
     if (steps < 1) steps = 1;
@@ -520,7 +527,7 @@ struct PagedAttention {
     float16_t o[DT];
     float m, l;   // of the lane's query; l of the lane's half of the keys until finish()
     __device__ __forceinline__ void clear() {
-      m = -1e30f;
+      m = kNothing;
       l = 0.0f;
 #pragma unroll
       for (int t = 0; t < DT; ++t)
@@ -666,17 +673,22 @@ struct PagedAttention {
   // shift, 510 without the priority, 530 with a workgroup barrier per half step that forces the waves to take turns.
   static constexpr int kRuns = (kWideKeys * CPR + MONONN_BLOCK_SIZE - 1) / MONONN_BLOCK_SIZE;   // pieces of K (and of V) a thread moves per step
   static __device__ __forceinline__ int wide_piece(const Lane& l, int run) { return (run * NW + l.wave) * kWaveSize; }
-  // Rows behind the sequence's last key become zeros: whatever those cells hold, NaN included, must not reach 0 * v.
-  static __device__ __forceinline__ void wide_store(const Lane& l, char* buf, int pitch, int mine, int key0, int ctx, half8_t (&x)[kRuns]) {
-    if (key0 + kWideKeys > ctx) {
-#pragma unroll
-      for (int i = 0; i < kRuns; ++i)
-        if (key0 + l.row_of(wide_piece(l, i)) >= ctx) x[i] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
-    }
+  static __device__ __forceinline__ void wide_store(const Lane& l, char* buf, int pitch, int mine, const half8_t (&x)[kRuns]) {
 #pragma unroll
     for (int i = 0; i < kRuns; ++i) {
       if (kWideKeys * CPR % MONONN_BLOCK_SIZE != 0 && l.row_of(wide_piece(l, i)) >= kWideKeys) break;
       *reinterpret_cast<half8_t*>(buf + l.lds(wide_piece(l, i), pitch, mine)) = x[i];
+    }
+  }
+  // Values of keys outside [lo, hi), which no row of the tile sees, become zeros: whatever those cells hold, NaN included,
+  // must not reach 0 * v.  (Their scores are replaced, not multiplied: keys may stay as they are.)
+  static __device__ __forceinline__ void clear_unseen(const Lane& l, int key0, int lo, int hi, half8_t (&x)[kRuns]) {
+    if (key0 + kWideKeys > hi || (WINDOW > 0 && key0 < lo)) {
+#pragma unroll
+      for (int i = 0; i < kRuns; ++i) {
+        const int key = key0 + l.row_of(wide_piece(l, i));
+        if (key >= hi || (WINDOW > 0 && key < lo)) x[i] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
+      }
     }
   }
   static __device__ __forceinline__ void wide(const T* q, const T* kc, const T* vc, const int* table, T* out, float* part, const Item& it, int from, int count, bool whole,
@@ -713,10 +725,13 @@ struct PagedAttention {
     // keys that the wave's first and last row see
     const int t_first = row0 / G, t_last = (row0 + 31 < rows ? row0 + 31 : rows - 1) / G;
     const int p_first = it.s.ctx - it.s.len + t_first, p_last = it.s.ctx - it.s.len + t_last;
+    int seen_lo, seen_hi;
+    tile_keys(it.s, it.tile, seen_lo, seen_hi);
     State st;
     st.clear();
-    wide_store(l, kbuf, KP, k_mine, begin, it.s.ctx, k);
-    wide_store(l, vbuf, VP, v_mine, begin, it.s.ctx, v);
+    wide_store(l, kbuf, KP, k_mine, k);
+    clear_unseen(l, begin, seen_lo, seen_hi, v);
+    wide_store(l, vbuf, VP, v_mine, v);
     load_tile(1);
     Scores s;
     Probabilities p;
@@ -727,8 +742,9 @@ struct PagedAttention {
       const bool some = live && key0 <= p_last && !(WINDOW > 0 && key0 + kWideKeys - 1 < p_first - WINDOW + 1);
       const int v_next = next_buffer(v_at);
       auto move = [&] {
-        wide_store(l, kbuf + ((i + 1) & 1) * kWideKeys * KP, KP, k_mine, key0 + kWideKeys, it.s.ctx, k);
-        wide_store(l, vbuf + v_next, VP, v_mine, key0 + kWideKeys, it.s.ctx, v);
+        wide_store(l, kbuf + ((i + 1) & 1) * kWideKeys * KP, KP, k_mine, k);
+        clear_unseen(l, key0 + kWideKeys, seen_lo, seen_hi, v);
+        wide_store(l, vbuf + v_next, VP, v_mine, v);
         load_tile(i + 2);
       };
       __syncthreads();
@@ -804,7 +820,7 @@ struct PagedAttention {
     float4_t o[kTiles];
     float m, l;   // of the lane's query; l of the lane's keys until finish()
     __device__ __forceinline__ void clear() {
-      m = -1e30f;
+      m = kNothing;
       l = 0.0f;
 #pragma unroll
       for (int t = 0; t < kTiles; ++t) o[t] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
@@ -902,11 +918,12 @@ struct PagedAttention {
       const int key0 = cur.key0(l);
       const bool some = live && key0 < cur.it.s.ctx;
       if (some) {
-        if (key0 + 32 > cur.it.s.ctx) {   // rows behind the last key: zeros, as in wide_store()
+        const int lo = WINDOW > 0 ? cur.it.s.ctx - cur.it.s.len - WINDOW + 1 : 0;   // first key that some row sees
+        if (key0 + 32 > cur.it.s.ctx || (WINDOW > 0 && key0 < lo)) {   // values that no row sees: as in clear_unseen()
 #pragma unroll
           for (int j = 0; j < kMine; ++j) {
-            const half8_t zero = {0, 0, 0, 0, 0, 0, 0, 0};
-            if (key0 + l.row_of(j * kWaveSize) >= cur.it.s.ctx) k[j] = zero, v[j] = zero;
+            const int key = key0 + l.row_of(j * kWaveSize);
+            if (key >= cur.it.s.ctx || (WINDOW > 0 && key < lo)) v[j] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
           }
         }
 #pragma unroll
@@ -948,7 +965,7 @@ struct PagedAttention {
           for (int t = 0; t < kTiles; ++t) *reinterpret_cast<float4_t*>(tiles + (wave * kTiles + t) * 256 + lane * 4) = st.o[t];
         }
         __syncthreads();
-        float m = -1e30f, l = 0.0f, w[NN];
+        float m = kNothing, l = 0.0f, w[NN];
 #pragma unroll
         for (int i = 0; i < NN; ++i) m = fmaxf(m, sums[i * 32 + query]);
 #pragma unroll
@@ -1032,7 +1049,7 @@ struct PagedAttention {
       const int block = e / per_block, g = e % per_block;
       const float* tile = part + block * kPartWave;
       float4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
-      float m = -1e30f, l = 0.0f;
+      float m = kNothing, l = 0.0f;
       const int step = shared ? NW : 1;
       int i = shared ? wave : 0;
       auto add = [&](float pm, float pl, float4_t po) {

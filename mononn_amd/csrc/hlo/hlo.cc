@@ -5,6 +5,8 @@
 #include <cmath>
 #include <cstdint>
 #include <cstdlib>
+#include <limits>
+#include <limits>
 #include <set>
 #include <sstream>
 
@@ -375,7 +377,8 @@ void decode_operator_config(Instr* ins) {
     if (j.contains("scale")) c.scale = j.at("scale").as_double();
     if (j.contains("window")) c.window = j.at("window").as_int();
   }
-  refuse_unless(std::isfinite(c.amplitude) && std::isfinite(c.scale), "amplitude and scale must be finite");
+  refuse_unless(std::isfinite(static_cast<float>(c.amplitude)) && std::isfinite(static_cast<float>(2 * c.scale)), "amplitude and scale must be finite f32 numbers");
+  refuse_unless(static_cast<float>(c.scale) >= std::numeric_limits<float>::min(), "scale must be positive");   // a hidden score is -infinity times the scale
   refuse_unless(c.window >= 0 && c.window <= INT32_MAX, "window must be 0 (all keys) or a positive number of keys");
   const size_t n = ins->operands.size();
   for (auto* o : ins->operands) {
@@ -445,7 +448,7 @@ void decode_operator_config(Instr* ins) {
       is(5, DType::kS32, 1, "context_len must be s32[sequences]");
       refuse_unless(dims(4)[0] == dims(3)[0] + 1 && dims(5)[0] == dims(3)[0], "page_table, query_start and context_len disagree about the number of sequences");
       supported(dims(0)[2] % 16 == 0 && dims(0)[2] <= 256, "the head size must be a multiple of 16 up to 256");
-      supported(small(dims(0)[0] * dims(0)[1]) && small(dims(1)[0]) && small(dims(3)[1] * dims(1)[1] + 4096), "too many tokens, pages or keys of a sequence");
+      supported(small(dims(0)[0] * dims(0)[1]) && small(dims(1)[0]) && small(dims(0)[0] + dims(3)[1] * dims(1)[1] + 4096), "too many tokens, pages or keys of a sequence");
       // steps of the whole call are counted in 32 bits: 32 rows and 32 keys at least per step
       supported((dims(0)[0] * dims(0)[1] / 32 + dims(1)[2] * (dims(3)[0] + 1)) * (dims(3)[1] * dims(1)[1] / 32 + 2) <= INT32_MAX, "too many tokens times keys");
       result(ins->shape, type(0), dims(0));

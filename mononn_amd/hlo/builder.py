@@ -410,8 +410,9 @@ class Computation:
         """`mononn$paged_attention`: soft-max attention of new tokens q [tokens, query heads, head size] (f16 or bf16) over
         paged caches laid out as for `kv_append`, which hold the new tokens already: token i of the n new ones of
         sequence b sees keys 0 .. context_len[b] - n + i, with `window` > 0 the last `window` of these.  Query head h
-        reads key head h * key heads // query heads; scores are multiplied by `scale`.  Rows that see no key, and tokens
-        of no sequence, are zero.  Cells behind a sequence's last key may hold anything; the cells of its keys must
+        reads key head h * key heads // query heads; scores are multiplied by `scale` (positive).  Rows that see no key,
+        and tokens of no sequence, are zero.  Cells that no new token of the sequence sees, behind its last key or before
+        the first window, may hold anything, and their pages need not be in the table; the cells of all other keys must
         hold finite numbers."""
         return self._operator("paged_attention", q.dtype, q.dims, [q, k_cache, v_cache, page_table, query_start, context_len], {"scale": float(scale), "window": int(window)})
 

@@ -39,9 +39,9 @@ class MonoNNFunction:
         self._in_place = module.liveout_parameters()   # live-outs that are an input tensor, updated by the call
         assert len(self._out_bytes) == len(self.outputs), "one {dtype, dims} entry per live-out is required"
         self._temp = None if module.owns_temp else torch.zeros(max(info["temp"], 256), dtype=torch.uint8, device=self.device)
-        # what a call fills in: the kernel's arguments, in order (parameters, live-outs, temp)
-        self._args = (ctypes.c_void_p * (len(self._param_bytes) + len(self._out_bytes) + 1))()
-        self._args[len(self._args) - 1] = 0 if self._temp is None else self._temp.data_ptr()
+        self._updates = any(p >= 0 for p in self._in_place)
+        self._args_type = ctypes.c_void_p * (len(self._param_bytes) + len(self._out_bytes) + 1)
+        self._temp_ptr = 0 if self._temp is None else self._temp.data_ptr()
         self._results = [(tuple(o["dims"]), _TORCH_DTYPE[o["dtype"]], p) for o, p in zip(self.outputs, self._in_place)]
         for (dims, dtype, _), nbytes in zip(self._results, self._out_bytes):
             assert torch.empty(dims, dtype=dtype, device="meta").nbytes == nbytes
@@ -65,25 +65,26 @@ class MonoNNFunction:
         # A call is a few microseconds of GPU work for the smallest modules, so the common case (tensors that can be
         # handed over as they are) does nothing twice.
         assert len(inputs) == len(self._param_bytes), f"expected {len(self._param_bytes)} tensors"
-        args, device, held = self._args, self.device, list(inputs)
+        device, held, ptrs = self.device, list(inputs), []
         for i, (t, nbytes) in enumerate(zip(inputs, self._param_bytes)):
             ptr = t.data_ptr()
             if ptr % 16 or t.nbytes != nbytes or t.device != device or not t.is_contiguous():
                 held[i] = t = self._input(i, t)
                 ptr = t.data_ptr()
-            args[i] = ptr
+            ptrs.append(ptr)
         outs = []
-        at = len(inputs)
         for dims, dtype, param in self._results:
             if param >= 0:
                 t = held[param]
                 assert t.dtype == dtype and t.shape == dims, "an input that the call updates in place must have the declared type and shape"
-                args[at] = None
+                assert ptrs.count(ptrs[param]) == 1, "an input that the call updates in place must not be passed twice"
+                ptrs.append(None)
             else:
                 t = torch.empty(dims, dtype=dtype, device=device)
-                args[at] = t.data_ptr()
+                ptrs.append(t.data_ptr())
             outs.append(t)
-            at += 1
+        ptrs.append(self._temp_ptr)
+        args = self._args_type(*ptrs)   # the kernel's arguments, in order: parameters, live-outs, temp
         stream = torch._C._cuda_getCurrentRawStream(device.index)   # what torch.cuda.current_stream(device).cuda_stream says, without the stream object
         self.module.launch_arguments(args, stream)
         if self.checked:
@@ -93,7 +94,10 @@ class MonoNNFunction:
 
 @torch.library.custom_op("mononn::forward", mutates_args=())
 def _forward(handle: int, inputs: Sequence[torch.Tensor]) -> List[torch.Tensor]:
-    return _REGISTRY[handle](*inputs)
+    fn = _REGISTRY[handle]
+    # the operator is declared to change no input and to return new tensors
+    assert not fn._updates, "a module that updates inputs in place is called through MonoNNFunction itself"
+    return fn(*inputs)
 
 
 @_forward.register_fake

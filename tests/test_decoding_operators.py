@@ -1,5 +1,6 @@
 """The decoding operators on the CPU: their oracle against restatements that share nothing with it, what the compiler
 refuses, how their nodes sit in a program, and the addresses their kernels touch."""
+import ctypes
 import json
 import os
 
@@ -8,7 +9,7 @@ import pytest
 
 import cpu_bounds
 import decoding_cases as dc
-from mononn_amd import MonoNNError, MonoNNModule
+from mononn_amd import MonoNNError, MonoNNModule, binding
 from mononn_amd.hlo import models
 from oracle import decoding, hlo_interp
 
@@ -141,6 +142,25 @@ def test_config_refusals():
     refused(params(*ROPE) + call(ROPE[0], "rope", 3, '{\\"amplitude\\":1e999}', "ROOT "), "INVALID_ARGUMENT", "finite")
     att = ["f16[4,8,64]{2,1,0}", "f16[9,16,2,64]{3,2,1,0}", "f16[9,16,2,64]{3,2,1,0}", "s32[3,5]{1,0}", "s32[4]{0}", "s32[3]{0}"]
     refused(params(*att) + call(att[0], "paged_attention", 6, '{\\"scale\\":1,\\"window\\":-1}', "ROOT "), "INVALID_ARGUMENT", "window")
+    refused(params(*ROPE) + call(ROPE[0], "rope", 3, '{\\"amplitude\\":1e300}', "ROOT "), "INVALID_ARGUMENT", "finite")   # not in f32
+    for scale in ("0", "-0.125", "1e-300"):
+        refused(params(*att) + call(att[0], "paged_attention", 6, '{\\"scale\\":' + scale + '}', "ROOT "), "INVALID_ARGUMENT", "scale must be positive")
+
+
+def test_a_window_of_every_key_is_no_window():
+    text = [dc.attention_module(4, 8, 2, 64, 9, 16, 3, 5, "f16", 0.125, w)[0] for w in (0, 80, (1 << 31) - 1, 79)]
+    src = [MonoNNModule.compile(t, build=False).get_source("main.hip") for t in text]
+    assert src[0] == src[1] == src[2] != src[3]
+
+
+def test_liveout_parameter_checks_its_arguments():
+    m = MonoNNModule.compile(dc.append_module(5, 2, 64, 9, 3, 2, 4, "f32")[0], build=False)
+    value = ctypes.c_int(7)
+    ask = binding._lib.mononn_module_liveout_parameter
+    assert ask(m._h, 1, ctypes.byref(value)) == 0 and value.value == 3
+    for handle, index, out in ((m._h, 2, ctypes.byref(value)), (m._h, -1, ctypes.byref(value)), (m._h, 0, None), (None, 0, ctypes.byref(value))):
+        assert ask(handle, index, out) == 1   # invalid argument
+    assert value.value == 3
 
 
 ATT = ["f16[4,8,64]{2,1,0}", "f16[9,16,2,64]{3,2,1,0}", "f16[9,16,2,64]{3,2,1,0}", "s32[3,5]{1,0}", "s32[4]{0}", "s32[3]{0}"]
@@ -319,7 +339,8 @@ def test_bounds_attention(monkeypatch, tmp_path, T, H, HKV, D, B, W, page, windo
     assert check(monkeypatch, tmp_path, text, {3: any_pages(rng, B, W, 30), 4: qs, 5: cl}, grid=8, block=block) == (True, "ok")
 
 
-@pytest.mark.parametrize("M, N, K, group, dtype, zeros", [(1, 100, 96, 32, "f16", False), (19, 33, 640, 32, "bf16", True), (70, 33, 256, 128, "f16", True), (3, 16, 64, 64, "bf16", False), (1, 1, 1280, 256, "f16", True)])
+@pytest.mark.parametrize("M, N, K, group, dtype, zeros", [(1, 100, 96, 32, "f16", False), (19, 33, 640, 32, "bf16", True), (70, 33, 256, 128, "f16", True), (3, 16, 64, 64, "bf16", False), (1, 1, 1280, 256, "f16", True),
+                                                         (16, 40, 4096, 64, "f16", True), (70, 33, 1056, 32, "bf16", False)])   # x in slices
 def test_bounds_w4(monkeypatch, tmp_path, M, N, K, group, dtype, zeros):
     assert check(monkeypatch, tmp_path, dc.w4_module(M, N, K, group, dtype, zeros)[0], grid=8) == (True, "ok")
 

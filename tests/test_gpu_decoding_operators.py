@@ -232,12 +232,43 @@ def test_paged_attention_page_addresses_beyond_32_bits(gpu_device):
     m.close()
 
 
+@pytest.mark.parametrize("block", [256, 512])
+def test_paged_attention_cells_before_the_window_may_hold_anything(gpu_device, block):
+    # pages that a sliding window has left are given back: not in the table any more, or written by others
+    rng = np.random.default_rng(34)
+    new, ctx, page, window, H, HKV, D = [1, 9, 70, 1, 200], [500, 300, 400, 64, 333], 16, 37, 4, 2, 64
+    table, qs, cl, pages = dc.paged_batch(rng, new, ctx, page)
+    text, outs = dc.attention_module(sum(new), H, HKV, D, pages, page, len(new), table.shape[1], "f16", 0.125, window)
+    q, kc, vc = (rng.normal(size=s).astype(np.float16) for s in ((sum(new), H, D), (pages, page, HKV, D), (pages, page, HKV, D)))
+    mags = {}
+    want = decoding.paged_attention(q, kc, vc, table, qs, cl, 0.125, window, mags)
+    seen = np.zeros((pages, page), bool)
+    for b, (n, x) in enumerate(zip(new, ctx)):
+        first = max(0, x - n - window + 1)
+        for p in range(first, x):
+            seen[table[b, p // page], p % page] = True
+        table[b, :first // page] = rng.choice([-1, 0, pages + 5], first // page)
+    kc[~seen], vc[~seen] = np.nan, np.inf
+    (got,) = run(text, outs, [q, kc, vc, table, qs, cl], block)
+    within(got.astype(np.float64), want, dc.attention_bound(want, mags, D, "f16"))
+
+
+def test_paged_attention_without_new_tokens(gpu_device):
+    rng = np.random.default_rng(35)
+    for H in (4, 40):   # at most 16 rows in all, and more
+        text, outs = dc.attention_module(3, H, 2, 64, 9, 16, 2, 4, "f16", 0.125)
+        a = [rng.normal(size=s).astype(np.float16) for s in ((3, H, 64), (9, 16, 2, 64), (9, 16, 2, 64))]
+        (got,) = run(text, outs, a + [np.zeros((2, 4), np.int32), np.zeros(3, np.int32), np.array([50, 3], np.int32)])
+        assert not got.any()
+
+
 # ---- 4-bit products -----------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("block", [256, 512])
 @pytest.mark.parametrize("M, N, K, group, dtype, zeros", [
     (1, 4096, 512, 128, "f16", False), (1, 1, 32, 32, "bf16", True), (2, 100, 96, 32, "f16", True), (3, 1025, 640, 64, "bf16", False), (4, 50, 1280, 256, "f16", True),
     (5, 333, 4096, 32, "bf16", True), (16, 64, 2048, 128, "bf16", False), (17, 40, 384, 64, "f16", False), (70, 33, 256, 128, "f16", True), (130, 20, 1056, 32, "bf16", True),
-    (1, 17, 11008, 64, "f16", True), (33, 5000, 160, 32, "f16", False)])
+    (1, 17, 11008, 64, "f16", True), (33, 5000, 160, 32, "f16", False),
+    (16, 130, 6144, 64, "f16", True), (9, 50, 8192, 128, "bf16", False), (70, 33, 1056, 32, "bf16", True), (40, 300, 2048, 32, "f16", True)])   # x in slices
 def test_matvec_w4(gpu_device, M, N, K, group, dtype, zeros, block):
     rng = np.random.default_rng(19)
     text, outs = dc.w4_module(M, N, K, group, dtype, zeros)
@@ -411,6 +442,94 @@ def test_caches_must_be_contiguous_and_of_the_declared_type(gpu_device):
     with pytest.raises(AssertionError, match="declared type"):
         fn(k, k, cache.clone().view(torch.bfloat16), cache, *meta)
     assert not cache.any()
+
+
+def test_an_updated_input_is_passed_once_and_not_through_the_pure_operator(gpu_device):
+    import torch
+    from mononn_amd.torch_op import forward
+    text, outs = dc.append_module(1, 2, 64, 3, 16, 1, 2, "f16")
+    fn = _function(text, outs, checked=True)
+    k = torch.ones((1, 2, 64), dtype=torch.float16, device="cuda")
+    kc, vc = (torch.zeros((3, 16, 2, 64), dtype=torch.float16, device="cuda") for _ in range(2))
+    meta = [torch.zeros((1, 2), dtype=torch.int32, device="cuda"), torch.tensor([0, 1], dtype=torch.int32, device="cuda"), torch.tensor([1], dtype=torch.int32, device="cuda")]
+    with pytest.raises(AssertionError, match="twice"):
+        fn(k, k, kc, kc, *meta)
+    with pytest.raises(AssertionError, match="in place"):
+        forward(fn, k, k, kc, vc, *meta)
+    assert not kc.any() and not vc.any()
+    fn(k, k, kc, vc, *meta)   # k and v may be one tensor
+    assert kc[0, 0].all() and vc[0, 0].all() and kc.sum() == vc.sum() == 128
+
+
+def test_two_functions_in_two_graphs(gpu_device):
+    """Parts of split sequences lie in each function's own memory: graphs of two, replayed in turn, keep their results."""
+    import torch
+    made = []
+    for seed, ctx in ((41, (3000, 70, 900)), (42, (50, 2000, 400))):
+        text, outs, args = _attention_call(torch, seed, ctx)
+        fn = _function(text, outs)
+        want = fn(*args)[0].clone()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = fn(*args)[0]
+        made.append((fn, args, want, graph, out))
+    for i in range(6):
+        for fn, args, want, graph, out in made:
+            out.zero_()
+            graph.replay()
+            if i % 2:
+                assert torch.equal(fn(*args)[0], want)
+        torch.cuda.synchronize()
+        for *_, want, graph, out in made:
+            assert torch.equal(out, want)
+
+
+def test_inputs_that_are_views(gpu_device):
+    import torch
+    text, outs, args = _attention_call(torch, 43)
+    fn = _function(text, outs, checked=True)
+    want = fn(*args)[0]
+    q = torch.zeros((42, 8, 2, 64), dtype=torch.float16, device="cuda")
+    q[:, :, 1] = args[0]
+    assert torch.equal(fn(q[:, :, 1], *args[1:])[0], want)
+    flat = torch.zeros(args[0].numel() + 8, dtype=torch.float16, device="cuda")
+    flat[8:] = args[0].reshape(-1)
+    assert torch.equal(fn(flat[8:].view(args[0].shape), *args[1:])[0], want)
+    with pytest.raises(AssertionError, match="aligned"):
+        fn(flat[1:-7].view(args[0].shape), *args[1:])
+
+
+def test_launch_with_the_static_arena_and_null_slots(gpu_device):
+    import torch
+    from mononn_amd import MonoNNError
+    text, outs, args = _attention_call(torch, 44)
+    (want,) = _function(text, outs, checked=True)(*args)
+    m = MonoNNModule.compile(text)
+    m.load(0)
+    assert 0 < m.buffer_info()["temp"]
+    out = torch.empty_like(want)
+    stream = torch.cuda.current_stream().cuda_stream
+    from mononn_amd import binding
+    if m.buffer_info()["temp"] <= binding._lib.mononn_static_temp_bytes():
+        m.launch_static_temp([t.data_ptr() for t in args] + [out.data_ptr()], stream)
+        m.synchronize(stream)
+        assert torch.equal(out, want)
+    with pytest.raises(MonoNNError):
+        m.launch_static_temp([t.data_ptr() for t in args] + [0], stream)
+    m.close()
+    text, outs = dc.append_module(1, 2, 64, 3, 16, 1, 2, "f16")
+    a = MonoNNModule.compile(text)
+    a.load(0)
+    k = torch.ones((1, 2, 64), dtype=torch.float16, device="cuda")
+    kc, vc = (torch.zeros((3, 16, 2, 64), dtype=torch.float16, device="cuda") for _ in range(2))
+    meta = [torch.zeros((1, 2), dtype=torch.int32, device="cuda"), torch.tensor([0, 1], dtype=torch.int32, device="cuda"), torch.tensor([1], dtype=torch.int32, device="cuda")]
+    a.launch_static_temp([t.data_ptr() for t in (k, k, kc, vc, *meta)] + [0, 0], stream)   # the live-outs are the caches: no buffers of their own
+    a.synchronize(stream)
+    assert kc.sum() == vc.sum() == 128
+    with pytest.raises(MonoNNError):
+        a.launch_static_temp([k.data_ptr(), k.data_ptr(), 0, vc.data_ptr()] + [t.data_ptr() for t in meta] + [0, 0], stream)
+    a.close()
 
 
 def test_weights_as_constants(gpu_device):
