@@ -320,6 +320,19 @@ def test_decoder_step_matches_the_oracle(gpu_device, kw):
         assert np.abs(g - w).max() <= 2e-2 and (g * w).sum() / np.sqrt((g * g).sum() * (w * w).sum()) >= 0.9999
 
 
+def test_tuned_step_matches_the_oracle(gpu_device, tmp_path):
+    from mononn_amd.binding import MonoNNModuleTuner
+    fx = models.gpt2_step(**{**STEP, "L": 1}, new_tokens=(1, 20), cached=(70, 9), NKV=2, rotary=True, weights_4bit=32)
+    consts, inputs = fx.make_constants(23, "random"), fx.make_inputs(23)
+    m = MonoNNModuleTuner.tune(fx.hlo_text, 0, str(tmp_path), budget=2)
+    m.set_constants(consts)
+    m.load(0)
+    got = m.run(inputs, fx.outputs)
+    m.close()
+    for g, w in zip(got, hlo_interp.evaluate(fx.hlo_text, inputs, consts, "fp32")):
+        assert np.abs(g.astype(np.float64) - w.astype(np.float64)).max() <= 2e-2
+
+
 def test_prompt_in_chunks_then_tokens_equals_the_whole_prompt(gpu_device):
     """Two sequences through the cache -- a chunk, a second chunk, then single tokens, each call on the caches the last
     one left -- give the logits of the dense causal decoder on the same tokens and weights."""
