@@ -1040,6 +1040,8 @@ struct PagedAttention {
     __syncthreads();
   }
 
+  template <int N>
+  struct Count { static constexpr int value = N; };
   // Adds up the parts of the items that were split: a few loads behind each other, 3.5 us at most (left to the range in
   // which an item begins, one workgroup for each: 157 us for one sequence of 131071 keys, where this takes 104).  The workgroups whose ranges hold a part of an item share its
   // output groups among them: `rank` of `count` is this workgroup's.  With many parts the waves of a workgroup take the
@@ -1054,52 +1056,73 @@ struct PagedAttention {
     auto slot = [&](int i) { return (long)(i == 0 ? 2 * first + 1 : 2 * (p.total >= GRID ? first + i : range_with_step(p.total, item0 + i))) * kPart; };
     const bool shared = count >= NW;
     float* share = reinterpret_cast<float*>(smem);   // [NW][64][4] outputs, [NW][64] maxima, [NW][64] sums
-    for (int e = shared ? rank : rank * NW + wave; e < groups; e += shared ? count : count * NW) {
-      const int block = e / per_block, g = e % per_block;
-      const float* tile = part + block * kPartWave;
-      float4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
-      float m = kNothing, l = 0.0f;
-      const int step = shared ? NW : 1;
-      int i = shared ? wave : 0;
-      auto add = [&](float pm, float pl, float4_t po) {
+    const int e0 = shared ? rank : rank * NW + wave, stride = shared ? count : count * NW;
+    const int i0 = shared ? wave : 0, step = shared ? NW : 1;
+    struct Sum {
+      float4_t o;
+      float m, l;
+      __device__ __forceinline__ void add(float pm, float pl, float4_t po) {
         const float top = fmaxf(m, pm), a = __builtin_amdgcn_exp2f(m - top), b = __builtin_amdgcn_exp2f(pm - top);
         m = top;
         l = l * a + pl * b;
         o = o * a + po * b;
-      };
-      for (; i + 3 * step < count; i += 4 * step) {   // four parts in flight
-        float pm[4], pl[4];
-        float4_t po[4];
+      }
+    };
+    // GROUPS output groups from e on, PARTS parts of each from i on: all loads on their way before the first is used
+    auto add_parts = [&](auto groups_at_once, auto parts_at_once, int e, int i, auto& sum) {
+      constexpr int GROUPS = groups_at_once.value, PARTS = parts_at_once.value;
+      float pm[GROUPS][PARTS], pl[GROUPS][PARTS];
+      float4_t po[GROUPS][PARTS];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float* t = tile + slot(i + k * step);
-          pm[k] = t[sums + query], pl[k] = t[sums + queries + query];
-          po[k] = *reinterpret_cast<const float4_t*>(t + g * 256 + lane * 4);
+      for (int j = 0; j < GROUPS; ++j)
+#pragma unroll
+        for (int k = 0; k < PARTS; ++k) {
+          const int at = e + j * stride;
+          const float* t = part + at / per_block * kPartWave + slot(i + k * step);
+          pm[j][k] = t[sums + query], pl[j][k] = t[sums + queries + query];
+          po[j][k] = *reinterpret_cast<const float4_t*>(t + at % per_block * 256 + lane * 4);
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) add(pm[k], pl[k], po[k]);
-      }
-      for (; i < count; i += step) {
-        const float* t = tile + slot(i);
-        add(t[sums + query], t[sums + queries + query], *reinterpret_cast<const float4_t*>(t + g * 256 + lane * 4));
-      }
+      for (int j = 0; j < GROUPS; ++j)
+#pragma unroll
+        for (int k = 0; k < PARTS; ++k) sum[j].add(pm[j][k], pl[j][k], po[j][k]);
+    };
+    auto finish = [&](int e, Sum& sum) {
       if (shared) {
         __syncthreads();
-        *reinterpret_cast<float4_t*>(share + (wave * 64 + lane) * 4) = o;
-        share[NW * 256 + wave * 64 + lane] = m;
-        share[NW * 320 + wave * 64 + lane] = l;
+        *reinterpret_cast<float4_t*>(share + (wave * 64 + lane) * 4) = sum.o;
+        share[NW * 256 + wave * 64 + lane] = sum.m;
+        share[NW * 320 + wave * 64 + lane] = sum.l;
         __syncthreads();
-        if (wave != 0) continue;
-        for (int w = 1; w < NW; ++w) add(share[NW * 256 + w * 64 + lane], share[NW * 320 + w * 64 + lane], *reinterpret_cast<const float4_t*>(share + (w * 64 + lane) * 4));
+        if (wave != 0) return;
+        for (int w = 1; w < NW; ++w) sum.add(share[NW * 256 + w * 64 + lane], share[NW * 320 + w * 64 + lane], *reinterpret_cast<const float4_t*>(share + (w * 64 + lane) * 4));
       }
+      const int block = e / per_block, g = e % per_block;
       Rows r;
       const int row = row0 + block * 32 + query;
       r.valid = row < rows;
       r.out = row_element(it, r.valid ? row : 0);
-      const float inv = inverse(l);
-      if (it.narrow) narrow_out(out, r.out, r.valid, g, o, inv);
-      else store_group(out, r, g, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
-    }
+      const float inv = inverse(sum.l);
+      if (it.narrow) narrow_out(out, r.out, r.valid, g, sum.o, inv);
+      else store_group(out, r, g, sum.o[0] * inv, sum.o[1] * inv, sum.o[2] * inv, sum.o[3] * inv);
+    };
+    auto take = [&](auto groups_at_once, int e) {
+      constexpr int GROUPS = groups_at_once.value;
+      Sum sum[GROUPS];
+#pragma unroll
+      for (int j = 0; j < GROUPS; ++j) sum[j] = {float4_t{0.0f, 0.0f, 0.0f, 0.0f}, kNothing, 0.0f};
+      int i = i0;
+      if constexpr (GROUPS == 1)
+        for (; i + 3 * step < count; i += 4 * step) add_parts(groups_at_once, Count<4>(), e, i, sum);
+      for (; i + step < count; i += 2 * step) add_parts(groups_at_once, Count<2>(), e, i, sum);
+      for (; i < count; i += step) add_parts(groups_at_once, Count<1>(), e, i, sum);
+#pragma unroll
+      for (int j = 0; j < GROUPS; ++j) finish(e + j * stride, sum[j]);
+    };
+    int e = e0;
+    if constexpr (!kAllNarrow)
+      for (; e + 3 * stride < groups; e += 4 * stride) take(Count<4>(), e);
+    for (; e < groups; e += stride) take(Count<1>(), e);
   }
   static constexpr int join_lds_bytes() { return NW * 384 * 4; }
   static __device__ __forceinline__ void join(int unit, const float* part, const int* qs, const int* cl, T* out, char* smem) {
