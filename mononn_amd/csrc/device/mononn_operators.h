@@ -341,6 +341,10 @@ struct PagedAttention {
     return n;
   }
   static __device__ __forceinline__ Sequence sequence(const int* qs, const int* cl, int b) { return sequence_at<TOKENS, MAX_KEYS>(qs, cl, b); }
+  // of the same sequence in all lanes: in scalar registers, and so what is decided by it
+  static __device__ __forceinline__ Sequence uniform(const Sequence& s) {
+    return {__builtin_amdgcn_readfirstlane(s.start), __builtin_amdgcn_readfirstlane(s.len), __builtin_amdgcn_readfirstlane(s.ctx)};
+  }
 
   // Steps up to and with every sequence: lane l of a wave holds those of sequence l; behind the first 64 sequences
   // they are added up again where they are needed.
@@ -403,10 +407,7 @@ struct PagedAttention {
     Item it;
     int rem = at;
     it.b = sequence_with_step(p, qs, cl, rem);
-    it.s = sequence(qs, cl, it.b);
-    it.s.start = __builtin_amdgcn_readfirstlane(it.s.start);
-    it.s.len = __builtin_amdgcn_readfirstlane(it.s.len);
-    it.s.ctx = __builtin_amdgcn_readfirstlane(it.s.ctx);
+    it.s = uniform(sequence(qs, cl, it.b));
     it.narrow = is_narrow(it.s.len);
     int per_head = head_steps(it.s);
     if (per_head < 1) per_head = 1;
@@ -434,11 +435,8 @@ struct PagedAttention {
         do {
           if (it.b + 1 >= SEQS) return;
           ++it.b;
-          it.s = sequence(qs, cl, it.b);
+          it.s = uniform(sequence(qs, cl, it.b));
         } while (it.s.len == 0);
-        it.s.start = __builtin_amdgcn_readfirstlane(it.s.start);
-        it.s.len = __builtin_amdgcn_readfirstlane(it.s.len);
-        it.s.ctx = __builtin_amdgcn_readfirstlane(it.s.ctx);
         it.narrow = is_narrow(it.s.len);
       }
     }
@@ -657,6 +655,24 @@ struct PagedAttention {
     const T v[4] = {(T)a, (T)b, (T)c, (T)d};
     store_run<COHERENT, T, 4>(out + r.out + at, v);
   }
+  // the groups g and g + 1: halves of the wave exchange four elements, so that a lane stores eight, of group g or g + 1
+  static __device__ __forceinline__ void store_groups(T* out, const Rows& r, int g, const float16_t& o, float scale) {
+    T four[2][4];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) four[i / 4][i % 4] = (T)(o[g % 4 * 4 + i] * scale);
+    struct Two { unsigned d[2]; };
+    const Two a = __builtin_bit_cast(Two, four[0]), b = __builtin_bit_cast(Two, four[1]);
+    struct { unsigned d[4]; } eight;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {   // lower lanes: their elements 0 .. 3 and the upper lane's 4 .. 7 of g; upper lanes likewise of g + 1
+      const auto x = __builtin_amdgcn_permlane32_swap(a.d[i], b.d[i], false, false);
+      eight.d[i] = x[0], eight.d[2 + i] = x[1];
+    }
+    const int at = (g / 4) * 32 + (g % 4 + (lane_id() >> 5)) * 8;
+    struct Eight { T v[8]; };
+    if (!r.valid || at >= D) return;
+    store_run<COHERENT, T, 8>(out + r.out + at, __builtin_bit_cast(Eight, eight).v);
+  }
   static __device__ __forceinline__ void store_part(float* to, int g, float a, float b, float c, float d) {
     const float v[4] = {a, b, c, d};
     stN<float, 4>(to + g * 256 + lane_id() * 4, v);
@@ -770,7 +786,7 @@ struct PagedAttention {
     if (whole) {
       const float inv = inverse(st.l);
 #pragma unroll
-      for (int g = 0; g < DT * 4; ++g) store_group(out, r, g, st.o[g / 4][g % 4 * 4] * inv, st.o[g / 4][g % 4 * 4 + 1] * inv, st.o[g / 4][g % 4 * 4 + 2] * inv, st.o[g / 4][g % 4 * 4 + 3] * inv);
+      for (int g = 0; g < DT * 4; g += 2) store_groups(out, r, g, st.o[g / 4], inv);
     } else {
       float* to = part + wave * kPartWave;
 #pragma unroll
