@@ -175,7 +175,8 @@ NodeFunction generate_operator(const graph::Program& prog, const graph::Node& no
       } else {
         const std::string pp = input(0), sp = input(1), lp = input(2);
         body << "Attention::join(unit, " << pp << ", " << sp << ", " << lp << ", " << ptrs.output(ins) << ", smem);";
-        f.smem_bytes = ls.waves() * 384 * 4;
+        const int64_t tile = q[0] * (q[1] / kc[2]) <= 16 ? 1 : 4;
+        f.smem_bytes = static_cast<int>(ls.waves() * (tile * 256 + 128) * 4);
         body << " static_assert(Attention::join_lds_bytes() == " << f.smem_bytes << ", \"LDS\");";
       }
       check_units(grid);

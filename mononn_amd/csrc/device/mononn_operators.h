@@ -648,14 +648,8 @@ struct PagedAttention {
   }
 
   // ---- results ---------------------------------------------------------------------------------------------------
-  // four output elements of the lane's row: d = 32 * (g / 4) + 8 * (g % 4) + 4 * (lane / 32)
-  static __device__ __forceinline__ void store_group(T* out, const Rows& r, int g, float a, float b, float c, float d) {
-    const int at = (g / 4) * 32 + (g % 4) * 8 + (lane_id() >> 5) * 4;
-    if (!r.valid || at >= D) return;
-    const T v[4] = {(T)a, (T)b, (T)c, (T)d};
-    store_run<COHERENT, T, 4>(out + r.out + at, v);
-  }
-  // the groups g and g + 1: halves of the wave exchange four elements, so that a lane stores eight, of group g or g + 1
+  // Group g of four output elements of the lane's row: d = 32 * (g / 4) + 8 * (g % 4) + 4 * (lane / 32).
+  // Groups g and g + 1: halves of the wave exchange four elements, so that a lane stores eight, of group g or g + 1
   static __device__ __forceinline__ void store_groups(T* out, const Rows& r, int g, const float16_t& o, float scale) {
     T four[2][4];
 #pragma unroll
@@ -691,8 +685,9 @@ struct PagedAttention {
   // step's tile, while the next one is on its way in registers.  So that a SIMD's two waves are not at the same part at
   // the same time, the later one runs half a step behind: it begins with the products of the last step's values, which
   // therefore stay a step longer (three buffers).  Waves at their products go first where both could issue.
-  // At 5 prompts of 6830 tokens in all on 32 / 8 heads of 128 elements in bf16: 500 us, 880 TFLOP/s; 515 without the
-  // shift, 510 without the priority, 530 with a workgroup barrier per half step that forces the waves to take turns.
+  // At 5 prompts of 6830 tokens in all on 32 / 8 heads of 128 elements in bf16: 493 us with the join, 893 TFLOP/s.
+  // Without the shift 3 % more, without the priority 2 %, with a barrier per half step that forces the waves to take turns
+  // 6 %, with the next item's first tile and queries requested before the last one's results are stored 5 %.
   static constexpr int kRuns = (kWideKeys * CPR + MONONN_BLOCK_SIZE - 1) / MONONN_BLOCK_SIZE;   // pieces of K (and of V) a thread moves per step
   static __device__ __forceinline__ int wide_piece(const Lane& l, int run) { return (run * NW + l.wave) * kWaveSize; }
   static __device__ __forceinline__ void wide_store(const Lane& l, char* buf, int pitch, int mine, const half8_t (&x)[kRuns]) {
@@ -1058,89 +1053,99 @@ struct PagedAttention {
 
   template <int N>
   struct Count { static constexpr int value = N; };
-  // Adds up the parts of the items that were split: a few loads behind each other, 3.5 us at most (left to the range in
-  // which an item begins, one workgroup for each: 157 us for one sequence of 131071 keys, where this takes 104).  The workgroups whose ranges hold a part of an item share its
+  // Adds up the parts of the items that were split: a few loads behind each other, 3 us for single
+  // tokens; 29 us behind 460 of products for 6830 prompt tokens, whose 512 parts are 68 MB, written and read (left to the
+  // range in which an item begins, one workgroup for each, one sequence of 131071 keys takes 157 us instead of 104).  The workgroups whose ranges hold a part of an item share its
   // output groups among them: `rank` of `count` is this workgroup's.  With many parts the waves of a workgroup take the
   // parts of a group between them, with few every wave its own groups.
   static __device__ __forceinline__ void join_item(const float* part, const Plan& p, const Item& it, int item0, int rank, int count, T* out, char* smem) {
-    const int wave = __builtin_amdgcn_readfirstlane(wave_id()), lane = lane_id(), queries = it.narrow ? 16 : 32, query = lane & (queries - 1);
-    const int rows = it.s.len * G, row0 = it.tile * (it.narrow ? 16 : 32 * NW);
-    const int per_block = it.narrow ? kTiles : DT * 4, sums = per_block * 256;   // groups of four elements per lane; maxima and sums lie behind
-    const int blocks = it.narrow ? 1 : clamp_int((rows - row0 + 31) / 32, 1, NW), groups = blocks * per_block;
+    if (kAllNarrow || it.narrow) join_tiles<true>(part, p, it, item0, rank, count, out, smem);
+    else if constexpr (!kAllNarrow) join_tiles<false>(part, p, it, item0, rank, count, out, smem);
+  }
+  // A unit of work is a tile of a block of queries: 16 output elements of 16 queries in a narrow item, 32 of 32 in a wide one.
+  template <bool NARROW>
+  static __device__ __forceinline__ void join_tiles(const float* part, const Plan& p, const Item& it, int item0, int rank, int count, T* out, char* smem) {
+    constexpr int QUERIES = NARROW ? 16 : 32, GROUPS = NARROW ? 1 : 4, TILES = NARROW ? kTiles : DT;   // groups: four elements per lane
+    constexpr int SUMS = TILES * GROUPS * 256;   // maxima and sums lie behind a block's tiles
+    const int wave = __builtin_amdgcn_readfirstlane(wave_id()), lane = lane_id(), query = lane & (QUERIES - 1);
+    const int rows = it.s.len * G, row0 = NARROW ? 0 : it.tile * 32 * NW;
+    const int blocks = NARROW ? 1 : clamp_int((rows - row0 + 31) / 32, 1, NW);
     const int first = range_with_step(p.total, item0);
     // part i: ranges follow each other, unless there are fewer steps than ranges; then every step is a part
     auto slot = [&](int i) { return (long)(i == 0 ? 2 * first + 1 : 2 * (p.total >= GRID ? first + i : range_with_step(p.total, item0 + i))) * kPart; };
     const bool shared = count >= NW;
-    float* share = reinterpret_cast<float*>(smem);   // [NW][64][4] outputs, [NW][64] maxima, [NW][64] sums
-    const int e0 = shared ? rank : rank * NW + wave, stride = shared ? count : count * NW;
-    const int i0 = shared ? wave : 0, step = shared ? NW : 1;
+    float* share = reinterpret_cast<float*>(smem);   // [NW][GROUPS][64][4] outputs, [NW][64] maxima, [NW][64] sums
+    const int step = shared ? NW : 1;
     struct Sum {
-      float4_t o;
+      float4_t o[GROUPS];
       float m, l;
-      __device__ __forceinline__ void add(float pm, float pl, float4_t po) {
+      __device__ __forceinline__ void add(float pm, float pl, const float4_t (&po)[GROUPS]) {
         const float top = fmaxf(m, pm), a = __builtin_amdgcn_exp2f(m - top), b = __builtin_amdgcn_exp2f(pm - top);
         m = top;
         l = l * a + pl * b;
-        o = o * a + po * b;
+#pragma unroll
+        for (int j = 0; j < GROUPS; ++j) o[j] = o[j] * a + po[j] * b;
       }
     };
-    // GROUPS output groups from e on, PARTS parts of each from i on: all loads on their way before the first is used
-    auto add_parts = [&](auto groups_at_once, auto parts_at_once, int e, int i, auto& sum) {
-      constexpr int GROUPS = groups_at_once.value, PARTS = parts_at_once.value;
-      float pm[GROUPS][PARTS], pl[GROUPS][PARTS];
-      float4_t po[GROUPS][PARTS];
+    for (int unit = shared ? rank : rank * NW + wave; unit < blocks * TILES; unit += shared ? count : count * NW) {
+      const int block = unit / TILES, tile = unit % TILES;
+      const float* from = part + block * kPartWave;
+      Sum sum;
+      sum.m = kNothing, sum.l = 0.0f;
 #pragma unroll
-      for (int j = 0; j < GROUPS; ++j)
+      for (int j = 0; j < GROUPS; ++j) sum.o[j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+      // PARTS parts from i on: all loads on their way before the first is used
+      auto add_parts = [&](auto parts_at_once, int i) {
+        constexpr int PARTS = parts_at_once.value;
+        float pm[PARTS], pl[PARTS];
+        float4_t po[PARTS][GROUPS];
 #pragma unroll
         for (int k = 0; k < PARTS; ++k) {
-          const int at = e + j * stride;
-          const float* t = part + at / per_block * kPartWave + slot(i + k * step);
-          pm[j][k] = t[sums + query], pl[j][k] = t[sums + queries + query];
-          po[j][k] = *reinterpret_cast<const float4_t*>(t + at % per_block * 256 + lane * 4);
+          const float* t = from + slot(i + k * step);
+          pm[k] = t[SUMS + query], pl[k] = t[SUMS + QUERIES + query];
+#pragma unroll
+          for (int j = 0; j < GROUPS; ++j) po[k][j] = *reinterpret_cast<const float4_t*>(t + (tile * GROUPS + j) * 256 + lane * 4);
         }
 #pragma unroll
-      for (int j = 0; j < GROUPS; ++j)
+        for (int k = 0; k < PARTS; ++k) sum.add(pm[k], pl[k], po[k]);
+      };
+      int i = shared ? wave : 0;
+      for (; i + 3 * step < count; i += 4 * step) add_parts(Count<4>(), i);
+      for (; i + step < count; i += 2 * step) add_parts(Count<2>(), i);
+      for (; i < count; i += step) add_parts(Count<1>(), i);
+      if (shared) {   // the waves' sums, one after the other through the first one's hands
+        float4_t* const outputs = reinterpret_cast<float4_t*>(share);
+        float* const maxima = share + NW * GROUPS * 256;
+        __syncthreads();
 #pragma unroll
-        for (int k = 0; k < PARTS; ++k) sum[j].add(pm[j][k], pl[j][k], po[j][k]);
-    };
-    auto finish = [&](int e, Sum& sum) {
-      if (shared) {
+        for (int j = 0; j < GROUPS; ++j) outputs[(wave * GROUPS + j) * 64 + lane] = sum.o[j];
+        maxima[wave * 64 + lane] = sum.m;
+        maxima[(NW + wave) * 64 + lane] = sum.l;
         __syncthreads();
-        *reinterpret_cast<float4_t*>(share + (wave * 64 + lane) * 4) = sum.o;
-        share[NW * 256 + wave * 64 + lane] = sum.m;
-        share[NW * 320 + wave * 64 + lane] = sum.l;
-        __syncthreads();
-        if (wave != 0) return;
-        for (int w = 1; w < NW; ++w) sum.add(share[NW * 256 + w * 64 + lane], share[NW * 320 + w * 64 + lane], *reinterpret_cast<const float4_t*>(share + (w * 64 + lane) * 4));
+        if (wave != 0) continue;
+        for (int w = 1; w < NW; ++w) {
+          float4_t po[GROUPS];
+#pragma unroll
+          for (int j = 0; j < GROUPS; ++j) po[j] = outputs[(w * GROUPS + j) * 64 + lane];
+          sum.add(maxima[w * 64 + lane], maxima[(NW + w) * 64 + lane], po);
+        }
       }
-      const int block = e / per_block, g = e % per_block;
       Rows r;
       const int row = row0 + block * 32 + query;
       r.valid = row < rows;
       r.out = row_element(it, r.valid ? row : 0);
       const float inv = inverse(sum.l);
-      if (it.narrow) narrow_out(out, r.out, r.valid, g, sum.o, inv);
-      else store_group(out, r, g, sum.o[0] * inv, sum.o[1] * inv, sum.o[2] * inv, sum.o[3] * inv);
-    };
-    auto take = [&](auto groups_at_once, int e) {
-      constexpr int GROUPS = groups_at_once.value;
-      Sum sum[GROUPS];
+      if constexpr (NARROW) narrow_out(out, r.out, r.valid, tile, sum.o[0], inv);
+      else {
+        float16_t o;
 #pragma unroll
-      for (int j = 0; j < GROUPS; ++j) sum[j] = {float4_t{0.0f, 0.0f, 0.0f, 0.0f}, kNothing, 0.0f};
-      int i = i0;
-      if constexpr (GROUPS == 1)
-        for (; i + 3 * step < count; i += 4 * step) add_parts(groups_at_once, Count<4>(), e, i, sum);
-      for (; i + step < count; i += 2 * step) add_parts(groups_at_once, Count<2>(), e, i, sum);
-      for (; i < count; i += step) add_parts(groups_at_once, Count<1>(), e, i, sum);
-#pragma unroll
-      for (int j = 0; j < GROUPS; ++j) finish(e + j * stride, sum[j]);
-    };
-    int e = e0;
-    if constexpr (!kAllNarrow)
-      for (; e + 3 * stride < groups; e += 4 * stride) take(Count<4>(), e);
-    for (; e < groups; e += stride) take(Count<1>(), e);
+        for (int e = 0; e < 16; ++e) o[e] = sum.o[e / 4][e % 4];
+        store_groups(out, r, tile * 4, o, inv);
+        store_groups(out, r, tile * 4 + 2, o, inv);
+      }
+    }
   }
-  static constexpr int join_lds_bytes() { return NW * 384 * 4; }
+  static constexpr int join_lds_bytes() { return NW * ((kAllNarrow ? 1 : 4) * 256 + 128) * 4; }
   static __device__ __forceinline__ void join(int unit, const float* part, const int* qs, const int* cl, T* out, char* smem) {
     const Plan p = plan(qs, cl);
     const int range = range_of(unit), begin = range_begin(p.total, range), end = range_begin(p.total, range + 1);
