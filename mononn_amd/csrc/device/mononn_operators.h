@@ -679,9 +679,9 @@ struct PagedAttention {
   static __device__ __forceinline__ float inverse(float l) { return l > 0.0f || l != l ? 1.0f / l : 0.0f; }   // a row without keys: zeros
 
   // ---- wide items ------------------------------------------------------------------------------------------------
-  // Bound by how well two waves per SIMD overlap: of the 5000 clocks of a step the matrix units are busy for 2050 (two
+  // Bound by how well two waves per SIMD overlap: of the 3900 clocks of a step the matrix units are busy for 2050 (two
   // waves), the vector units for 2000 (an exponential per score takes a quarter of that), the LDS reads of K and V for
-  // about as long; leaving out any one of them saves no more than 8 %.  One barrier per step: it ends the stores of the
+  // about as long; leaving out any one of them saves no more than 6 %.  One barrier per step: it ends the stores of the
   // step's tile, while the next one is on its way in registers.  So that a SIMD's two waves are not at the same part at
   // the same time, the later one runs half a step behind: it begins with the products of the last step's values, which
   // therefore stay a step longer (three buffers).  Waves at their products go first where both could issue.

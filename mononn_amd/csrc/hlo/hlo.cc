@@ -5,6 +5,7 @@
 #include <cmath>
 #include <cstdint>
 #include <cstdlib>
+#include <initializer_list>
 #include <limits>
 #include <limits>
 #include <set>
@@ -394,7 +395,13 @@ void decode_operator_config(Instr* ins) {
     is(i, DType::kF32, 1, "inv_freq must be f32[rotated / 2]");
     refuse_unless(2 * dims(i)[0] <= head, "inv_freq has more pairs than a head");
   };
-  auto small = [&](int64_t v) { return v <= INT32_MAX; };
+  // 32-bit offsets of the kernels: the product of the extents, none of which is larger either
+  auto small = [](std::initializer_list<int64_t> extents) {
+    int64_t product = 1;
+    for (int64_t e : extents)
+      if (e > INT32_MAX || (product *= e) > INT32_MAX) return false;
+    return true;
+  };
   switch (c.kind) {
     case OperatorConfig::kRope: {
       refuse_unless(n == 3, "takes (x, positions, inv_freq)");
@@ -404,7 +411,7 @@ void decode_operator_config(Instr* ins) {
       refuse_unless(dims(1)[0] == dims(0)[0], "one position per token");
       rotary(2, dims(0)[2]);
       supported(dims(0)[2] <= 1024, "head size above 1024");
-      supported(small(dims(0)[0]), "too many tokens");
+      supported(small({dims(0)[0]}) && small({dims(0)[1], dims(0)[2]}), "too many tokens or heads");
       result(ins->shape, type(0), dims(0));
       break;
     }
@@ -421,7 +428,8 @@ void decode_operator_config(Instr* ins) {
       refuse_unless(dims(5)[0] == dims(4)[0] + 1 && dims(6)[0] == dims(4)[0], "page_table, query_start and context_len disagree about the number of sequences");
       if (n == 8) rotary(7, dims(0)[2]);
       supported(dims(0)[2] <= 1024, "head size above 1024");
-      supported(small(dims(0)[0]) && small(dims(2)[0]) && small(dims(4)[1] * dims(2)[1]) && small(dims(4)[0]), "too many tokens, pages, sequences or keys of a sequence");
+      supported(small({dims(0)[0]}) && small({dims(0)[1], dims(0)[2]}) && small({dims(2)[0]}) && small({dims(4)[1], dims(2)[1]}) && small({dims(4)[0]}),
+                "too many tokens, heads, pages, sequences or keys of a sequence");
       refuse_unless(ins->shape.is_tuple() && ins->shape.tuple.size() == 2, "yields (k_cache, v_cache)");
       result(ins->shape.tuple[0], type(2), dims(2));
       result(ins->shape.tuple[1], type(3), dims(3));
@@ -448,7 +456,9 @@ void decode_operator_config(Instr* ins) {
       is(5, DType::kS32, 1, "context_len must be s32[sequences]");
       refuse_unless(dims(4)[0] == dims(3)[0] + 1 && dims(5)[0] == dims(3)[0], "page_table, query_start and context_len disagree about the number of sequences");
       supported(dims(0)[2] % 16 == 0 && dims(0)[2] <= 256, "the head size must be a multiple of 16 up to 256");
-      supported(small(dims(0)[0] * dims(0)[1]) && small(dims(1)[0]) && small(dims(0)[0] + dims(3)[1] * dims(1)[1] + 4096), "too many tokens, pages or keys of a sequence");
+      supported(small({dims(0)[0], dims(0)[1]}) && small({dims(1)[0]}) && small({dims(3)[0]}) && small({dims(3)[1], dims(1)[1]}) && small({dims(0)[0] + dims(3)[1] * dims(1)[1] + 4096}),
+                "too many tokens, pages, sequences or keys of a sequence");
+      supported(small({dims(1)[1], dims(1)[2], dims(1)[3]}), "a page has too many elements");
       // steps of the whole call are counted in 32 bits: 32 rows and 32 keys at least per step
       supported((dims(0)[0] * dims(0)[1] / 32 + dims(1)[2] * (dims(3)[0] + 1)) * (dims(3)[1] * dims(1)[1] / 32 + 2) <= INT32_MAX, "too many tokens times keys");
       result(ins->shape, type(0), dims(0));
@@ -464,7 +474,7 @@ void decode_operator_config(Instr* ins) {
       if (n == 4) refuse_unless(type(3) == DType::kU8 && dims(3) == dims(2), "zeros must be u8 of the shape of scales");
       const int64_t group = dims(0)[1] / dims(2)[1];
       supported(group == 32 || group == 64 || group % 128 == 0, "the group size must be 32, 64 or a multiple of 128");
-      supported(small(dims(0)[0]) && small(dims(0)[1]) && small(dims(1)[0]), "too many rows or columns");
+      supported(small({dims(0)[0] + 64, dims(1)[0] + 64}) && small({4 * dims(0)[1]}), "too many rows or columns");
       result(ins->shape, type(0), {dims(0)[0], dims(1)[0]});
     }
   }

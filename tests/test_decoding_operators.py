@@ -177,6 +177,8 @@ ATT = ["f16[4,8,64]{2,1,0}", "f16[9,16,2,64]{3,2,1,0}", "f16[9,16,2,64]{3,2,1,0}
     ({4: "s32[3]{0}"}, "INVALID_ARGUMENT", "number of sequences"),
     ({5: "s32[4]{0}"}, "INVALID_ARGUMENT", "number of sequences"),
     ({3: "s32[3,200000000]{1,0}"}, "UNSUPPORTED", "too many"),
+    ({1: "f16[9,4294967296,2,64]{3,2,1,0}", 2: "f16[9,4294967296,2,64]{3,2,1,0}", 3: "s32[3,4294967296]{1,0}"}, "UNSUPPORTED", "too many"),   # a product of 2^64
+    ({1: "f16[9,33554432,2,64]{3,2,1,0}", 2: "f16[9,33554432,2,64]{3,2,1,0}", 3: "s32[3,1]{1,0}"}, "UNSUPPORTED", "a page has too many"),
 ])
 def test_paged_attention_refusals(change, status, words):
     shapes = [change.get(i, s) for i, s in enumerate(ATT)]
@@ -223,6 +225,16 @@ W4 = ["f16[2,256]{1,0}", "u8[48,128]{1,0}", "f16[48,2]{1,0}", "u8[48,2]{1,0}"]
 def test_matvec_w4_refusals(change, status, words):
     shapes = [change.get(i, s) for i, s in enumerate(W4)]
     refused(params(*shapes) + call("f16[2,48]{1,0}", "matvec_w4", 4, extra="ROOT "), status, words)
+
+
+def test_extents_beyond_32_bits_are_refused():
+    big = ["f16[70000,256]{1,0}", "u8[40000,128]{1,0}", "f16[40000,2]{1,0}"]
+    refused(params(*big) + call("f16[70000,40000]{1,0}", "matvec_w4", 3, extra="ROOT "), "UNSUPPORTED", "too many rows")
+    wide = ["f16[1,4194304,1024]{2,1,0}", "s32[1]{0}", "f32[16]{0}"]
+    refused(params(*wide) + call(wide[0], "rope", 3, extra="ROOT "), "UNSUPPORTED", "too many tokens or heads")
+    c = "f16[9,1,4194304,1024]{3,2,1,0}"
+    shapes = ["f16[1,4194304,1024]{2,1,0}"] * 2 + [c, c] + APP[4:6] + [APP[6]]
+    refused(append_body(shapes, result=f"({c}, {c})"), "UNSUPPORTED", "too many tokens")
 
 
 def test_other_targets_stay_refused():
@@ -332,6 +344,7 @@ def test_bounds_append(monkeypatch, tmp_path, qs, cl, R):
     (9, 4, 2, 256, 2, 20, 8, 7, 512, [0, 8, 9], [170, 30]),
     (5, 3, 1, 16, 2, 9, 1, 0, 64, [0, 5, 3], [-4, 1 << 30]),
     (130, 2, 2, 96, 1, 30, 5, 0, 128, [0, 130], [149]),
+    (600, 8, 2, 64, 3, 90, 8, 33, 1024, [0, 1, 520, 600], [160, 719, 80]),
 ])
 def test_bounds_attention(monkeypatch, tmp_path, T, H, HKV, D, B, W, page, window, block, qs, cl):
     rng = np.random.default_rng(7)

@@ -13,11 +13,12 @@ from oracle import decoding, hlo_interp
 pytestmark = pytest.mark.gpu
 
 
-def run(text, outputs, inputs, block=None):
+def run(text, outputs, inputs, block=None, grid=None):
     spec = None
     if block:
         spec = json.loads(MonoNNModule.compile(text, build=False).get_tuning_spec())
-        spec["cuda_context"]["cuda_runtime_context"]["block_dim"]["x"] = block
+        launch = spec["cuda_context"]["cuda_runtime_context"]
+        launch["block_dim"]["x"], launch["grid_dim"]["x"] = block, grid or launch["grid_dim"]["x"]
         spec = json.dumps(spec)
     m = MonoNNModule.compile(text, spec)
     m.load(0)
@@ -160,6 +161,23 @@ def test_paged_attention(gpu_device, c, block):
     within(dc.values(got, dt), want, dc.attention_bound(want, mags, D, dt))
     empty = ~mags["weighted"].any(-1)
     assert not dc.values(got, dt)[empty].any()
+
+
+@pytest.mark.parametrize("block, grid", [(64, 256), (128, 100), (512, 128), (1024, 256), (256, 1)])
+def test_paged_attention_of_other_launches(gpu_device, block, grid):
+    # few and many ranges, waves and keys per step
+    rng = np.random.default_rng(36)
+    new, ctx, page, H, HKV, D = [65, 1, 0, 300, 17], [65, 900, 12, 1203, 17], 16, 8, 2, 128
+    table, qs, cl, pages = dc.paged_batch(rng, new, ctx, page)
+    for T in (sum(new), 5):
+        starts = qs if T > 5 else np.arange(6, dtype=np.int32)
+        lens = cl if T > 5 else np.minimum(cl, 1000)
+        text, outs = dc.attention_module(T, H if T > 5 else 4, HKV, D, pages, page, 5, table.shape[1], "bf16", 0.09)
+        q, kc, vc = (dc.bits(rng.normal(size=s), "bf16") for s in ((T, H if T > 5 else 4, D), (pages, page, HKV, D), (pages, page, HKV, D)))
+        mags = {}
+        want = decoding.paged_attention(dc.values(q, "bf16"), dc.values(kc, "bf16"), dc.values(vc, "bf16"), table, starts, lens, 0.09, 0, mags)
+        (got,) = run(text, outs, [q, kc, vc, table, starts, lens], block, grid)
+        within(dc.values(got, "bf16"), want, dc.attention_bound(want, mags, D, "bf16"))
 
 
 def test_paged_attention_large_scores_and_one_sided_weights(gpu_device):
