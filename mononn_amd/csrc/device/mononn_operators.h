@@ -351,6 +351,7 @@ struct PagedAttention {
   struct Plan {
     int total;          // steps of the call
     int steps, upto;    // of the lane's sequence; of all sequences up to it
+    Sequence mine;      // the lane's sequence
   };
   static __device__ __forceinline__ int steps_of(const int* qs, const int* cl, int b) { return b < SEQS ? HKV * head_steps(sequence(qs, cl, b)) : 0; }
 #ifndef MONONN_ONE_THREAD
@@ -364,7 +365,8 @@ struct PagedAttention {
   }
   static __device__ __forceinline__ Plan plan(const int* qs, const int* cl) {
     Plan p;
-    p.steps = steps_of(qs, cl, lane_id());
+    p.mine = sequence(qs, cl, lane_id() < SEQS ? lane_id() : SEQS - 1);
+    p.steps = lane_id() < SEQS ? HKV * head_steps(p.mine) : 0;
     p.upto = sum_upto(p.steps);
     p.total = __builtin_amdgcn_readlane(p.upto, kWaveSize - 1);
     for (int base = kWaveSize; base < SEQS; base += kWaveSize)
@@ -388,9 +390,14 @@ struct PagedAttention {
       upto = sum_upto(steps);
     }
   }
+  static __device__ __forceinline__ Sequence planned(const Plan& p, const int* qs, const int* cl, int b) {   // b is the same in all lanes
+    if (b >= kWaveSize) return uniform(sequence(qs, cl, b));
+    return {__builtin_amdgcn_readlane(p.mine.start, b), __builtin_amdgcn_readlane(p.mine.len, b), __builtin_amdgcn_readlane(p.mine.ctx, b)};
+  }
 #else   // for a host build that runs one thread at a time
+  static __device__ __forceinline__ Sequence planned(const Plan&, const int* qs, const int* cl, int b) { return sequence(qs, cl, b); }
   static __device__ __forceinline__ Plan plan(const int* qs, const int* cl) {
-    Plan p = {0, 0, 0};
+    Plan p = {0, 0, 0, {0, 0, 0}};
     for (int b = 0; b < SEQS; ++b) p.total += steps_of(qs, cl, b);
     return p;
   }
@@ -407,7 +414,7 @@ struct PagedAttention {
     Item it;
     int rem = at;
     it.b = sequence_with_step(p, qs, cl, rem);
-    it.s = uniform(sequence(qs, cl, it.b));
+    it.s = planned(p, qs, cl, it.b);
     it.narrow = is_narrow(it.s.len);
     int per_head = head_steps(it.s);
     if (per_head < 1) per_head = 1;
@@ -446,7 +453,10 @@ struct PagedAttention {
   // then read its keys through the same L2.
   static __device__ __forceinline__ int range_of(int unit) { return GRID % kXcds == 0 ? unit % kXcds * (GRID / kXcds) + unit / kXcds : unit; }
   static __device__ __forceinline__ int range_begin(int total, int range) { return (int)((long)total * range / GRID); }
-  static __device__ __forceinline__ int range_with_step(int total, int step) { return (int)((((long)step + 1) * GRID + total - 1) / total) - 1; }
+  static __device__ __forceinline__ int range_with_step(int total, int step) {
+    if (total < 0x7fffffff / GRID) return (int)((((unsigned)step + 1) * GRID + total - 1) / (unsigned)total) - 1;   // a division in 64 bits takes ten times as long
+    return (int)((((long)step + 1) * GRID + total - 1) / total) - 1;
+  }
 
   // ---- loads -----------------------------------------------------------------------------------------------------
   // The pieces of consecutive rows are dealt to the lanes in order.  Lane l fetches the page of row l of a step (one
@@ -1018,15 +1028,16 @@ struct PagedAttention {
   // part: [2 * GRID][kPart]; slot 2 r: a part that an earlier range began, slot 2 r + 1: one that range r begins
   static __device__ __forceinline__ void partial(int unit, const T* q, const T* kc, const T* vc, const int* table, const int* qs, const int* cl, T* out, float* part, float scale,
                                                  char* smem) {
+    const int first_token = qs[0], end_token = qs[SEQS];   // on their way with the lengths
+    const Plan p = plan(qs, cl);
+    const int inside0 = clamp_int(first_token, 0, TOKENS), inside1 = clamp_int(end_token, 0, TOKENS);
     // tokens of no sequence: zeros
-    const int inside0 = clamp_int(qs[0], 0, TOKENS), inside1 = clamp_int(qs[SEQS], 0, TOKENS);
     if (inside0 > 0 || inside1 < TOKENS) {
       const T zero[8] = {(T)0.0f, (T)0.0f, (T)0.0f, (T)0.0f, (T)0.0f, (T)0.0f, (T)0.0f, (T)0.0f};
       for (int t = unit; t < TOKENS; t += GRID)
         if (t < inside0 || t >= inside1)
           for (int c = thread_id(); c < H * CPR; c += MONONN_BLOCK_SIZE) store_run<COHERENT, T, 8>(out + (long)t * H * D + c * 8, zero);
     }
-    const Plan p = plan(qs, cl);
     const int range = range_of(unit), end = range_begin(p.total, range + 1);
     int at = range_begin(p.total, range);
     const float scale_log2 = scale * 1.44269504088896f;
