@@ -352,6 +352,7 @@ struct PagedAttention {
     int total;          // steps of the call
     int steps, upto;    // of the lane's sequence; of all sequences up to it
     Sequence mine;      // the lane's sequence
+    bool whole;         // counted in items instead: every range is an item, or none
   };
   static __device__ __forceinline__ int steps_of(const int* qs, const int* cl, int b) { return b < SEQS ? HKV * head_steps(sequence(qs, cl, b)) : 0; }
 #ifndef MONONN_ONE_THREAD
@@ -366,7 +367,12 @@ struct PagedAttention {
   static __device__ __forceinline__ Plan plan(const int* qs, const int* cl) {
     Plan p;
     p.mine = sequence(qs, cl, lane_id() < SEQS ? lane_id() : SEQS - 1);
-    p.steps = lane_id() < SEQS ? HKV * head_steps(p.mine) : 0;
+    const int per_head = lane_id() < SEQS ? head_steps(p.mine) : 0;
+    p.whole = false;
+    // A handful of short narrow items is not cut, one for a workgroup: a second step costs less than a join (12 heads of
+    // 64 elements, 4 sequences of 210 .. 505 keys: 8.9 us, 9.3 with every step a part).
+    if constexpr (SEQS <= kWaveSize && SEQS * HKV <= GRID) p.whole = __all(per_head == 0 || (per_head <= 2 && is_narrow(p.mine.len)));
+    p.steps = HKV * (p.whole ? (per_head > 0 ? 1 : 0) : per_head);
     p.upto = sum_upto(p.steps);
     p.total = __builtin_amdgcn_readlane(p.upto, kWaveSize - 1);
     for (int base = kWaveSize; base < SEQS; base += kWaveSize)
@@ -397,7 +403,7 @@ struct PagedAttention {
 #else   // for a host build that runs one thread at a time
   static __device__ __forceinline__ Sequence planned(const Plan&, const int* qs, const int* cl, int b) { return sequence(qs, cl, b); }
   static __device__ __forceinline__ Plan plan(const int* qs, const int* cl) {
-    Plan p = {0, 0, 0, {0, 0, 0}};
+    Plan p = {0, 0, 0, {0, 0, 0}, false};
     for (int b = 0; b < SEQS; ++b) p.total += steps_of(qs, cl, b);
     return p;
   }
@@ -416,13 +422,17 @@ struct PagedAttention {
     it.b = sequence_with_step(p, qs, cl, rem);
     it.s = planned(p, qs, cl, it.b);
     it.narrow = is_narrow(it.s.len);
-    int per_head = head_steps(it.s);
+    int per_head = p.whole ? 1 : head_steps(it.s);
     if (per_head < 1) per_head = 1;
     it.h = clamp_int(rem / per_head, 0, HKV - 1);
     rem -= it.h * per_head;
     const int tiles = tiles_of(it.s.len);
     it.tile = 0;
     tile_steps(it.s, 0, it.first, it.steps);
+    if (p.whole) {
+      inside = 0;
+      return it;
+    }
     while (rem >= it.steps && it.tile + 1 < tiles) {
       rem -= it.steps;
       ++it.tile;
@@ -803,7 +813,7 @@ struct PagedAttention {
   // ---- narrow items ----------------------------------------------------------------------------------------------
   // Bound by the reads of keys and values: 32 sequences of 200 .. 8191 keys on 32 / 8 heads of 128 in bf16 take 120 us, 108
   // of them at 5.0 TB/s in this stage (a large copy reaches 5.2); one of 131071 keys 104 us, 5.1 TB/s; 4 sequences of up to
-  // 512 keys on 12 heads of 64, where the chain of lengths, pages, rows counts, 10.4 us.  Every wave streams its own 32 keys of a step: requested a step ahead into
+  // 512 keys on 12 heads of 64, where the chain of lengths, pages, rows counts, 8.9 us.  Every wave streams its own 32 keys of a step: requested a step ahead into
   // registers, through the wave's own LDS rows (no workgroup barrier) into the products.  The next step may belong to
   // the next item: its keys, and that item's queries, are on their way while the waves' shares of the last one are added up.
   static constexpr int kMine = CPR / 2;   // pieces of K (and of V) a lane moves per step: 32 rows over 64 lanes
@@ -1038,12 +1048,13 @@ struct PagedAttention {
         if (t < inside0 || t >= inside1)
           for (int c = thread_id(); c < H * CPR; c += MONONN_BLOCK_SIZE) store_run<COHERENT, T, 8>(out + (long)t * H * D + c * 8, zero);
     }
-    const int range = range_of(unit), end = range_begin(p.total, range + 1);
-    int at = range_begin(p.total, range);
+    const int range = range_of(unit);
+    int at = range_begin(p.total, range), end = range_begin(p.total, range + 1);
     const float scale_log2 = scale * 1.44269504088896f;
     if (at >= end) return;
     int inside;
     Item it = locate(p, qs, cl, at, inside);
+    if (p.whole) end = at + it.steps;
     __syncthreads();
     while (at < end) {
       if (it.narrow) {
@@ -1160,7 +1171,7 @@ struct PagedAttention {
   static __device__ __forceinline__ void join(int unit, const float* part, const int* qs, const int* cl, T* out, char* smem) {
     const Plan p = plan(qs, cl);
     const int range = range_of(unit), begin = range_begin(p.total, range), end = range_begin(p.total, range + 1);
-    if (begin >= end) return;
+    if (p.whole || begin >= end) return;
     // the item that an earlier range began, if there is one, and the one that this range leaves unfinished
     for (int k = 0; k < 2; ++k) {
       int inside;

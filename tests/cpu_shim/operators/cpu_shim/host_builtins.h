@@ -15,6 +15,7 @@ inline void sincospif(float x, float* s, float* c) { *s = sinf(3.14159265f * x),
 #define __builtin_amdgcn_exp2f(x) exp2f(x)
 #define __builtin_amdgcn_s_setprio(p) ((void)0)
 #define __any(x) (x)
+#define __all(x) (x)
 #define __ballot(x) ((x) ? 1ull : 0ull)
 #define __shfl(v, ...) (v)
 #define __builtin_amdgcn_readlane(v, l) (v)
