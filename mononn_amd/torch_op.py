@@ -42,9 +42,11 @@ class MonoNNFunction:
         self._updates = any(p >= 0 for p in self._in_place)
         self._args_type = ctypes.c_void_p * (len(self._param_bytes) + len(self._out_bytes) + 1)
         self._temp_ptr = 0 if self._temp is None else self._temp.data_ptr()
-        self._results = [(tuple(o["dims"]), _TORCH_DTYPE[o["dtype"]], p) for o, p in zip(self.outputs, self._in_place)]
-        for (dims, dtype, _), nbytes in zip(self._results, self._out_bytes):
-            assert torch.empty(dims, dtype=dtype, device="meta").nbytes == nbytes
+        self._results = []   # extents, strides, type, parameter that is updated or -1
+        for o, p, nbytes in zip(self.outputs, self._in_place, self._out_bytes):
+            like = torch.empty(tuple(o["dims"]), dtype=_TORCH_DTYPE[o["dtype"]], device="meta")
+            assert like.nbytes == nbytes
+            self._results.append((tuple(like.shape), like.stride(), like.dtype, p))
         self.handle = id(self)
         _REGISTRY[self.handle] = self
 
@@ -73,14 +75,14 @@ class MonoNNFunction:
                 ptr = t.data_ptr()
             ptrs.append(ptr)
         outs = []
-        for dims, dtype, param in self._results:
+        for dims, strides, dtype, param in self._results:
             if param >= 0:
                 t = held[param]
                 assert t.dtype == dtype and t.shape == dims, "an input that the call updates in place must have the declared type and shape"
                 assert ptrs.count(ptrs[param]) == 1, "an input that the call updates in place must not be passed twice"
                 ptrs.append(None)
             else:
-                t = torch.empty(dims, dtype=dtype, device=device)
+                t = torch.empty_strided(dims, strides, dtype=dtype, device=device)   # a little cheaper than torch.empty
                 ptrs.append(t.data_ptr())
             outs.append(t)
         ptrs.append(self._temp_ptr)
