@@ -567,9 +567,7 @@ struct PagedAttention {
   static constexpr int kBatch = 4;
   typedef float16_t Scores[2];
   typedef half8_t Probabilities[4];   // 16 keys each
-  // row: the lane's first operand; before(): work done while the first operands are on their way
-  template <class F>
-  static __device__ __forceinline__ void score(const char* row, const Rows& r, Scores& s, F before) {
+  static __device__ __forceinline__ void score(const char* row, const Rows& r, Scores& s) {   // row: the lane's first operand
     constexpr int kProducts = 2 * QS, kBatches = (kProducts + kBatch - 1) / kBatch;   // numbered block by block of 32 keys
     half8_t k[2][kBatch];
     auto read = [&](int batch) {
@@ -581,8 +579,6 @@ struct PagedAttention {
     };
     __builtin_amdgcn_s_setprio(1);
     read(0);
-    __builtin_amdgcn_sched_barrier(0);
-    before();
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int b = 0; b < 2; ++b)
@@ -705,7 +701,8 @@ struct PagedAttention {
   // step's tile, while the next one is on its way in registers.  So that a SIMD's two waves are not at the same part at
   // the same time, the later one runs half a step behind: it begins with the products of the last step's values, which
   // therefore stay a step longer (three buffers).  Waves at their products go first where both could issue.
-  // At 5 prompts of 6830 tokens in all on 32 / 8 heads of 128 elements in bf16: 493 us with the join, 893 TFLOP/s.
+  // At 5 prompts of 6830 tokens in all on 32 / 8 heads of 128 elements in bf16: 484 us with the join, 910 TFLOP/s,
+  // at a clock that falls to 1.9 GHz: deeper prefetches of operands change nothing any more.
   // Without the shift 3 % more, without the priority 2 %, with a barrier per half step that forces the waves to take turns
   // 6 %, with the next item's first tile and queries requested before the last one's results are stored 5 %.
   static constexpr int kRuns = (kWideKeys * CPR + MONONN_BLOCK_SIZE - 1) / MONONN_BLOCK_SIZE;   // pieces of K (and of V) a thread moves per step
@@ -778,17 +775,17 @@ struct PagedAttention {
       const int key0 = begin + i * kWideKeys;
       const bool some = live && key0 <= p_last && !(WINDOW > 0 && key0 + kWideKeys - 1 < p_first - WINDOW + 1);
       const int v_next = next_buffer(v_at);
-      auto move = [&] {
-        wide_store(l, kbuf + ((i + 1) & 1) * kWideKeys * KP, KP, k_mine, k);
-        clear_unseen(l, key0 + kWideKeys, seen_lo, seen_hi, v);
-        wide_store(l, vbuf + v_next, VP, v_mine, v);
-        load_tile(i + 2);
-      };
       __syncthreads();
       if (later && weighing) weigh(vbuf + v_last + v_read, p, st);
-      if (some) score(kbuf + (i & 1) * kWideKeys * KP + k_read, r, s, move);
-      else move();
-      if (some) soft_max(key0, r, st, scale_log2, key0 + kWideKeys - 1 > p_first || (WINDOW > 0 && key0 < p_last - WINDOW + 1), s, p);
+      if (some) {
+        score(kbuf + (i & 1) * kWideKeys * KP + k_read, r, s);
+        soft_max(key0, r, st, scale_log2, key0 + kWideKeys - 1 > p_first || (WINDOW > 0 && key0 < p_last - WINDOW + 1), s, p);
+      }
+      // the next tile, where the LDS has least to do
+      wide_store(l, kbuf + ((i + 1) & 1) * kWideKeys * KP, KP, k_mine, k);
+      clear_unseen(l, key0 + kWideKeys, seen_lo, seen_hi, v);
+      wide_store(l, vbuf + v_next, VP, v_mine, v);
+      load_tile(i + 2);
       if (!later && some) weigh(vbuf + v_at + v_read, p, st);
       weighing = some;
       v_last = v_at;
