@@ -66,7 +66,7 @@ void mononn_module_destroy(mononn_module* m);
  *           and stays valid until the next call that regenerates it or until destroy. */
 const char* mononn_module_kernel_name(const mononn_module* m);
 int mononn_module_spec_json(mononn_module* m, const char** text, size_t* len);
-int mononn_module_source(const mononn_module* m, const char* file /* "main.hip" | "headers.h" */,
+int mononn_module_source(const mononn_module* m, const char* file /* "main.hip" | "headers.h" | "operators.h" (modules with mononn$ calls) */,
                          const char** text, size_t* len);
 int mononn_module_code_object(const mononn_module* m, const void** data, size_t* len);
 int mononn_module_summary(mononn_module* m, const char** text, size_t* len);

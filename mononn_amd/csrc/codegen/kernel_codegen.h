@@ -48,7 +48,7 @@ struct NodeReport {
 
 struct HipProgram {
   std::string kernel_name;
-  std::map<std::string, std::string> files;   // "headers.h" (device runtime) and "main.hip"
+  std::map<std::string, std::string> files;   // "headers.h" (device runtime), "main.hip" and, where it is included, "operators.h"
   // main.hip = preamble + global_decls + body; kept apart for multi-candidate translation units
   std::string preamble, body;
   std::vector<std::string> global_decls;

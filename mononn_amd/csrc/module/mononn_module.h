@@ -71,7 +71,7 @@ class MonoNNModule {
   double read_stage_clock(std::vector<unsigned long long>* ticks, int* n_stages, int* grid);
 
   // ---- dump (TF_MONONN_DUMP_DIR layout, mononn_module_tuner.cc:457-603) ------------------------
-  // writes <dir>/<cluster_N>/<context>.json, <context>.hsaco, <context>_src/{headers.h,main.hip}
+  // writes <dir>/<cluster_N>/<context>.json, <context>.hsaco, <context>_src/{headers.h,main.hip[,operators.h]}
   void dump_candidate(const std::string& dump_dir) const;
   // writes best_tuning_spec.{json,hsaco}
   void dump_best(const std::string& dump_dir) const;

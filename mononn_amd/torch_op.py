@@ -78,7 +78,9 @@ class MonoNNFunction:
         for dims, strides, dtype, param in self._results:
             if param >= 0:
                 t = held[param]
-                assert t.dtype == dtype and t.shape == dims, "an input that the call updates in place must have the declared type and shape"
+                assert t.dtype == dtype, "an input that the call updates in place must have the declared type"
+                if t.shape != dims:
+                    t = t.view(dims)
                 assert ptrs.count(ptrs[param]) == 1, "an input that the call updates in place must not be passed twice"
                 ptrs.append(None)
             else:

@@ -490,6 +490,9 @@ def test_an_updated_input_is_passed_once_and_not_through_the_pure_operator(gpu_d
     assert not kc.any() and not vc.any()
     fn(k, k, kc, vc, *meta)   # k and v may be one tensor
     assert kc[0, 0].all() and vc[0, 0].all() and kc.sum() == vc.sum() == 128
+    # a cache of another shape is its bytes, as every input is; the result has the declared one and the same storage
+    new_k, _ = fn(k, k, kc.view(48, 128), vc, *meta)
+    assert new_k.shape == (3, 16, 2, 64) and new_k.data_ptr() == kc.data_ptr()
 
 
 def test_two_functions_in_two_graphs(gpu_device):
