@@ -566,6 +566,31 @@ def test_launch_with_the_static_arena_and_null_slots(gpu_device):
     a.close()
 
 
+def test_operands_and_results_in_other_layouts(gpu_device):
+    # any order of dimensions in memory at the module's boundary; the operators themselves work on row-major values
+    rng = np.random.default_rng(45)
+    T, H, HKV, D, page = 5, 4, 2, 32, 4
+    table, qs, cl, pages = dc.paged_batch(rng, [2, 3], [9, 30], page)
+    text, outs = dc.attention_module(T, H, HKV, D, pages, page, 2, table.shape[1], "f16", 0.2)
+    args = [rng.normal(size=s).astype(np.float16) for s in ((T, H, D), (pages, page, HKV, D), (pages, page, HKV, D))] + [table, qs, cl]
+    (want,) = run(text, outs, args)
+    # q with the heads slowest, the keys with the elements slowest, the table by columns
+    q, c, t = f"f16[{T},{H},{D}]", f"f16[{pages},{page},{HKV},{D}]", f"s32[2,{table.shape[1]}]"
+    turned = [args[0].transpose(1, 0, 2), args[1].transpose(3, 2, 1, 0), args[2], table.T, qs, cl]
+    lines = []
+    for line in text.splitlines():
+        if "parameter(0)" in line:
+            line = line.replace(q + "{2,1,0}", q + "{2,0,1}")
+        elif "parameter(1)" in line:
+            line = line.replace(c + "{3,2,1,0}", c + "{0,1,2,3}")
+        elif "parameter(3)" in line:
+            line = line.replace(t + "{1,0}", t + "{0,1}")
+        lines.append(line)
+    assert lines != text.splitlines()
+    (got,) = run("\n".join(lines), outs, [np.ascontiguousarray(a) for a in turned])
+    assert np.array_equal(got, want)
+
+
 def test_weights_as_constants(gpu_device):
     # the usual home of weights: module constants, uploaded once, read in place
     rng = np.random.default_rng(33)
