@@ -356,23 +356,67 @@ struct PagedAttention {
   };
   static __device__ __forceinline__ int steps_of(const int* qs, const int* cl, int b) { return b < SEQS ? HKV * head_steps(sequence(qs, cl, b)) : 0; }
 #ifndef MONONN_ONE_THREAD
+  // Sums and maxima over the lanes of the first 64 sequences: moves inside rows of 16 lanes on the vector unit, then the
+  // rows' results through scalar registers.  (Six exchanges through the LDS take half a microsecond, which a call of single
+  // tokens has twice.)
+  static constexpr int kRows = SEQS >= kWaveSize ? 4 : (SEQS + 15) / 16;
+  template <int SHIFT>
+  static __device__ __forceinline__ int lanes_before(int v) { return __builtin_amdgcn_update_dpp(0, v, 0x110 + SHIFT, 0xf, 0xf, false); }   // 0 where the row begins
   static __device__ __forceinline__ int sum_upto(int v) {
+    v += lanes_before<1>(v);
+    v += lanes_before<2>(v);
+    v += lanes_before<4>(v);
+    v += lanes_before<8>(v);
+    const int row = lane_id() >> 4;
+    int before = 0;   // of the rows in front
 #pragma unroll
-    for (int off = 1; off < kWaveSize; off <<= 1) {
-      const int o = __shfl_up(v, off, kWaveSize);
-      if (lane_id() >= off) v += o;
+    for (int i = 0; i < 3; ++i) {
+      const int of_row = __builtin_amdgcn_readlane(v, i * 16 + 15);
+      before += row > i ? of_row : 0;
     }
+    v += before;
     return v;
+  }
+  template <class Op>
+  static __device__ __forceinline__ int over_sequences(int v, Op op) {   // lanes behind the last sequence hold 0
+    v = op(v, dpp_move<0xB1>(v));    // quad_perm [1,0,3,2]
+    v = op(v, dpp_move<0x4E>(v));    // quad_perm [2,3,0,1]
+    v = op(v, dpp_move<0x141>(v));   // row_half_mirror
+    v = op(v, dpp_move<0x140>(v));   // row_mirror
+    int r = __builtin_amdgcn_readlane(v, 0);
+#pragma unroll
+    for (int row = 1; row < kRows; ++row) r = op(r, __builtin_amdgcn_readlane(v, row * 16));
+    return r;
+  }
+  // Where there are no more items than ranges, an item may be a range, uncut: as long as the longest takes no more steps
+  // than an equal share and what the parts would cost.  In steps, that is two for the barrier and the join, and one for
+  // 256 blocks of 32 rows in parts, written and read (a wide block of 128 elements is 17 KB).
+  //   32 / 8 heads of 128 elements in bf16, us uncut and cut: one prompt of 256 tokens 16.7 and 21.3, of 1024 36 and 47, of
+  //   2048 63 and 100; 32 tokens each behind two caches of 1200 keys 33 and 19 (cut, by the rule)
+  //   12 heads of 64 elements, single tokens of 4 sequences of 210 .. 505 keys: 8.5 and 8.9
+  static __device__ __forceinline__ bool fewer_without_cuts(const Sequence& s, int tiles) {
+    int first, shortest = 0, longest = 0;
+    if (tiles > 0) {
+      tile_steps(s, 0, first, shortest);
+      tile_steps(s, tiles - 1, first, longest);
+      shortest = shortest < 1 << 18 ? shortest : 1 << 18, longest = longest < 1 << 18 ? longest : 1 << 18;   // sums stay below 2^31
+    }
+    if constexpr (kAllNarrow) return SEQS * HKV <= GRID && __all(longest <= 2);
+    const auto sum = [](int a, int b) { return a + b; };
+    const auto larger = [](int a, int b) { return a > b ? a : b; };
+    const int items = over_sequences(HKV * tiles, sum);
+    if (items > GRID) return false;
+    const int steps = over_sequences(HKV * tiles * (shortest + longest) / 2, sum), most = over_sequences(longest, larger);
+    const int blocks = over_sequences(tiles == 0 || is_narrow(s.len) ? 0 : clamp_int((s.len * G + 31) / 32, 0, NW), larger);
+    const int parts = steps < GRID + items ? steps : GRID + items;
+    return most <= steps / GRID + 2 + parts * blocks / 256;
   }
   static __device__ __forceinline__ Plan plan(const int* qs, const int* cl) {
     Plan p;
     p.mine = sequence(qs, cl, lane_id() < SEQS ? lane_id() : SEQS - 1);
-    const int per_head = lane_id() < SEQS ? head_steps(p.mine) : 0;
-    p.whole = false;
-    // A handful of short narrow items is not cut, one for a workgroup: a second step costs less than a join (12 heads of
-    // 64 elements, 4 sequences of 210 .. 505 keys: 8.9 us, 9.3 with every step a part).
-    if constexpr (SEQS <= kWaveSize && SEQS * HKV <= GRID) p.whole = __all(per_head == 0 || (per_head <= 2 && is_narrow(p.mine.len)));
-    p.steps = HKV * (p.whole ? (per_head > 0 ? 1 : 0) : per_head);
+    const int tiles = lane_id() < SEQS ? tiles_of(p.mine.len) : 0;
+    p.whole = SEQS <= kWaveSize && fewer_without_cuts(p.mine, tiles);
+    p.steps = HKV * (p.whole || tiles == 0 ? tiles : head_steps(p.mine));
     p.upto = sum_upto(p.steps);
     p.total = __builtin_amdgcn_readlane(p.upto, kWaveSize - 1);
     for (int base = kWaveSize; base < SEQS; base += kWaveSize)
@@ -422,13 +466,13 @@ struct PagedAttention {
     it.b = sequence_with_step(p, qs, cl, rem);
     it.s = planned(p, qs, cl, it.b);
     it.narrow = is_narrow(it.s.len);
-    int per_head = p.whole ? 1 : head_steps(it.s);
+    const int tiles = tiles_of(it.s.len);
+    int per_head = p.whole ? tiles : head_steps(it.s);
     if (per_head < 1) per_head = 1;
     it.h = clamp_int(rem / per_head, 0, HKV - 1);
     rem -= it.h * per_head;
-    const int tiles = tiles_of(it.s.len);
-    it.tile = 0;
-    tile_steps(it.s, 0, it.first, it.steps);
+    it.tile = p.whole ? rem : 0;
+    tile_steps(it.s, it.tile, it.first, it.steps);
     if (p.whole) {
       inside = 0;
       return it;
