@@ -58,8 +58,9 @@ struct MatvecPlan {
   int64_t blocks_per_workgroup() const { return ((K + 128 * p - 1) / (128 * p) + sk - 1) / sk; }
   int64_t x_bytes() const { return blocks_per_workgroup() * p * 256 * (x_rows() | 1); }   // an odd pitch
 };
-// The plan whose busiest workgroup reads least, weights and its slice of x together (16 rows of x on 4096 x 14336 weights:
-// 13.4 us with slices of 57 KB of x, 17 with the 115 KB that the weights alone would choose); among equals larger blocks
+// The plan whose busiest workgroup reads least: weights, its slice of x (16 rows of x on 4096 x 14336 weights: 13.4 us with
+// slices of 57 KB of x, 17 with the 115 KB that the weights alone would choose) and its share of the parts (7 rows on
+// 5185 x 10880 weights: 12.6 us with 6 slices, 20 with the 43 that would be chosen without).  Among equals larger blocks
 // (fewer loads of scales), then fewer slices, then fewer shares (fewer starts of a workgroup's loads).
 MatvecPlan plan_matvec(const Instr* call, int64_t grid, int64_t waves) {
   const auto &x = call->operands[0]->shape.dims, &w = call->operands[1]->shape.dims, &s = call->operands[2]->shape.dims;
@@ -76,8 +77,9 @@ MatvecPlan plan_matvec(const Instr* call, int64_t grid, int64_t waves) {
         c.p = p, c.sk = sk, c.wk = wk;
         if (c.x_bytes() > 128 * 1024) continue;
         const int64_t at_once = waves / wk, units = (tiles + at_once - 1) / at_once * sk * passes;
-        // 16-byte loads of the busiest workgroup: weights, and x
-        const int64_t busiest = (units + grid - 1) / grid * ((c.blocks_per_workgroup() + wk - 1) / wk * p * 64 * waves + c.x_bytes() / 16);
+        // 16-byte loads of the busiest workgroup: weights and x, and its share of the parts, written and read
+        const int64_t parts = split ? sk * best.M * best.N * 8 / 16 / grid : 0;
+        const int64_t busiest = (units + grid - 1) / grid * ((c.blocks_per_workgroup() + wk - 1) / wk * p * 64 * waves + c.x_bytes() / 16) + parts;
         if (least < 0 || busiest < least) {
           least = busiest;
           best.p = p, best.sk = sk, best.wk = wk;

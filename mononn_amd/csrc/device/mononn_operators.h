@@ -1426,7 +1426,7 @@ struct MatvecW4 {
       for (int k = 0; k < 4; ++k) a[0][t][k] = a[1][t][k] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
     }
     __syncthreads();
-    x_operands(xs, block_at(0) - first, 0, a[0]);
+    if (count > 0) x_operands(xs, block_at(0) - first, 0, a[0]);   // a wave behind the slice's last block has none
     for (int base = 0; base < count; base += DEPTH) {
 #pragma unroll
       for (int i = 0; i < DEPTH; ++i) {
