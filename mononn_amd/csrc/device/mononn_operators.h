@@ -854,7 +854,7 @@ struct PagedAttention {
   // ---- narrow items ----------------------------------------------------------------------------------------------
   // Bound by the reads of keys and values: 32 sequences of 200 .. 8191 keys on 32 / 8 heads of 128 in bf16 take 120 us, 108
   // of them at 5.0 TB/s in this stage (a large copy reaches 5.2); one of 131071 keys 104 us, 5.1 TB/s; 4 sequences of up to
-  // 512 keys on 12 heads of 64, where the chain of lengths, pages, rows counts, 8.9 us.  Every wave streams its own 32 keys of a step: requested a step ahead into
+  // 512 keys on 12 heads of 64, where the chain of lengths, pages, rows counts, 8.5 us.  Every wave streams its own 32 keys of a step: requested a step ahead into
   // registers, through the wave's own LDS rows (no workgroup barrier) into the products.  The next step may belong to
   // the next item: its keys, and that item's queries, are on their way while the waves' shares of the last one are added up.
   static constexpr int kMine = CPR / 2;   // pieces of K (and of V) a lane moves per step: 32 rows over 64 lanes
