@@ -62,11 +62,15 @@ struct MatvecPlan {
 // slices of 57 KB of x, 17 with the 115 KB that the weights alone would choose) and its share of the parts (7 rows on
 // 5185 x 10880 weights: 12.6 us with 6 slices, 20 with the 43 that would be chosen without).  Among equals larger blocks
 // (fewer loads of scales), then fewer slices, then fewer shares (fewer starts of a workgroup's loads).
+// What a unit's first loads cost, in 16-byte loads of a workgroup: without it one row on 27648 x 5120 weights takes seven
+// rounds of small blocks, 22.6 us instead of 15.8; with 1024 8 rows on 11008 x 4096 take one round, 14.7 instead of 12.3.
+constexpr int64_t kUnitStart = 512;
 MatvecPlan plan_matvec(const Instr* call, int64_t grid, int64_t waves) {
   const auto &x = call->operands[0]->shape.dims, &w = call->operands[1]->shape.dims, &s = call->operands[2]->shape.dims;
   MatvecPlan best{x[0], w[0], x[1], x[1] / s[1]};
   const bool split = hlo::matvec_w4_in_parts(best.M, best.K);
   const int64_t tiles = (best.N + 15) / 16, passes = (best.M + 16 * best.row_blocks() - 1) / (16 * best.row_blocks());
+  const int64_t products = best.M > 4 && best.group >= 128 ? best.row_blocks() : 1;   // a pass of more rows reads more of the LDS for the same weights
   int64_t least = -1;
   for (int64_t p : {4, 2, 1}) {
     if (p > 1 && best.M > 4 && (best.group >= 128 || p > 2)) continue;   // MatvecW4::kWhole, and the scales of kSwap
@@ -79,7 +83,8 @@ MatvecPlan plan_matvec(const Instr* call, int64_t grid, int64_t waves) {
         const int64_t at_once = waves / wk, units = (tiles + at_once - 1) / at_once * sk * passes;
         // 16-byte loads of the busiest workgroup: weights and x, and its share of the parts, written and read
         const int64_t parts = split ? sk * best.M * best.N * 8 / 16 / grid : 0;
-        const int64_t busiest = (units + grid - 1) / grid * ((c.blocks_per_workgroup() + wk - 1) / wk * p * 64 * waves + c.x_bytes() / 16) + parts;
+        const int64_t rounds = (units + grid - 1) / grid, stagings = sk * passes == 1 ? 1 : rounds;
+        const int64_t busiest = rounds * ((c.blocks_per_workgroup() + wk - 1) / wk * p * 64 * waves * products + kUnitStart) + stagings * (c.x_bytes() / 16) + parts;
         if (least < 0 || busiest < least) {
           least = busiest;
           best.p = p, best.sk = sk, best.wk = wk;
@@ -199,11 +204,12 @@ NodeFunction generate_operator(const graph::Program& prog, const graph::Node& no
         break;
       }
       const std::string x = input(0), w = input(1), s = input(2), z = zeros ? input(3) : "nullptr", out = ptrs.output(ins);
-      body << "Matvec::unit(unit, " << x << ", " << w << ", " << s << ", " << z << ", " << (parts_stage ? "nullptr, " + out : out + ", nullptr") << ", smem);";
       const int64_t at_once = ls.waves() / p.wk, row_blocks = p.row_blocks();
+      const int64_t units = ((p.N + 15) / 16 + at_once - 1) / at_once * p.sk * ((p.M + 16 * row_blocks - 1) / (16 * row_blocks));
+      check_units(std::min<int64_t>(units, grid));   // a workgroup's units are one unit of the stage: x may stay in its LDS
+      body << "Matvec::units<" << f.num_units << ">(unit, " << x << ", " << w << ", " << s << ", " << z << ", " << (parts_stage ? "nullptr, " + out : out + ", nullptr") << ", smem);";
       f.smem_bytes = static_cast<int>((p.wk > 1 ? ls.waves() * row_blocks * 1024 : 0) + p.x_bytes());
-      check_units(((p.N + 15) / 16 + at_once - 1) / at_once * p.sk * ((p.M + 16 * row_blocks - 1) / (16 * row_blocks)));
-      body << " static_assert(Matvec::lds_bytes() == " << f.smem_bytes << " && Matvec::num_units() == " << f.num_units << ", \"launch\");";
+      body << " static_assert(Matvec::lds_bytes() == " << f.smem_bytes << " && Matvec::num_units() == " << units << ", \"launch\");";
       break;
     }
     default: MONONN_FAIL(kInternal) << node.name << " is not an operator";
