@@ -74,10 +74,9 @@ void MonoNNModule::generate_code() {
     kernel_name_ = "mononn_" + shortn;
   }
   if (!spec_given_) {
-    // Default launch: four waves per compute unit, eight when every node is an operator call.  Their kernels hide the
-    // memory's latency and the soft-max behind a second wave per SIMD (256 -> 512 threads: attention of prompt chunks
-    // 900 -> 533 us, of one token over 131071 keys 116 -> 106); GEMM tiles want the registers of one (the 12-layer
-    // decoder step of four tokens 445 -> 795 us).
+    // Default launch: four waves per compute unit, eight when every node is an operator call.  A second wave per SIMD hides
+    // the soft-max of attention over prompts (6830 tokens, 256 -> 512 threads: 742 -> 490 us; single tokens, bound by
+    // memory, take the same); GEMM tiles want the registers of one (the 12-layer decoder step of four tokens 426 -> 453 us).
     bool operators = false, others = false;
     for (auto& up : mod->entry->instrs) {
       const hlo::Instr& i = *up;
