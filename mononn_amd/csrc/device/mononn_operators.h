@@ -610,7 +610,30 @@ struct PagedAttention {
   // moves across the marks between them.
   static constexpr int kBatch = 4;
   typedef float16_t Scores[2];
-  typedef half8_t Probabilities[4];   // 16 keys each
+  // Rounded to the element type, probabilities would cost a result as much as its own rounding does (its error against 64
+  // bits grows by 25 to 45 %), so each goes into the second product as two values of that type: its leading bits, and what
+  // they leave.  Together they hold 16 bits of it in bf16, 22 in f16.  Single tokens, bound by the reads, take the same time
+  // (1 % more at most); 6830 prompt tokens, bound by the products, take 645 us instead of 486.
+  struct Probabilities {
+    half8_t lead[4], rest[4];   // 16 keys each
+  };
+  static __device__ __forceinline__ void split(float e, half_t& lead, half_t& rest) {
+    if constexpr (kBf16) {
+      const unsigned top = __builtin_bit_cast(unsigned, e) & 0xffff0000u;   // cut, not rounded: the remainder is exact
+      lead = __builtin_bit_cast(half_t, (unsigned short)(top >> 16));
+      rest = __builtin_bit_cast(half_t, (T)(e - __builtin_bit_cast(float, top)));
+    } else {
+      lead = (half_t)e;
+      rest = (half_t)(e - (float)lead);
+    }
+  }
+  // The reference of a query's exponentials only has to stay near its maximum: it moves, and what has been added up
+  // is rescaled, when some query of the wave has outgrown its own by 2^6, which after the first steps is rare.  In f16 it
+  // is set 2^9 below the maximum: exponentials up to 2^15 are in range, and keys count that lie 2^34 below the maximum
+  // (without it those 2^25 below would vanish from the product, but not from the sum: 131071 of them are 0.4 % of it).
+  static constexpr float kOutgrown = 6.0f, kBelow = kBf16 ? 0.0f : 9.0f;
+  static __device__ __forceinline__ float moved(float reference, float top) { return fmaxf(reference, top - kBelow); }
+  static __device__ __forceinline__ bool outgrown(float reference, float top) { return __any(top - kBelow > reference + kOutgrown); }
   static __device__ __forceinline__ void score(const char* row, const Rows& r, Scores& s) {   // row: the lane's first operand
     constexpr int kProducts = 2 * QS, kBatches = (kProducts + kBatch - 1) / kBatch;   // numbered block by block of 32 keys
     half8_t k[2][kBatch];
@@ -658,11 +681,8 @@ struct PagedAttention {
 #pragma unroll
       for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
     top = half_waves_max(top) * scale_log2;
-    // The reference of a query's exponentials only has to stay near its maximum: it moves, and what has been added up
-    // is rescaled, when some query of the wave has outgrown its own by 2^6 (probabilities up to 64 leave f16 and the
-    // sums room), which after the first steps is rare.
-    if (__any(top > st.m + 6.0f)) {
-      const float m = fmaxf(st.m, top);
+    if (outgrown(st.m, top)) {
+      const float m = moved(st.m, top);
       const float a = __builtin_amdgcn_exp2f(st.m - m);
       st.l *= a;
 #pragma unroll
@@ -671,7 +691,6 @@ struct PagedAttention {
         for (int i = 0; i < 16; ++i) st.o[t][i] *= a;
       st.m = m;
     }
-    // probabilities are rounded to the element type for the second product; the sum takes the unrounded ones
     float sum = 0.0f;
 #pragma unroll
     for (int b = 0; b < 2; ++b)
@@ -679,7 +698,10 @@ struct PagedAttention {
       for (int i = 0; i < 16; ++i) {
         const float e = __builtin_amdgcn_exp2f(s[b][i] * scale_log2 - st.m);
         sum += e;
-        p[b * 2 + i / 8][i % 8] = __builtin_bit_cast(half_t, (T)e);
+        half_t lead, rest;
+        split(e, lead, rest);
+        p.lead[b * 2 + i / 8][i % 8] = lead;
+        p.rest[b * 2 + i / 8][i % 8] = rest;
       }
     st.l += sum;
   }
@@ -701,7 +723,11 @@ struct PagedAttention {
       if (t + 1 < kBatches) read(t + 1);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) st.o[t] = mfma_32x32x16<kBf16>(__builtin_bit_cast(half8_t, v[t & 1][k]), p[k], st.o[t]);
+      for (int k = 0; k < 4; ++k) {
+        const half8_t values = __builtin_bit_cast(half8_t, v[t & 1][k]);
+        st.o[t] = mfma_32x32x16<kBf16>(values, p.rest[k], st.o[t]);
+        st.o[t] = mfma_32x32x16<kBf16>(values, p.lead[k], st.o[t]);
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
     static_assert(kProducts == kBatches * kBatch, "a batch per tile");
@@ -739,16 +765,17 @@ struct PagedAttention {
   static __device__ __forceinline__ float inverse(float l) { return l > 0.0f || l != l ? 1.0f / l : 0.0f; }   // a row without keys: zeros
 
   // ---- wide items ------------------------------------------------------------------------------------------------
-  // Bound by how well two waves per SIMD overlap: of the 3900 clocks of a step the matrix units are busy for 2050 (two
-  // waves), the vector units for 2000 (an exponential per score takes a quarter of that), the LDS reads of K and V for
-  // about as long; leaving out any one of them saves no more than 6 %.  One barrier per step: it ends the stores of the
+  // Bound by the matrix units, and by how well two waves per SIMD hide the rest behind them: of the 5200 clocks of a step they
+  // are busy for 3070 (two waves; a third of it the remainders of the probabilities), the vector units for 2600 (an
+  // exponential per score takes a fifth of that), the LDS reads of K and V for 2000.  One barrier per step: it ends the stores of the
   // step's tile, while the next one is on its way in registers.  So that a SIMD's two waves are not at the same part at
   // the same time, the later one runs half a step behind: it begins with the products of the last step's values, which
   // therefore stay a step longer (three buffers).  Waves at their products go first where both could issue.
-  // At 5 prompts of 6830 tokens in all on 32 / 8 heads of 128 elements in bf16: 484 us with the join, 910 TFLOP/s,
-  // at a clock that falls to 1.9 GHz: deeper prefetches of operands change nothing any more.
-  // Without the shift 3 % more, without the priority 2 %, with a barrier per half step that forces the waves to take turns
-  // 6 %, with the next item's first tile and queries requested before the last one's results are stored 5 %.
+  // At 5 prompts of 6830 tokens in all on 32 / 8 heads of 128 elements in bf16: 645 us with the join, 682 TFLOP/s, 1020 with
+  // the remainders' products, at a clock that falls to 1.9 GHz.
+  // With probabilities in one value (486 us): without the shift 3 % more, without the priority 2 %, with a barrier per half step
+  // that forces the waves to take turns 6 %, with the next item's first tile and queries requested before the last one's
+  // results are stored 5 %.
   static constexpr int kRuns = (kWideKeys * CPR + MONONN_BLOCK_SIZE - 1) / MONONN_BLOCK_SIZE;   // pieces of K (and of V) a thread moves per step
   static __device__ __forceinline__ int wide_piece(const Lane& l, int run) { return (run * NW + l.wave) * kWaveSize; }
   static __device__ __forceinline__ void wide_store(const Lane& l, char* buf, int pitch, int mine, const half8_t (&x)[kRuns]) {
@@ -933,29 +960,34 @@ struct PagedAttention {
     }
     float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
     top = quarter_waves_max(half_waves_max(top)) * scale_log2;
-    if (__any(top > st.m + 6.0f)) {   // as in soft_max()
-      const float m = fmaxf(st.m, top);
+    if (outgrown(st.m, top)) {   // as in soft_max()
+      const float m = moved(st.m, top);
       const float a = __builtin_amdgcn_exp2f(st.m - m);
       st.l *= a;
 #pragma unroll
       for (int t = 0; t < kTiles; ++t) st.o[t] *= a;
       st.m = m;
     }
-    half8_t p;
+    half8_t lead, rest;
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float e = __builtin_amdgcn_exp2f(s[b][i] * scale_log2 - st.m);
         st.l += e;
-        p[b * 4 + i] = __builtin_bit_cast(half_t, (T)e);
+        half_t l16, r16;
+        split(e, l16, r16);
+        lead[b * 4 + i] = l16;
+        rest[b * 4 + i] = r16;
       }
 #pragma unroll
     for (int t = 0; t < kTiles; ++t) {
       struct { mononn_short4 lo, hi; } v;
       v.lo = MONONN_LDS_READ_TR16(vrow + t * 32);
       v.hi = MONONN_LDS_READ_TR16(vrow + 16 * VPN + t * 32);
-      st.o[t] = mfma_16x16x32<kBf16>(__builtin_bit_cast(half8_t, v), p, st.o[t]);
+      const half8_t values = __builtin_bit_cast(half8_t, v);
+      st.o[t] = mfma_16x16x32<kBf16>(values, rest, st.o[t]);
+      st.o[t] = mfma_16x16x32<kBf16>(values, lead, st.o[t]);
     }
   }
   static __device__ __forceinline__ void narrow_out(T* out, long row, bool valid, int tile, float4_t o, float inv) {

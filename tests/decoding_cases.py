@@ -92,6 +92,16 @@ def attention_bound(want, mags, D, dtype):
     return (u + 3 * ds + 2.0 ** -20) * mags["weighted"] + under * mags["plain"] + u * np.abs(want) * 1.01 + under
 
 
+def split_attention_bound(want, mags, D, dtype):
+    """attention_bound for probabilities that go into the second product in two values of the element type.  Scores as there.
+    The leading value leaves less than 2^-7 (bf16, cut) or at most 2^-11 (f16) of a probability, and the second is that to
+    half a step: 2^-9 of 2^-7 (the remainder's own leading bit counts), or 2^-11 of 2^-11.  In f16 a second value below the
+    normal range is off by 2^-25 where the sum is at least 2^9.  The products are added in f32 (2^-22), likewise the sum."""
+    ds = (D + 4) * 2.0 ** -24 * mags["scores"][..., None] + 2.0 ** -21
+    lost, under, tiny = (2.0 ** -16, 0.0, 0.0) if dtype == "bf16" else (2.0 ** -22, 2.0 ** -34, 2.0 ** -25)
+    return (3 * ds + lost + 2.0 ** -20) * mags["weighted"] + under * mags["plain"] + HALF_STEP[dtype] * np.abs(want) * 1.01 + tiny
+
+
 # ---- 4-bit products -----------------------------------------------------------------------------------------------------
 def w4_module(M, N, K, group, dtype, zeros):
     def build(e):

@@ -280,6 +280,42 @@ def test_paged_attention_without_new_tokens(gpu_device):
         assert not got.any()
 
 
+@pytest.mark.parametrize("block", [256, 512])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("n", [1, 30])
+def test_paged_attention_of_values_that_cancel(gpu_device, n, dtype, block):
+    # few keys of opposite values: what is left of them shows every bit that a weight has lost on the way
+    rng = np.random.default_rng(46)
+    H, D, page, B = 2, 16, 8, 24
+    new, ctx = [n] * B, [n + 1 + 2 * i for i in range(B)]
+    table, qs, cl, pages = dc.paged_batch(rng, new, ctx, page)
+    text, outs = dc.attention_module(sum(new), H, H, D, pages, page, B, table.shape[1], dtype, 0.25)
+    q, kc = dc.bits(rng.normal(size=(sum(new), H, D)), dtype), dc.bits(rng.normal(size=(pages, page, H, D)), dtype)
+    vc = dc.bits(rng.choice([-1.0, 1.0], (pages, page, H, D)), dtype)
+    mags = {}
+    want = decoding.paged_attention(dc.values(q, dtype), dc.values(kc, dtype), dc.values(vc, dtype), table, qs, cl, 0.25, 0, mags)
+    (got,) = run(text, outs, [q, kc, vc, table, qs, cl], block)
+    within(dc.values(got, dtype), want, dc.split_attention_bound(want, mags, D, dtype))
+
+
+@pytest.mark.parametrize("n", [1, 20])
+def test_paged_attention_counts_keys_far_below_the_maximum(gpu_device, n):
+    # f16: one key that outweighs each of the others by 2^26, which together are a five-hundredth of it; one workgroup, whose
+    # waves see all of them
+    D, page, ctx = 16, 32, 131072
+    rng = np.random.default_rng(47)
+    table, qs, cl, pages = dc.paged_batch(rng, [n], [ctx], page)
+    text, outs = dc.attention_module(n, 1, 1, D, pages, page, 1, table.shape[1], "f16", 1.0)
+    q, kc, vc = np.zeros((n, 1, D), np.float16), np.zeros((pages, page, 1, D), np.float16), np.ones((pages, page, 1, D), np.float16)
+    q[..., 0], kc[table[0, 0], 0, 0, 0] = 1.0, 18.0
+    vc[table[0, 0], 0] = 0.0
+    mags = {}
+    want = decoding.paged_attention(q, kc, vc, table, qs, cl, 1.0, 0, mags)
+    assert 1.9e-3 < want.min() and want.max() < 2.1e-3
+    (got,) = run(text, outs, [q, kc, vc, table, qs, cl], 256, 1)
+    within(got.astype(np.float64), want, dc.split_attention_bound(want, mags, D, "f16"))
+
+
 # ---- 4-bit products -----------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("block", [256, 512])
 @pytest.mark.parametrize("M, N, K, group, dtype, zeros", [
