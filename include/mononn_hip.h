@@ -81,6 +81,10 @@ int mononn_module_buffer_info(const mononn_module* m, int* n_params, const int64
  * nor written and may be NULL.
  * No counterpart in the reference. */
 int mononn_module_liveout_parameter(const mononn_module* m, int index, int* parameter);
+/* *updated receives 1 if a launch writes to the buffer of entry parameter `index` (a cache of mononn$kv_append, whether or
+ * not the updated cache is a live-out as well), else 0; *element_type (NULL to skip) its declared element type, "f16" ...
+ * No counterpart in the reference. */
+int mononn_module_parameter_updated(const mononn_module* m, int index, int* updated, const char** element_type);
 /* grid / block / dynamic LDS of the launch (best_tuning_spec.json keys grid_dim, block_dim, smem_size;
  * README.md:199-200) and the number of grid-wide barriers in the kernel. */
 /* Whether the module brings its own temp arena (the caller would then pass NULL in the temp slot of

@@ -55,6 +55,7 @@ def _load_library() -> ctypes.CDLL:
     lib.mononn_module_buffer_info.argtypes = [c.c_void_p, P(c.c_int), P(P(c.c_int64)), P(c.c_int), P(P(c.c_int64)),
                                               P(c.c_int64)]
     lib.mononn_module_liveout_parameter.argtypes = [c.c_void_p, c.c_int, P(c.c_int)]
+    lib.mononn_module_parameter_updated.argtypes = [c.c_void_p, c.c_int, P(c.c_int), P(c.c_char_p)]
     lib.mononn_module_launch_dims.argtypes = [c.c_void_p, P(c.c_int), P(c.c_int), P(c.c_int), P(c.c_int)]
     lib.mononn_module_regional_barriers.argtypes = [c.c_void_p, P(c.c_int)]
     lib.mononn_module_owns_temp.argtypes = [c.c_void_p]
@@ -83,7 +84,7 @@ _lib = _load_library()
 EXPORTED_SYMBOLS = [
     "mononn_last_error", "mononn_version", "mononn_compile", "mononn_tune", "mononn_compile_from_spec_dir",
     "mononn_module_destroy", "mononn_module_kernel_name", "mononn_module_spec_json", "mononn_module_source",
-    "mononn_module_code_object", "mononn_module_summary", "mononn_module_buffer_info", "mononn_module_liveout_parameter", "mononn_module_launch_dims", "mononn_module_regional_barriers", "mononn_module_owns_temp",
+    "mononn_module_code_object", "mononn_module_summary", "mononn_module_buffer_info", "mononn_module_liveout_parameter", "mononn_module_parameter_updated", "mononn_module_launch_dims", "mononn_module_regional_barriers", "mononn_module_owns_temp",
     "mononn_module_num_constants", "mononn_module_constant_info", "mononn_module_set_constant", "mononn_module_load",
     "mononn_launch", "mononn_launch_static_temp", "mononn_static_temp_bytes", "mononn_module_synchronize", "mononn_module_global", "mononn_time_kernel", "mononn_module_stage_clock", "mononn_module_stage_name", "mononn_module_dump", "mononn_device_count", "mononn_device_info"]
 
@@ -191,6 +192,16 @@ class MonoNNModule:
             p = ctypes.c_int()
             _check(_lib.mononn_module_liveout_parameter(self._h, i, ctypes.byref(p)))
             out.append(p.value)
+        return out
+
+    def updated_parameters(self) -> Dict[int, str]:
+        """The entry parameters whose buffers a launch writes to, whether or not what it leaves there is a live-out too,
+        and their element types."""
+        out, updated, name = {}, ctypes.c_int(), ctypes.c_char_p()
+        for i in range(len(self.buffer_info()["parameters"])):
+            _check(_lib.mononn_module_parameter_updated(self._h, i, ctypes.byref(updated), ctypes.byref(name)))
+            if updated.value:
+                out[i] = name.value.decode()
         return out
 
     def launch_dims(self) -> dict:

@@ -175,6 +175,16 @@ int mononn_module_liveout_parameter(const mononn_module* m, int index, int* para
   });
 }
 
+int mononn_module_parameter_updated(const mononn_module* m, int index, int* updated, const char** element_type) {
+  return guarded([&] {
+    require(m != nullptr && updated != nullptr, "NULL argument");
+    auto& pu = m->impl->hip_program().parameter_updated;
+    require(index >= 0 && index < static_cast<int>(pu.size()), "parameter index out of range");
+    *updated = pu[static_cast<size_t>(index)] ? 1 : 0;
+    if (element_type) *element_type = m->impl->hip_program().parameter_type[static_cast<size_t>(index)];
+  });
+}
+
 int mononn_module_owns_temp(const mononn_module* m) { return (m && m->impl->owns_temp()) ? 1 : 0; }
 
 int mononn_module_launch_dims(const mononn_module* m, int* grid, int* block, int* smem, int* barriers) {

@@ -363,6 +363,10 @@ HipProgram generate_program(const graph::Program& prog, spec::GraphSpecification
     auto ip = prog.in_place.find(l);
     hp.liveout_parameter.push_back(ip == prog.in_place.end() ? -1 : static_cast<int>(ip->second->parameter_number));
   }
+  for (auto* p : prog.parameters) {
+    hp.parameter_type.push_back(hlo::dtype_name(p->shape.dtype));
+    hp.parameter_updated.push_back(prog.updated_parameters.count(static_cast<int>(p->parameter_number)) > 0);
+  }
   hp.temp_bytes = prog.temp_bytes;
 
   // node functions, de-duplicated by text

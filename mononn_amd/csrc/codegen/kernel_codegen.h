@@ -54,6 +54,8 @@ struct HipProgram {
   std::vector<std::string> global_decls;
   std::vector<int64_t> param_bytes, liveout_bytes;
   std::vector<int> liveout_parameter;   // entry parameter that a live-out updates in place (its own slot is not used), or -1
+  std::vector<bool> parameter_updated;  // the kernel writes to the parameter's buffer
+  std::vector<const char*> parameter_type;   // element type, as the text spells it
   int64_t temp_bytes = 0;
   std::vector<ConstantInfo> constants;
   std::vector<NodeReport> nodes;

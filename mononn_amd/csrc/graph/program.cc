@@ -737,8 +737,10 @@ struct Builder {
     for (auto& n : p.nodes) {
       if (n.kind != NodeKind::kOperator) continue;
       const Instr* ins = n.members[0];
-      if (ins->oper.kind == hlo::OperatorConfig::kKvAppend)
+      if (ins->oper.kind == hlo::OperatorConfig::kKvAppend) {
         for (auto* v : n.outputs) p.in_place[v] = ins->operands[v->tuple_index == 0 ? 2 : 3];
+        for (size_t i : {size_t(2), size_t(3)}) p.updated_parameters.insert(static_cast<int>(ins->operands[i]->parameter_number));
+      }
       if (ins->oper.kind == hlo::OperatorConfig::kPagedAttentionParts || ins->oper.kind == hlo::OperatorConfig::kMatvecW4Parts)
         p.temp_size[ins] = codegen::operator_part_bytes(ins, opt.grid, opt.waves);
     }

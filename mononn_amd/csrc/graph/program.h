@@ -153,6 +153,7 @@ struct Program {
   std::vector<const hlo::Instr*> live_outs;                        // storage roots, root-tuple order
   // results of an operator that updates an operand in place -> the entry parameter whose buffer holds them
   std::map<const hlo::Instr*, const hlo::Instr*> in_place;
+  std::set<int> updated_parameters;   // entry parameters that an operator writes to, whether a result of it is a live-out or not
   // bytes of temp values whose size the shape does not tell (the parts of a paged attention)
   std::map<const hlo::Instr*, int64_t> temp_size;
   std::map<const hlo::Instr*, int> producer;                       // storage root -> node id

@@ -37,15 +37,16 @@ class MonoNNFunction:
         self._param_bytes = info["parameters"]
         self._out_bytes = info["liveouts"]
         self._in_place = module.liveout_parameters()   # live-outs that are an input tensor, updated by the call
+        self._updated = {i: _TORCH_DTYPE[t] for i, t in module.updated_parameters().items()}   # all such inputs, returned or not
         assert len(self._out_bytes) == len(self.outputs), "one {dtype, dims} entry per live-out is required"
         self._temp = None if module.owns_temp else torch.zeros(max(info["temp"], 256), dtype=torch.uint8, device=self.device)
-        self._updates = any(p >= 0 for p in self._in_place)
         self._args_type = ctypes.c_void_p * (len(self._param_bytes) + len(self._out_bytes) + 1)
         self._temp_ptr = 0 if self._temp is None else self._temp.data_ptr()
         self._results = []   # extents, strides, type, parameter that is updated or -1
         for o, p, nbytes in zip(self.outputs, self._in_place, self._out_bytes):
             like = torch.empty(tuple(o["dims"]), dtype=_TORCH_DTYPE[o["dtype"]], device="meta")
             assert like.nbytes == nbytes
+            assert p < 0 or like.dtype == self._updated[p], "a live-out that is an updated input has its declared type"
             self._results.append((tuple(like.shape), like.stride(), like.dtype, p))
         self.handle = id(self)
         _REGISTRY[self.handle] = self
@@ -56,7 +57,7 @@ class MonoNNFunction:
     def _input(self, i: int, t: torch.Tensor) -> torch.Tensor:
         """Parameter i from a tensor that is not simply the parameter's bytes: made contiguous, or refused."""
         assert t.is_cuda and t.device == self.device, "inputs must live on the module's GPU"
-        assert t.is_contiguous() or i not in self._in_place, "an input that the call updates in place must be contiguous"
+        assert t.is_contiguous() or i not in self._updated, "an input that the call updates in place must be contiguous"
         t = t.contiguous()
         nbytes = self._param_bytes[i]
         assert t.numel() * t.element_size() == nbytes, f"parameter needs {nbytes} bytes, got {t.numel() * t.element_size()}"
@@ -74,14 +75,15 @@ class MonoNNFunction:
                 held[i] = t = self._input(i, t)
                 ptr = t.data_ptr()
             ptrs.append(ptr)
+        for i, dtype in self._updated.items():
+            assert held[i].dtype == dtype, "an input that the call updates in place must have the declared type"
+            assert ptrs.count(ptrs[i]) == 1, "an input that the call updates in place must not be passed twice"
         outs = []
         for dims, strides, dtype, param in self._results:
             if param >= 0:
                 t = held[param]
-                assert t.dtype == dtype, "an input that the call updates in place must have the declared type"
                 if t.shape != dims:
                     t = t.view(dims)
-                assert ptrs.count(ptrs[param]) == 1, "an input that the call updates in place must not be passed twice"
                 ptrs.append(None)
             else:
                 t = torch.empty_strided(dims, strides, dtype=dtype, device=device)   # a little cheaper than torch.empty
@@ -100,7 +102,7 @@ class MonoNNFunction:
 def _forward(handle: int, inputs: Sequence[torch.Tensor]) -> List[torch.Tensor]:
     fn = _REGISTRY[handle]
     # the operator is declared to change no input and to return new tensors
-    assert not fn._updates, "a module that updates inputs in place is called through MonoNNFunction itself"
+    assert not fn._updated, "a module that updates inputs in place is called through MonoNNFunction itself"
     return fn(*inputs)
 
 

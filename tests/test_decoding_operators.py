@@ -163,6 +163,37 @@ def test_liveout_parameter_checks_its_arguments():
     assert value.value == 3
 
 
+def append_and_attend(returned):
+    """A module that appends to its caches (parameters 2 and 3) and attends over them; `returned` of out, kc, vc are its results."""
+    def build(e):
+        cache = (9, 16, 2, 64)
+        a = [e.parameter("f16", (5, 2, 64), "k"), e.parameter("f16", (5, 2, 64), "v"), e.parameter("f16", cache, "k_cache"), e.parameter("f16", cache, "v_cache"),
+             e.parameter("s32", (2, 4), "page_table"), e.parameter("s32", (3,), "query_start"), e.parameter("s32", (2,), "context_len")]
+        kc, vc = e.kv_append(*a)
+        out = e.paged_attention(e.parameter("f16", (5, 4, 64), "q"), kc, vc, *a[4:], 0.125)
+        return [{"out": out, "kc": kc, "vc": vc}[r] for r in returned]
+    return dc.module(build)
+
+
+@pytest.mark.parametrize("returned, liveouts", [(["out"], [-1]), (["out", "vc"], [-1, 3]), (["kc", "out"], [2, -1]), (["out", "kc", "vc"], [-1, 2, 3])])
+def test_updated_parameters_do_not_depend_on_what_is_returned(returned, liveouts):
+    m = MonoNNModule.compile(append_and_attend(returned)[0], build=False)
+    assert m.liveout_parameters() == liveouts and m.updated_parameters() == {2: "f16", 3: "f16"}
+
+
+def test_parameter_updated_checks_its_arguments():
+    m = MonoNNModule.compile(append_and_attend(["out"])[0], build=False)
+    value, name = ctypes.c_int(7), ctypes.c_char_p()
+    ask = binding._lib.mononn_module_parameter_updated
+    assert ask(m._h, 3, ctypes.byref(value), None) == 0 and value.value == 1
+    assert ask(m._h, 4, ctypes.byref(value), ctypes.byref(name)) == 0 and value.value == 0 and name.value == b"s32"
+    value.value = 7
+    for handle, index, out in ((m._h, 8, ctypes.byref(value)), (m._h, -1, ctypes.byref(value)), (m._h, 0, None), (None, 0, ctypes.byref(value))):
+        assert ask(handle, index, out, None) == 1   # invalid argument
+    assert value.value == 7
+    assert MonoNNModule.compile(dc.rope_module(3, 5, 80, 20, "f16")[0], build=False).updated_parameters() == {}
+
+
 ATT = ["f16[4,8,64]{2,1,0}", "f16[9,16,2,64]{3,2,1,0}", "f16[9,16,2,64]{3,2,1,0}", "s32[3,5]{1,0}", "s32[4]{0}", "s32[3]{0}"]
 
 

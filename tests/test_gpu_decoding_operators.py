@@ -531,6 +531,28 @@ def test_an_updated_input_is_passed_once_and_not_through_the_pure_operator(gpu_d
     assert new_k.shape == (3, 16, 2, 64) and new_k.data_ptr() == kc.data_ptr()
 
 
+@pytest.mark.parametrize("returned", [["out"], ["out", "vc"], ["kc", "out"]])
+def test_a_cache_that_is_not_returned_is_guarded_too(gpu_device, returned):
+    import torch
+    from mononn_amd.torch_op import forward
+    from test_decoding_operators import append_and_attend
+    fn = _function(*append_and_attend(returned), checked=True)
+    k = torch.ones((5, 2, 64), dtype=torch.float16, device="cuda")
+    kc, vc = (torch.zeros((9, 16, 2, 64), dtype=torch.float16, device="cuda") for _ in range(2))
+    strided = torch.zeros((9, 16, 64, 2), dtype=torch.float16, device="cuda").transpose(2, 3)
+    meta = [torch.tensor(a, dtype=torch.int32, device="cuda") for a in ([[0, 1, 2, 3], [4, 5, 6, 7]], [0, 2, 5], [20, 3])]
+    q = torch.ones((5, 4, 64), dtype=torch.float16, device="cuda")
+    for caches, words in (((strided, vc), "contiguous"), ((kc, strided), "contiguous"), ((kc.view(torch.bfloat16), vc), "declared type"), ((kc, vc.view(torch.bfloat16)), "declared type"), ((kc, kc), "twice")):
+        with pytest.raises(AssertionError, match=words):
+            fn(k, k, *caches, *meta, q)
+    with pytest.raises(AssertionError, match="in place"):
+        forward(fn, k, k, kc, vc, *meta, q)
+    torch.cuda.synchronize()
+    assert not kc.any() and not vc.any() and not strided.any()
+    fn(k, k, kc, vc, *meta, q)
+    assert kc.sum() == vc.sum() == 5 * 128 and kc[1, 2].all() and vc[4, :3].all()
+
+
 def test_two_functions_in_two_graphs(gpu_device):
     """Parts of split sequences lie in each function's own memory: graphs of two, replayed in turn, keep their results."""
     import torch
