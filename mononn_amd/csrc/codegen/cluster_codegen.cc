@@ -110,6 +110,7 @@ NodeFunction finish(const std::string& body, PointerTable& ptrs, const std::vect
   f.pointers = ptrs.entries;
   f.num_units = units;
   f.smem_bytes = smem;
+  f.lds_at_once = smem > 0;
   f.globals = globals;
   f.text = pre + "__device__ __forceinline__ void @NAME@(" + signature(ptrs.entries) + ") {\n" + align_prologue(ptrs.entries) + body + "}\n";
   return f;
@@ -2022,6 +2023,7 @@ NodeFunction gen_gemm(const Program& prog, const std::vector<const Instr*>& memb
   std::vector<std::string> globals = epi.globals;
   for (auto& gl : pro.globals) globals.push_back(gl);
   NodeFunction f = finish(fb.text(), ptrs, globals, units, smem, pro.struct_text + rows_struct + epi.struct_text + conv_struct);
+  f.lds_at_once = pro.smem > 0 && !lds_fold;   // the tiles themselves begin with a barrier
   f.write_maps = epi.writes;
   if (preload) {
     const std::string tail = ", char* smem) {";

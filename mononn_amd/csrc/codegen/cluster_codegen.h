@@ -80,6 +80,7 @@ struct NodeFunction {
   std::vector<PointerTable::Entry> pointers;   // call arguments after `unit`, before `smem`
   int64_t num_units = 0;                       // independent work units (one workgroup each)
   int smem_bytes = 0;
+  bool lds_at_once = false;                    // stores to the LDS before a workgroup barrier of its own
   std::vector<std::string> globals;            // device-global definitions the function needs
   // Optional companion `@NAME@_pre(unit, <pointers>, @NAME@_preb&)`: requests operands that do not depend on
   // the previous stage.  When present, `text` defines the register block type `@NAME@_preb` and takes a trailing

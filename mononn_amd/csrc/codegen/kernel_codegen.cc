@@ -380,6 +380,8 @@ HipProgram generate_program(const graph::Program& prog, spec::GraphSpecification
     std::vector<Operand> args;
     int64_t units;
     int parts = 0;   // regional synchronisation: XCDs that take part in the node (unit u belongs to XCD u % 8); 0 = units dealt round-robin
+    bool lds = false;   // the function uses the LDS
+    bool lds_at_once = false, own_reads = false;   // ... stores there before a barrier of its own; its unit before may still be read for
   };
   std::map<std::string, int> fn_ids;
   std::set<int> preload_fns;   // functions with a companion that requests constant operands ahead of the barrier wait
@@ -540,6 +542,11 @@ HipProgram generate_program(const graph::Program& prog, spec::GraphSpecification
     c.parts = partition[ni].on() ? partition[ni].parts : 0;
     c.fn = fn;
     c.units = f.num_units;
+    c.lds = f.smem_bytes > 0;
+    c.lds_at_once = f.lds_at_once;
+    // a row program in front of a GEMM exchanges its sums where the tile before has added up its k slices (a folded
+    // LayerNorm has room of its own)
+    c.own_reads = n.kind == NodeKind::kGemm && !n.ln_fold.on();
     c.fn_id = fn_ids.at(fn);
     for (auto& e : f.pointers) c.args.push_back(make_operand(prog, e.root, e.is_output, e.dtype, const_symbol, hp.param_bytes.size(), hp.liveout_bytes.size()));
     if (!fn_arg_types.count(c.fn_id))
@@ -661,6 +668,10 @@ HipProgram generate_program(const graph::Program& prog, spec::GraphSpecification
     bool new_stage;
     int rot;   // unit u of the stage runs on workgroup (u + rot) % grid
     bool regional;   // the barrier in front of the stage is one of the regional tier
+    // A workgroup may come to a unit of this call, which stores to the LDS at once, from another unit of the stage that other
+    // waves of it still read the LDS for: functions mind their own units only, so a barrier goes in between.  Only stages of
+    // more units than workgroups have such calls.
+    bool lds_shared;
   };
   std::vector<Flat> flat;
   // A workgroup that had a unit in the previous stage reaches the barrier later than an idle one and has asked for
@@ -679,11 +690,13 @@ HipProgram generate_program(const graph::Program& prog, spec::GraphSpecification
     any_rot = any_rot || rot != 0;
     hp.stage_nodes.emplace_back();
     int64_t first = 0;
-    bool ns = true;
+    bool ns = true, lds_used = false;
     for (auto& c : st.second) {
       hp.stage_nodes.back().push_back(c.node->name);
       if (c.parts) first = (first + 7) / 8 * 8;
-      flat.push_back({&c, static_cast<int>(first), static_cast<int>(total), ns, static_cast<int>(rot), regional_before[hp.stage_nodes.size() - 1]});
+      flat.push_back({&c, static_cast<int>(first), static_cast<int>(total), ns, static_cast<int>(rot), regional_before[hp.stage_nodes.size() - 1],
+                      total > hp.grid && c.lds_at_once && (lds_used || (c.own_reads && c.units > hp.grid))});
+      lds_used = lds_used || c.lds;
       ns = false;
       first += c.units;
     }
@@ -715,7 +728,10 @@ HipProgram generate_program(const graph::Program& prog, spec::GraphSpecification
   if (any_regional) src << "  barrier.init_regional(mononn_regional_flags);\n";
   bool any_parts = false;
   for (auto& f : flat) any_parts = any_parts || f.call->parts > 0;
+  bool any_lds_shared = false;
+  for (auto& f : flat) any_lds_shared = any_lds_shared || f.lds_shared;
   src << "  int stage = -1;\n";
+  if (any_lds_shared) src << "  bool worked = false;   // the workgroup has had a unit of this stage\n";
   const bool lazy = !preload_fns.empty();
   if (lazy) {
     // The wait half of a barrier is put off until the workgroup's first unit of the new stage, behind the
@@ -729,6 +745,7 @@ HipProgram generate_program(const graph::Program& prog, spec::GraphSpecification
   src << "    int fn = 0, units = 0, first = 0, total = 0" << (any_rot ? ", rot = 0" : "") << ";\n    bool new_stage = false;\n";
   if (any_regional) src << "    bool regional = false;   // the barrier in front of the stage orders the workgroups of one XCD only\n";
   if (any_parts) src << "    int parts = 0;   // > 0: unit u belongs to XCD u % 8, and only this many XCDs take part\n";
+  if (any_lds_shared) src << "    bool lds_shared = false;   // waves may still read the LDS for another unit of the stage\n";
   src << "    char*";
   for (size_t i = 0; i < max_ptrs; ++i) src << (i ? ", *" : " ") << "p" << i << " = nullptr";
   src << ";\n";
@@ -740,6 +757,7 @@ HipProgram generate_program(const graph::Program& prog, spec::GraphSpecification
     if (f.rot) src << " rot = " << f.rot << ";";
     if (f.regional && f.new_stage) src << " regional = true;";
     if (f.call->parts) src << " parts = " << f.call->parts << ";";
+    if (f.lds_shared) src << " lds_shared = true;";
     for (size_t a = 0; a < f.call->args.size(); ++a) src << " p" << a << " = " << base_expr(f.call->args[a]) << ";";
     src << " break;   // " << f.call->node->name.substr(0, 50) << "\n";
   }
@@ -748,6 +766,7 @@ HipProgram generate_program(const graph::Program& prog, spec::GraphSpecification
   // a workgroup that has no unit in a stage leaves both at zero
   const std::string clk = "mononn_stage_clock[(stage * " + std::to_string(hp.grid) + " + blockIdx.x) * 2";
   src << "    if (new_stage) {\n";
+  if (any_lds_shared) src << "      worked = false;\n";
   if (!lazy) {
     if (hp.profiled) {
       src << "      if (stage >= 0) {\n        __syncthreads();\n";
@@ -779,6 +798,7 @@ HipProgram generate_program(const graph::Program& prog, spec::GraphSpecification
   src << "      const int unit = u - first;\n";
   src << "      if (unit < 0 || unit >= units) continue;\n";
   if (any_parts) src << "      if (parts > 0 && (unit & 7) >= parts) continue;   // an XCD without a share of this node\n";
+  if (any_lds_shared) src << "      if (lds_shared && worked) __syncthreads();\n      worked = true;\n";
   // One dispatch switch; in the lazy form every case first requests what it can, then waits if a barrier is pending
   // (the wait is spelled out per case so that the requested registers flow straight into the function that uses
   // them instead of meeting at a join of all cases).

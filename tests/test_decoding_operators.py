@@ -317,6 +317,48 @@ def test_parts_have_their_own_memory():
         assert m.buffer_info()["temp"] >= 2 * part
 
 
+def between_units(source):
+    """The statements of the kernel's unit loop in front of its dispatch, and the calls that have LDS to wait for."""
+    kernel = source[source.index('extern "C"'):]
+    loop = kernel[kernel.index("const int unit = u - first;"):]
+    return loop[:loop.index("switch (fn)")], [line for line in kernel.splitlines() if "lds_shared = true" in line]
+
+
+def test_units_of_a_stage_do_not_meet_in_the_lds():
+    # 224 units of a 4-bit product and 64 of a LayerNorm on 256 workgroups: 32 of them go from the one, whose waves end with
+    # reads of the LDS, to the other, which begins with stores there
+    def build(e):
+        y = e.matvec_w4(e.parameter("f16", (1, 128), "x"), e.parameter("u8", (14336, 64), "w"), e.parameter("f16", (14336, 1), "s"))
+        h, g, b = e.parameter("f16", (64, 768), "h"), e.parameter("f16", (768,), "g"), e.parameter("f16", (768,), "b")
+        return y, models._layer_norm(e, e.module, h, g, b, 1e-5)
+    m = MonoNNModule.compile(dc.module(build)[0], build=False)
+    assert "stages=1 nodes=2" in m.summary()
+    loop, calls = between_units(m.get_source("main.hip"))
+    assert "if (lds_shared && worked) __syncthreads();" in loop and "worked = true;" in loop
+    assert len(calls) == 1 and "units = 64; first = 224; total = 288;" in calls[0]
+
+
+def test_a_gemm_behind_its_row_program_waits_for_its_own_last_unit():
+    # k split over waves: a unit ends with reads of the sums in the LDS, the next one begins with the row program's exchange there
+    def build(e):
+        h, g, b = e.parameter("f16", (1024, 256), "h"), e.parameter("f16", (256,), "g"), e.parameter("f16", (256,), "b")
+        return e.gemm(models._layer_norm(e, e.module, h, g, b, 1e-5), e.parameter("f16", (256, 1024), "w"), 1, 0)
+    text = dc.module(build)[0]
+    spec = json.loads(MonoNNModule.compile(text, build=False).get_tuning_spec())
+    spec["mononn_hip"]["gemm_prologue_fusion"] = True
+    for nodes in ("gemm_spec_list", "cluster_reduce_spec", "cluster_elewise_spec"):
+        spec[nodes] = {}
+    spec = json.loads(MonoNNModule.compile(text, json.dumps(spec), build=False).get_tuning_spec())
+    (gemm,) = spec["gemm_spec_list"].values()
+    for waves_k, wait in ((4, True), (1, False)):
+        gemm["cutlass_config"].update(threadblockshape={"m": 32, "n": 32, "k": 32}, warpshape={"m": 32 if waves_k == 4 else 16, "n": 32 if waves_k == 4 else 16, "k": 256 // waves_k},
+                                      wave_arrangement={"m": 1 if waves_k == 4 else 2, "n": 1 if waves_k == 4 else 2, "k": waves_k})
+        m = MonoNNModule.compile(text, json.dumps(spec))
+        assert "+row-prologue" in m.summary() and m.launch_dims()["grid"] == 256
+        loop, calls = between_units(m.get_source("main.hip"))
+        assert len(calls) == (1 if wait else 0) and ("__syncthreads" in loop) == wait
+
+
 # ---- every variant builds -----------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("text", [
     dc.rope_module(3, 5, 80, 20, "bf16", True)[0], dc.rope_module(7, 3, 10, 6, "f32")[0], dc.append_module(5, 2, 64, 9, 3, 2, 4, "f32")[0],
