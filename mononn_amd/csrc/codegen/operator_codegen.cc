@@ -54,9 +54,10 @@ struct MatvecPlan {
   int64_t M, N, K, group;
   int64_t wk = 1, sk = 1, p = 1;
   int64_t row_blocks() const { return std::min<int64_t>((M + 15) / 16, 4); }
-  int64_t x_rows() const { return std::min(M, 16 * row_blocks()); }
   int64_t blocks_per_workgroup() const { return ((K + 128 * p - 1) / (128 * p) + sk - 1) / sk; }
-  int64_t x_bytes() const { return blocks_per_workgroup() * p * 256 * (x_rows() | 1); }   // an odd pitch
+  int64_t x_bytes() const { return hlo::matvec_w4_x_bytes(M, blocks_per_workgroup() * p); }
+  int64_t lds_bytes(int64_t waves) const { return x_bytes() + (wk > 1 ? waves * row_blocks() * 1024 : 0); }   // and the shares of a tile's waves
+  bool fits(int64_t waves) const { return x_bytes() <= hlo::kMatvecW4XBytes && lds_bytes(waves) <= 160 * 1024; }
 };
 // The plan whose busiest workgroup reads least: weights, its slice of x (16 rows of x on 4096 x 14336 weights: 13.4 us with
 // slices of 57 KB of x, 17 with the 115 KB that the weights alone would choose) and its share of the parts (7 rows on
@@ -72,14 +73,16 @@ MatvecPlan plan_matvec(const Instr* call, int64_t grid, int64_t waves) {
   const int64_t tiles = (best.N + 15) / 16, passes = (best.M + 16 * best.row_blocks() - 1) / (16 * best.row_blocks());
   const int64_t products = best.M > 4 && best.group >= 128 ? best.row_blocks() : 1;   // a pass of more rows reads more of the LDS for the same weights
   int64_t least = -1;
+  // 64 slices at most, unless x is so wide that it takes more: then as few as hold it
+  const int64_t columns_at_once = hlo::kMatvecW4XBytes / hlo::matvec_w4_x_bytes(best.M, 1), fewest = split ? ((best.K + 127) / 128 + columns_at_once - 1) / columns_at_once : 1;
   for (int64_t p : {4, 2, 1}) {
     if (p > 1 && best.M > 4 && (best.group >= 128 || p > 2)) continue;   // MatvecW4::kWhole, and the scales of kSwap
-    for (int64_t sk = 1; sk <= (split ? 64 : 1); ++sk)
+    for (int64_t sk = fewest > 64 ? fewest : 1; sk <= (split ? std::max<int64_t>(fewest, 64) : 1); ++sk)
       for (int64_t wk = 1; wk <= waves; wk *= 2) {
         if (waves % wk != 0) break;
         MatvecPlan c = best;
         c.p = p, c.sk = sk, c.wk = wk;
-        if (c.x_bytes() > 128 * 1024) continue;
+        if (!c.fits(waves)) continue;
         const int64_t at_once = waves / wk, units = (tiles + at_once - 1) / at_once * sk * passes;
         // 16-byte loads of the busiest workgroup: weights and x, and its share of the parts, written and read
         const int64_t parts = split ? sk * best.M * best.N * 8 / 16 / grid : 0;
@@ -208,7 +211,7 @@ NodeFunction generate_operator(const graph::Program& prog, const graph::Node& no
       const int64_t units = ((p.N + 15) / 16 + at_once - 1) / at_once * p.sk * ((p.M + 16 * row_blocks - 1) / (16 * row_blocks));
       check_units(std::min<int64_t>(units, grid));   // a workgroup's units are one unit of the stage: x may stay in its LDS
       body << "Matvec::units<" << f.num_units << ">(unit, " << x << ", " << w << ", " << s << ", " << z << ", " << (parts_stage ? "nullptr, " + out : out + ", nullptr") << ", smem);";
-      f.smem_bytes = static_cast<int>((p.wk > 1 ? ls.waves() * row_blocks * 1024 : 0) + p.x_bytes());
+      f.smem_bytes = static_cast<int>(p.lds_bytes(ls.waves()));
       body << " static_assert(Matvec::lds_bytes() == " << f.smem_bytes << " && Matvec::num_units() == " << units << ", \"launch\");";
       break;
     }

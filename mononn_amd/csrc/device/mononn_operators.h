@@ -1572,7 +1572,7 @@ struct MatvecW4 {
     const long i = (long)unit * MONONN_BLOCK_SIZE + thread_id();
     if (i >= (long)M * N) return;
     float v = parts[i];
-#pragma unroll
+#pragma unroll 64
     for (int s = 1; s < SK; ++s) v += parts[(long)s * M * N + i];
     const T r[1] = {(T)v};
     store_run<COHERENT, T, 1>(y + i, r);

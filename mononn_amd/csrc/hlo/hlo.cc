@@ -1268,7 +1268,11 @@ void split_operators(Module* mod) {
   for (size_t i = 0; i < comp->instrs.size(); ++i) comp->instrs[i]->index_in_comp = static_cast<int>(i);
 }
 
-bool matvec_w4_in_parts(int64_t rows, int64_t columns) { return (columns + 127) / 128 * 256 * std::min<int64_t>(rows, 64) > kMatvecW4RowBytes; }
+int64_t matvec_w4_x_bytes(int64_t rows, int64_t blocks) { return blocks * 256 * (std::min<int64_t>(rows, 64) | 1); }
+bool matvec_w4_in_parts(int64_t rows, int64_t columns) {
+  const int64_t blocks = (columns + 127) / 128, values = blocks * 256 * std::min<int64_t>(rows, 64);
+  return values > 96 * 1024 || matvec_w4_x_bytes(rows, blocks) > kMatvecW4XBytes;   // two rows: the pitch of three decides
+}
 
 std::unique_ptr<Module> parse_module(const std::string& text) {
   auto mod = std::make_unique<Module>();

@@ -83,8 +83,10 @@ struct OperatorConfig {
   int64_t window = 0;        // paged_attention: keys a query sees, itself included; 0 = all before it
 };
 
-// LDS that a workgroup of matvec_w4 gives to x: its rows for all columns, or a slice of the columns
-constexpr int64_t kMatvecW4RowBytes = 96 * 1024;
+// matvec_w4 keeps x in the LDS of a workgroup: its rows (64 at a time, in an odd pitch) for all columns, or a slice of the
+// columns.  Bytes of that for `blocks` of 128 columns, the most a workgroup gives to it, and whether a call is sliced.
+constexpr int64_t kMatvecW4XBytes = 128 * 1024;
+int64_t matvec_w4_x_bytes(int64_t rows, int64_t blocks);
 bool matvec_w4_in_parts(int64_t rows, int64_t columns);
 
 struct Instr {

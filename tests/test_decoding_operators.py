@@ -258,6 +258,21 @@ def test_matvec_w4_refusals(change, status, words):
     refused(params(*shapes) + call("f16[2,48]{1,0}", "matvec_w4", 4, extra="ROOT "), status, words)
 
 
+# rows, columns, threads around the widths at which x no longer fits a workgroup's LDS: whole and in slices
+W4_WIDE = [(1, 49152, 512), (1, 49280, 512), (2, 21760, 512), (2, 21888, 512), (2, 22016, 256), (2, 24576, 512), (2, 24704, 512), (3, 16384, 512), (3, 16512, 512),
+           (64, 768, 512), (64, 896, 512), (64, 65536, 512), (65, 65536, 256), (64, 768, 1024), (128, 768, 1024), (128, 11008, 1024)]
+
+
+@pytest.mark.parametrize("M, K, block", W4_WIDE)
+def test_matvec_w4_has_a_plan_for_every_width(M, K, block):
+    for dtype, group, zeros in (("f16", 32, False), ("bf16", 128, True)):
+        text, _ = dc.w4_module(M, 40, K, group, dtype, zeros)
+        spec = json.loads(MonoNNModule.compile(text, build=False).get_tuning_spec())
+        spec["cuda_context"]["cuda_runtime_context"]["block_dim"]["x"] = block
+        m = MonoNNModule.compile(text, json.dumps(spec))
+        assert 0 < m.launch_dims()["smem"] <= 160 * 1024 and len(m.get_code_object()) > 0
+
+
 def test_extents_beyond_32_bits_are_refused():
     big = ["f16[70000,256]{1,0}", "u8[40000,128]{1,0}", "f16[40000,2]{1,0}"]
     refused(params(*big) + call("f16[70000,40000]{1,0}", "matvec_w4", 3, extra="ROOT "), "UNSUPPORTED", "too many rows")
@@ -429,6 +444,11 @@ def test_bounds_attention(monkeypatch, tmp_path, T, H, HKV, D, B, W, page, windo
                                                          (16, 40, 4096, 64, "f16", True), (70, 33, 1056, 32, "bf16", False)])   # x in slices
 def test_bounds_w4(monkeypatch, tmp_path, M, N, K, group, dtype, zeros):
     assert check(monkeypatch, tmp_path, dc.w4_module(M, N, K, group, dtype, zeros)[0], grid=8) == (True, "ok")
+
+
+@pytest.mark.parametrize("M, K, group, block", [(2, 21888, 32, 256), (64, 768, 32, 1024), (65, 65536, 128, 256)])
+def test_bounds_w4_of_wide_x(monkeypatch, tmp_path, M, K, group, block):
+    assert check(monkeypatch, tmp_path, dc.w4_module(M, 20, K, group, "f16", True)[0], grid=8, block=block) == (True, "ok")
 
 
 def test_bounds_harness_sees_the_operators(monkeypatch, tmp_path):

@@ -335,6 +335,21 @@ def test_matvec_w4(gpu_device, M, N, K, group, dtype, zeros, block):
     within(dc.values(got, dtype), want, dc.w4_bound(want, mags, K, group, dtype, zeros))
 
 
+@pytest.mark.parametrize("M, K, group, dtype, zeros, block", [(2, 21760, 32, "f16", False, 512), (2, 21888, 32, "bf16", True, 512), (2, 24576, 128, "f16", True, 256), (3, 16512, 32, "f16", False, 512),
+                                                              (64, 896, 32, "bf16", True, 512), (65, 65536, 128, "f16", False, 512), (64, 768, 32, "f16", True, 1024), (128, 11008, 64, "bf16", False, 1024)])
+def test_matvec_w4_of_wide_x(gpu_device, M, K, group, dtype, zeros, block):
+    rng = np.random.default_rng(48)
+    N = 50
+    text, outs = dc.w4_module(M, N, K, group, dtype, zeros)
+    x, w = dc.bits(rng.normal(size=(M, K)), dtype), rng.integers(0, 256, (N, K // 2), dtype=np.uint8)
+    s = dc.bits(rng.uniform(-0.02, 0.02, (N, K // group)), dtype)
+    z = rng.integers(0, 16, (N, K // group), dtype=np.uint8) if zeros else None
+    mags = {}
+    want = decoding.matvec_w4(dc.values(x, dtype), w, dc.values(s, dtype), z, mags)
+    (got,) = run(text, outs, [x, w, s] + ([z] if zeros else []), block)
+    within(dc.values(got, dtype), want, dc.w4_bound(want, mags, K, group, dtype, zeros))
+
+
 def test_matvec_w4_values_one_by_one(gpu_device):
     # unit rows of x pick single columns: every nibble value at every place of a byte, exactly
     K, N = 128, 16
