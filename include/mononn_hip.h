@@ -127,11 +127,11 @@ int mononn_module_load(mononn_module* m, int device);
 int mononn_launch(mononn_module* m, void* const* device_ptrs, size_t n_ptrs, void* stream);
 
 /* mononn_launch for callers that cannot allocate device memory (code under HIP graph capture, tight serving loops,
- * harnesses that forbid hipMalloc): the temp arena is a fixed array of mononn_static_temp_bytes() bytes (64 MiB) in
+ * harnesses that forbid hipMalloc): the temp arena is a fixed array of mononn_static_temp_bytes() bytes (80 MiB) in
  * the library's own device image instead of a buffer of the caller, and the call allocates nothing.  device_ptrs:
  * entry parameters in parameter order, then live-out buffers -- no temp slot.  A module whose temp arena is larger
  * is refused with MONONN_RESOURCE_EXHAUSTED.  Each GPU holds one such array from the first mononn_module_load on it
- * until the process ends (64 MiB of device memory per GPU for every process that loads a module, whether it uses
+ * until the process ends (80 MiB of device memory per GPU for every process that loads a module, whether it uses
  * this entry point or not); every call on a GPU, from any module, shares it, so calls that overlap on one GPU race.
  * Nothing in the arena has to start at zero: every temp address is written before it is read in the same launch.
  * No counterpart in the reference. */

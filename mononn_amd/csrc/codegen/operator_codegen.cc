@@ -106,8 +106,9 @@ int64_t operator_part_bytes(const Instr* parts, int grid, int waves) {
     return p.sk * p.M * p.N * 4;
   }
   const int64_t group = q[1] / parts->operands[1]->shape.dims[2];
-  const int64_t D = q[2], narrow = D / 16 * 256 + 32, wide = waves * ((D + 31) / 32 * 1024 + 64);   // floats
-  return 2 * int64_t(grid) * (q[0] * group <= 16 ? narrow : wide) * 4;   // at most 16 query rows in all: no wide item
+  const int64_t D = q[2], rows = q[0] * group, blocks = std::min<int64_t>((rows + 31) / 32, waves);   // mirrors PagedAttention::kPart
+  const int64_t narrow = D / 16 * 256 + 32, wide = blocks * ((D + 31) / 32 * 1024 + 64);   // floats
+  return 2 * int64_t(grid) * (rows <= 16 ? narrow : wide) * 4;   // at most 16 query rows in all: no wide item
 }
 
 NodeFunction generate_operator(const graph::Program& prog, const graph::Node& node, const LaunchShape& ls, int grid) {

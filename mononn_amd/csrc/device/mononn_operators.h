@@ -293,7 +293,9 @@ struct PagedAttention {
   static constexpr bool kAllNarrow = TOKENS * G <= 16;      // no sequence can have more rows
   static constexpr int kPartWave = DT * 1024 + 64;          // floats: output tiles as they lie in the registers, maxima, sums
   static constexpr int kPartNarrow = kTiles * 256 + 32;
-  static constexpr int kPart = kAllNarrow ? kPartNarrow : NW * kPartWave;   // floats of one partial result; two per workgroup
+  static constexpr long kMostRows = (long)TOKENS * G;       // no item has more
+  static constexpr int kBlocks = kMostRows < 32 * NW ? (int)((kMostRows + 31) / 32) : NW;   // blocks of 32 rows of an item, at most
+  static constexpr int kPart = kAllNarrow ? kPartNarrow : kBlocks * kPartWave;   // floats of one partial result; two per workgroup
   static constexpr int kMergeBytes = NN * (kTiles * 1024 + 128);
   static constexpr int lds_bytes() {
     int n = kAllNarrow ? 0 : kWideKeys * (2 * KP + kValueBuffers * VP);

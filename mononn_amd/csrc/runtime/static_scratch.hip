@@ -8,7 +8,9 @@
 
 namespace {
 
-constexpr size_t kScratchBytes = size_t(64) << 20;   // BERT-base b1 s128 needs 48 MB with write-once temp addresses
+// BERT-base b1 s128 needs 48 MB with write-once temp addresses, attention over prompts on heads of 128 elements 65 MiB for
+// the parts of its items
+constexpr size_t kScratchBytes = size_t(80) << 20;
 static __device__ __align__(256) unsigned char scratch[kScratchBytes];
 
 constexpr int kMaxDevices = 64;

@@ -374,6 +374,19 @@ def test_a_gemm_behind_its_row_program_waits_for_its_own_last_unit():
         assert len(calls) == (1 if wait else 0) and ("__syncthreads" in loop) == wait
 
 
+@pytest.mark.parametrize("T, H, HKV, D, block", [(5, 32, 8, 128, None), (32, 32, 8, 128, None), (4000, 32, 8, 128, None), (4, 8, 1, 256, None), (90, 4, 4, 64, 1024)])
+def test_parts_of_attention_fit_the_static_arena(T, H, HKV, D, block):
+    text = dc.attention_module(T, H, HKV, D, 90, 16, 4, 300, "bf16", 0.1)[0]
+    spec = json.loads(MonoNNModule.compile(text, build=False).get_tuning_spec())
+    if block:
+        spec["cuda_context"]["cuda_runtime_context"]["block_dim"]["x"] = block
+    m = MonoNNModule.compile(text, json.dumps(spec), build=False)
+    waves, rows = (block or 512) // 64, T * H // HKV
+    part = min(waves, -(-rows // 32)) * (D // 32 * 1024 + 64) * 4   # per block of 32 rows: its output, maxima and sums
+    assert 2 * 256 * part <= m.buffer_info()["temp"] <= binding._lib.mononn_static_temp_bytes()
+    assert m.buffer_info()["temp"] < 2 * 256 * part + 4096
+
+
 # ---- every variant builds -----------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("text", [
     dc.rope_module(3, 5, 80, 20, "bf16", True)[0], dc.rope_module(7, 3, 10, 6, "f32")[0], dc.append_module(5, 2, 64, 9, 3, 2, 4, "f32")[0],

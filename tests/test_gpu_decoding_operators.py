@@ -639,6 +639,28 @@ def test_launch_with_the_static_arena_and_null_slots(gpu_device):
     a.close()
 
 
+@pytest.mark.parametrize("new, ctx, H, HKV, D", [([1] * 32, [40 + 61 * i for i in range(32)], 32, 8, 128), ([300, 1, 40], [300, 999, 70], 32, 8, 128), ([1] * 90, [200] * 90, 32, 8, 128), ([2, 2], [500, 60], 8, 1, 256)])
+def test_attention_launches_with_the_static_arena(gpu_device, new, ctx, H, HKV, D):
+    import torch
+    from mononn_amd import binding
+    rng = np.random.default_rng(49)
+    table, qs, cl, pages = dc.paged_batch(rng, new, ctx, 16)
+    text, outs = dc.attention_module(sum(new), H, HKV, D, pages, 16, len(new), table.shape[1], "bf16", D ** -0.5)
+    args = [torch.from_numpy(rng.normal(size=s).astype(np.float32)).cuda().bfloat16() for s in ((sum(new), H, D), (pages, 16, HKV, D), (pages, 16, HKV, D))]
+    args += [torch.from_numpy(a).cuda() for a in (table, qs, cl)]
+    m = MonoNNModule.compile(text)
+    m.load(0)
+    assert m.buffer_info()["temp"] <= binding._lib.mononn_static_temp_bytes()
+    from mononn_amd.torch_op import MonoNNFunction
+    (want,) = MonoNNFunction(m, outs, checked=True)(*args)
+    out = torch.zeros_like(want)
+    stream = torch.cuda.current_stream().cuda_stream
+    m.launch_static_temp([t.data_ptr() for t in args] + [out.data_ptr()], stream)
+    m.synchronize(stream)
+    assert torch.equal(out, want) and out.any()
+    m.close()
+
+
 def test_operands_and_results_in_other_layouts(gpu_device):
     # any order of dimensions in memory at the module's boundary; the operators themselves work on row-major values
     rng = np.random.default_rng(45)
