@@ -357,6 +357,31 @@ struct PagedAttention {
     bool whole;         // counted in items instead: every range is an item, or none
   };
   static __device__ __forceinline__ int steps_of(const int* qs, const int* cl, int b) { return b < SEQS ? HKV * head_steps(sequence(qs, cl, b)) : 0; }
+  // Where there are no more items than ranges, an item may be a range, uncut: as long as the longest takes no more steps
+  // than an equal share and what the parts would cost.  In steps, that is two for the barrier and the join, and one for
+  // 256 blocks of 32 rows in parts, written and read (a wide block of 128 elements is 17 KB).
+  //   32 / 8 heads of 128 elements in bf16, us uncut and cut: one prompt of 256 tokens 16.7 and 21.3, of 1024 36 and 47, of
+  //   2048 63 and 100; 32 tokens each behind two caches of 1200 keys 33 and 19 (cut, by the rule)
+  //   12 heads of 64 elements, single tokens of 4 sequences of 210 .. 505 keys: 8.5 and 8.9
+  struct Uncut {   // what a sequence adds to the decision
+    int items, steps, longest, blocks;
+  };
+  static __device__ __forceinline__ Uncut uncut(const Sequence& s, int tiles) {
+    Uncut u = {HKV * tiles, 0, 0, 0};
+    if (tiles > 0) {
+      int first, shortest;
+      tile_steps(s, 0, first, shortest);
+      tile_steps(s, tiles - 1, first, u.longest);
+      shortest = shortest < 1 << 18 ? shortest : 1 << 18, u.longest = u.longest < 1 << 18 ? u.longest : 1 << 18;   // sums stay below 2^31
+      u.steps = (int)((unsigned)(HKV * tiles) * (unsigned)(shortest + u.longest) / 2);   // taken where there are at most GRID items
+      u.blocks = is_narrow(s.len) ? 0 : clamp_int((s.len * G + 31) / 32, 0, NW);
+    }
+    return u;
+  }
+  static __device__ __forceinline__ bool cuts_cost_more(const Uncut& all) {
+    const int parts = all.steps < GRID + all.items ? all.steps : GRID + all.items;
+    return all.longest <= all.steps / GRID + 2 + parts * all.blocks / 256;
+  }
 #ifndef MONONN_ONE_THREAD
   // Sums and maxima over the lanes of the first 64 sequences: moves inside rows of 16 lanes on the vector unit, then the
   // rows' results through scalar registers.  (Six exchanges through the LDS take half a microsecond, which a call of single
@@ -390,28 +415,16 @@ struct PagedAttention {
     for (int row = 1; row < kRows; ++row) r = op(r, __builtin_amdgcn_readlane(v, row * 16));
     return r;
   }
-  // Where there are no more items than ranges, an item may be a range, uncut: as long as the longest takes no more steps
-  // than an equal share and what the parts would cost.  In steps, that is two for the barrier and the join, and one for
-  // 256 blocks of 32 rows in parts, written and read (a wide block of 128 elements is 17 KB).
-  //   32 / 8 heads of 128 elements in bf16, us uncut and cut: one prompt of 256 tokens 16.7 and 21.3, of 1024 36 and 47, of
-  //   2048 63 and 100; 32 tokens each behind two caches of 1200 keys 33 and 19 (cut, by the rule)
-  //   12 heads of 64 elements, single tokens of 4 sequences of 210 .. 505 keys: 8.5 and 8.9
   static __device__ __forceinline__ bool fewer_without_cuts(const Sequence& s, int tiles) {
-    int first, shortest = 0, longest = 0;
-    if (tiles > 0) {
-      tile_steps(s, 0, first, shortest);
-      tile_steps(s, tiles - 1, first, longest);
-      shortest = shortest < 1 << 18 ? shortest : 1 << 18, longest = longest < 1 << 18 ? longest : 1 << 18;   // sums stay below 2^31
-    }
-    if constexpr (kAllNarrow) return SEQS * HKV <= GRID && __all(longest <= 2);
+    Uncut u = uncut(s, tiles);
+    if constexpr (kAllNarrow) return SEQS * HKV <= GRID && __all(u.longest <= 2);
     const auto sum = [](int a, int b) { return a + b; };
     const auto larger = [](int a, int b) { return a > b ? a : b; };
-    const int items = over_sequences(HKV * tiles, sum);
-    if (items > GRID) return false;
-    const int steps = over_sequences(HKV * tiles * (shortest + longest) / 2, sum), most = over_sequences(longest, larger);
-    const int blocks = over_sequences(tiles == 0 || is_narrow(s.len) ? 0 : clamp_int((s.len * G + 31) / 32, 0, NW), larger);
-    const int parts = steps < GRID + items ? steps : GRID + items;
-    return most <= steps / GRID + 2 + parts * blocks / 256;
+    u.items = over_sequences(u.items, sum);
+    if (u.items > GRID) return false;
+    u.steps = over_sequences(u.steps, sum), u.longest = over_sequences(u.longest, larger);
+    u.blocks = over_sequences(u.blocks, larger);
+    return cuts_cost_more(u);
   }
   static __device__ __forceinline__ Plan plan(const int* qs, const int* cl) {
     Plan p;
@@ -448,15 +461,28 @@ struct PagedAttention {
   }
 #else   // for a host build that runs one thread at a time
   static __device__ __forceinline__ Sequence planned(const Plan&, const int* qs, const int* cl, int b) { return sequence(qs, cl, b); }
+  static __device__ __forceinline__ bool fewer_without_cuts(const int* qs, const int* cl) {
+    Uncut all = {0, 0, 0, 0};
+    for (int b = 0; b < SEQS; ++b) {
+      const Sequence s = sequence(qs, cl, b);
+      const Uncut u = uncut(s, tiles_of(s.len));
+      all.items += u.items;
+      if (all.items > GRID || (kAllNarrow && u.longest > 2)) return false;
+      all.steps += u.steps;
+      all.longest = u.longest > all.longest ? u.longest : all.longest, all.blocks = u.blocks > all.blocks ? u.blocks : all.blocks;
+    }
+    return kAllNarrow ? SEQS * HKV <= GRID : cuts_cost_more(all);
+  }
+  static __device__ __forceinline__ int counted(const Plan& p, const int* qs, const int* cl, int b) { return p.whole ? HKV * tiles_of(sequence(qs, cl, b).len) : steps_of(qs, cl, b); }
   static __device__ __forceinline__ Plan plan(const int* qs, const int* cl) {
-    Plan p = {0, 0, 0, {0, 0, 0}, false};
-    for (int b = 0; b < SEQS; ++b) p.total += steps_of(qs, cl, b);
+    Plan p = {0, 0, 0, {0, 0, 0}, SEQS <= kWaveSize && fewer_without_cuts(qs, cl)};
+    for (int b = 0; b < SEQS; ++b) p.total += counted(p, qs, cl, b);
     return p;
   }
-  static __device__ __forceinline__ int sequence_with_step(const Plan&, const int* qs, const int* cl, int& rem) {
+  static __device__ __forceinline__ int sequence_with_step(const Plan& p, const int* qs, const int* cl, int& rem) {
     for (int b = 0; b < SEQS; ++b) {
-      if (rem < steps_of(qs, cl, b)) return b;
-      rem -= steps_of(qs, cl, b);
+      if (rem < counted(p, qs, cl, b)) return b;
+      rem -= counted(p, qs, cl, b);
     }
     return SEQS - 1;
   }

@@ -453,6 +453,28 @@ def test_bounds_attention(monkeypatch, tmp_path, T, H, HKV, D, B, W, page, windo
     assert check(monkeypatch, tmp_path, text, {3: any_pages(rng, B, W, 30), 4: qs, 5: cl}, grid=8, block=block) == (True, "ok")
 
 
+@pytest.mark.parametrize("T, H, HKV, D, B, W, page, window, block, qs, cl, whole", [
+    (4, 4, 2, 64, 4, 8, 16, 0, 256, [0, 1, 2, 3, 4], [1, 128, 77, 0], True),          # single tokens
+    (4, 4, 2, 64, 4, 32, 16, 0, 256, [0, 1, 2, 3, 4], [1, 500, 77, 0], False),        # one of them long
+    (70, 8, 2, 80, 3, 20, 8, 0, 256, [0, 70, 70, 70], [70, 99, 12], True),            # one prompt
+    (70, 8, 2, 80, 3, 20, 8, 30, 512, [0, 3, 3, 70], [100, 99, 90], True),            # a few tokens and a prompt, with a window
+    (70, 8, 2, 80, 3, 20, 8, 0, 256, [2, 3, 60, 1000], [1 << 30, -3, 12], True),      # lengths that are cut to the table and the tokens
+    (70, 8, 2, 80, 3, 90, 8, 0, 256, [0, 3, 60, 70], [700, 99, 12], False),           # a cache that one range would work on for long
+    (40, 4, 4, 256, 2, 20, 8, 0, 256, [0, 39, 40], [60, 30], True),
+])
+def test_bounds_attention_of_uncut_items(monkeypatch, tmp_path, T, H, HKV, D, B, W, page, window, block, qs, cl, whole):
+    # items that are not cut leave no parts: without memory for them the run still ends well, and only then
+    rng = np.random.default_rng(8)
+    text, _ = dc.attention_module(T, H, HKV, D, 30, page, B, W, "f16", 0.1, window)
+    spec = json.loads(MonoNNModule.compile(text, build=False).get_tuning_spec())
+    launch = spec["cuda_context"]["cuda_runtime_context"]
+    launch["grid_dim"]["x"], launch["block_dim"]["x"] = 8, block
+    parts = MonoNNModule.compile(text, json.dumps(spec), build=False).buffer_info()["temp"]
+    data = {3: any_pages(rng, B, W, 30), 4: qs, 5: cl}
+    ok, message = check(monkeypatch, tmp_path, text, data, grid=8, block=block, shrink=("temp arena", parts))
+    assert ok == whole and (ok or "temp arena" in message), message
+
+
 @pytest.mark.parametrize("M, N, K, group, dtype, zeros", [(1, 100, 96, 32, "f16", False), (19, 33, 640, 32, "bf16", True), (70, 33, 256, 128, "f16", True), (3, 16, 64, 64, "bf16", False), (1, 1, 1280, 256, "f16", True),
                                                          (16, 40, 4096, 64, "f16", True), (70, 33, 1056, 32, "bf16", False)])   # x in slices
 def test_bounds_w4(monkeypatch, tmp_path, M, N, K, group, dtype, zeros):
