@@ -15,13 +15,15 @@ using hlo::OperatorConfig;
 
 namespace {
 
-std::string float_literal(double v) {
+std::string literal(double v, const char* format) {
   char buf[64];
-  std::snprintf(buf, sizeof buf, "%.9g", v);
+  std::snprintf(buf, sizeof buf, format, v);
   std::string s = buf;
   if (s.find_first_of(".en") == std::string::npos) s += ".0";
-  return s + "f";
+  return s;
 }
+std::string float_literal(double v) { return literal(v, "%.9g") + "f"; }
+std::string double_literal(double v) { return literal(v, "%.17g"); }
 
 // elements of one access: the largest power of two up to 16 bytes that divides all of `extents`
 int run_length(hlo::DType t, std::initializer_list<int64_t> extents) {
@@ -137,7 +139,7 @@ NodeFunction generate_operator(const graph::Program& prog, const graph::Node& no
       const int heads = heads_per_thread(T, H, pieces, cus * block);
       const std::string x = input(0), pos = input(1), freq = input(2), out = ptrs.output(ins);
       body << "mononn_dev::rope_unit<" << ctype(0) << ", " << T << ", " << H << ", " << D << ", " << R << ", " << flag(c.interleaved) << ", " << vec << ", " << heads << ", "
-           << flag(read_in_kernel(prog, ins)) << ">(unit, " << x << ", " << pos << ", " << freq << ", " << out << ", " << float_literal(c.amplitude) << ");";
+           << flag(read_in_kernel(prog, ins)) << ">(unit, " << x << ", " << pos << ", " << freq << ", " << out << ", " << double_literal(c.amplitude) << ");";
       check_units((T * pieces * ((H + heads - 1) / heads) + block - 1) / block);
       break;
     }
@@ -155,7 +157,7 @@ NodeFunction generate_operator(const graph::Program& prog, const graph::Node& no
       const std::string table = input(4), qs = input(5), cl = input(6), freq = R > 0 ? input(7) : "nullptr";
       body << "mononn_dev::kv_append_unit<" << ctype(0) << ", " << T << ", " << dims(4)[0] << ", " << H << ", " << D << ", " << R << ", " << flag(c.interleaved) << ", " << vec << ", " << heads
            << ", " << dims(2)[1] << ", " << dims(2)[0] << ", " << dims(4)[1] << ", " << flag(coherent) << ">(unit, " << k << ", " << v << ", " << kc << ", " << vc << ", " << table << ", " << qs
-           << ", " << cl << ", " << freq << ", " << float_literal(c.amplitude) << ");";
+           << ", " << cl << ", " << freq << ", " << double_literal(c.amplitude) << ");";
       check_units((T * pieces * ((H + heads - 1) / heads) + block - 1) / block);
       break;
     }

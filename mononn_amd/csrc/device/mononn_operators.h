@@ -56,14 +56,18 @@ __device__ __forceinline__ int clamp_int(int v, int lo, int hi) { return v < lo 
 // rotary positions
 // ---------------------------------------------------------------------------------------------
 // Pair i of a head turns by position * inv_freq[i].  The angle is reduced to a fraction of a turn in 64 bits: at
-// position 10^6 a 32-bit angle is off by 0.03 rad.
-__device__ __forceinline__ void rotation_of(int position, float inv_freq, float amplitude, float& c, float& s) {
-  double turns = (double)position * (double)inv_freq * 0.15915494309189533577;
-  turns -= __builtin_rint(turns);
+// position 10^6 a 32-bit angle is off by 0.03 rad.  The functions themselves take 32 bits of it; what those leave, up to
+// 9e-8 rad, turns their results further (to first order: its square is 10^-14), and the amplitude goes on before the one
+// rounding to f32.
+__device__ __forceinline__ void rotation_of(int position, float inv_freq, double amplitude, float& c, float& s) {
+  double half_turns = (double)position * (double)inv_freq * 0.31830988618379067154;
+  half_turns -= 2.0 * __builtin_rint(0.5 * half_turns);
+  const float near = (float)half_turns;
+  const double rest = (half_turns - (double)near) * 3.14159265358979323846;
   float sn, cs;
-  sincospif(2.0f * (float)turns, &sn, &cs);
-  c = cs * amplitude;
-  s = sn * amplitude;
+  sincospif(near, &sn, &cs);
+  c = (float)(((double)cs - (double)sn * rest) * amplitude);
+  s = (float)(((double)sn + (double)cs * rest) * amplitude);
 }
 
 // A head of D elements, the first R of them rotated, cut into pieces a thread handles: VEC pairs (two runs of VEC
@@ -77,7 +81,7 @@ struct RotaryHead {
   float c[VEC], s[VEC];
   int first, second;   // element offsets of the piece's runs; second < 0: a copied piece
 
-  __device__ __forceinline__ RotaryHead(int piece, int position, const float* inv_freq, float amplitude) {
+  __device__ __forceinline__ RotaryHead(int piece, int position, const float* inv_freq, double amplitude) {
     if (piece < kTurned) {
       first = INTERLEAVED ? 2 * piece * VEC : piece * VEC;
       second = INTERLEAVED ? first + VEC : first + R / 2;
@@ -127,7 +131,7 @@ struct RotaryHead {
 // us where eight take 21).  8192 tokens of 32 heads of 128 in bf16: 21.3 us (134 MB, 6.3 TB/s while the input is in the
 // last-level cache, 5.4 TB/s from memory); a single token: 2.5 us, the launch.
 template <class T, int TOKENS, int H, int D, int R, bool INTERLEAVED, int VEC, int HEADS, bool COHERENT>
-__device__ __forceinline__ void rope_unit(int unit, const T* x, const int* positions, const float* inv_freq, T* y, float amplitude) {
+__device__ __forceinline__ void rope_unit(int unit, const T* x, const int* positions, const float* inv_freq, T* y, double amplitude) {
   using Head = RotaryHead<T, D, R, INTERLEAVED, VEC>;
   constexpr int STRIDE = (H + HEADS - 1) / HEADS;   // neighbouring threads take neighbouring heads
   const long item = (long)unit * MONONN_BLOCK_SIZE + thread_id();
@@ -184,7 +188,7 @@ __device__ __forceinline__ int sequence_of(const int* query_start, int t) {
 // us, a chain of small loads (the token's sequence, its lengths, its page) behind the launch.
 template <class T, int TOKENS, int SEQS, int H, int D, int R, bool INTERLEAVED, int VEC, int HEADS, int PAGE, int PAGES, int WIDTH, bool COHERENT>
 __device__ __forceinline__ void kv_append_unit(int unit, const T* k, const T* v, T* k_cache, T* v_cache, const int* page_table, const int* query_start, const int* context_len,
-                                               const float* inv_freq, float amplitude) {
+                                               const float* inv_freq, double amplitude) {
   using Head = RotaryHead<T, D, R, INTERLEAVED, VEC>;
   constexpr int STRIDE = (H + HEADS - 1) / HEADS;
   const long item = (long)unit * MONONN_BLOCK_SIZE + thread_id();

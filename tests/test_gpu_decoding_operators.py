@@ -63,6 +63,27 @@ def test_rope_negative_positions_turn_back(gpu_device):
     assert np.abs(back - x).max() < 1e-5
 
 
+@pytest.mark.parametrize("amplitude", [1.0, 1.2079441541679836])
+def test_rotation_next_to_half_a_turn(gpu_device, amplitude):
+    # sines of angles within 0.01 of pi: their 32-bit angle is off by up to 9e-8, their value by four units of its last place
+    # at most when what that leaves is taken into account (two of the function, one each of the further turn and the rounding).
+    # The reduction itself is in 64 bits: 1 / pi and its product with the angle are rounded by 2^-53 each, which is 2^-52 of
+    # the angle before its whole turns are taken off (1.7e-10 of 7.4e5 rad).
+    f = np.array([0.7071, 0.0123], np.float32)
+    turns = np.arange(1, 1 << 20)[:, None] * f.astype(np.float64) / (2 * np.pi) % 1.0
+    pos = np.concatenate([np.nonzero(np.abs(turns[:, i] - 0.5) < 1.5e-3)[0][-200:] + 1 for i in range(2)]).astype(np.int32)
+    near = np.abs(turns[pos - 1] - 0.5) < 1.5e-3
+    assert near.sum(0).min() >= 200
+    text, outs = dc.rope_module(len(pos), 1, 4, 4, "f32", False, amplitude)
+    x = np.zeros((len(pos), 1, 4), np.float32)
+    x[..., :2] = 1.0
+    (got,) = run(text, outs, [x, pos, f])
+    want = decoding.rope(x, pos, f, False, amplitude)
+    sines, exact = got[:, 0, 2:].astype(np.float64)[near], want[:, 0, 2:][near]
+    angle = (pos.astype(np.float64)[:, None] * f)[near]
+    within(sines, exact, 4 * 2.0 ** -23 * np.abs(exact) + amplitude * 2.0 ** -52 * angle + 1e-13)
+
+
 # ---- append -----------------------------------------------------------------------------------------------------------
 APPEND = [
     dict(new=[1] * 5, ctx=[1, 2, 16, 17, 300], H=8, D=128, page=16, R=128, dtype="f16"),
