@@ -1311,15 +1311,16 @@ template <class T>
 struct Nibbles;
 template <>
 struct Nibbles<half_t> {
-  static constexpr int kBias = 8;   // subtracted on the way
+  static constexpr bool kExact = true;   // operands are value - zero
   // (w >> s) & 15 in f16 by setting exponent bits: 1024 + v where the four bits are the last of the mantissa, 64 + v where
-  // they stand four places higher; elements 0, 4, 1, 5, 2, 6, 3, 7 of the dword
-  static __device__ __forceinline__ half8_t operands(unsigned w) {
+  // they stand four places higher; elements 0, 4, 1, 5, 2, 6, 3, 7 of the dword.  Less 1024 or 64 and the zero point (any
+  // byte): all are whole numbers that f16 holds.
+  static __device__ __forceinline__ half8_t operands(unsigned w, unsigned zero) {
     half8_t r;
     unsigned low = 0x64006400u, high = 0x54005400u;   // in vector registers: one instruction then masks and sets (two constants would need two)
     MONONN_KEEP_IN_VGPR(low);
     MONONN_KEEP_IN_VGPR(high);
-    const half2_t l8 = {(half_t)1032.0f, (half_t)1032.0f}, h8 = {(half_t)72.0f, (half_t)72.0f};
+    const half2_t l8 = __builtin_bit_cast(half2_t, zero * 0x00010001u + 0x64006400u), h8 = l8 - half2_t{(half_t)960.0f, (half_t)960.0f};
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const unsigned x = i ? w >> 8 : w;
@@ -1331,8 +1332,11 @@ struct Nibbles<half_t> {
 };
 template <>
 struct Nibbles<__bf16> {
-  static constexpr int kBias = -128;   // 128 + v: there is no packed bf16 subtraction, the sum of x takes it out again
-  static __device__ __forceinline__ half8_t operands(unsigned w) {
+  // 128 + v: there is no packed bf16 subtraction, a sum of x takes 128 and the zero point out again.  That leaves the result
+  // off by what 128 + zero times the sum of |x| loses in f32, and x that is not finite without a result (infinity less infinity).
+  static constexpr bool kExact = false;
+  static constexpr int kBias = 128;
+  static __device__ __forceinline__ half8_t operands(unsigned w, unsigned) {
     struct { unsigned d[4]; } r;
     unsigned bits = 0x43004300u;
     MONONN_KEEP_IN_VGPR(bits);
@@ -1382,7 +1386,7 @@ struct MatvecW4 {
   static constexpr int AHEAD = 8 / P;
   static constexpr int DEPTH = MINE < AHEAD ? MINE : AHEAD;   // blocks in flight
   static constexpr bool kBf16 = IsBf16<T>::value;
-  static constexpr bool kSums = ZEROS || Nibbles<T>::kBias != 8;
+  static constexpr bool kSums = !Nibbles<T>::kExact;
   static constexpr int ROWS = M < 4 ? M : 4;                  // result rows a lane looks at
   static constexpr int kShareBytes = WK > 1 ? NW * MT * 1024 : 0;
   static constexpr int kPieces = PER_GROUP * BLOCK / 8;       // x in LDS: [piece of 8 columns][row][8], elements in the operands' order
@@ -1398,6 +1402,12 @@ struct MatvecW4 {
     Scales scale;
     Zeros zero;
   };
+  // of a lane's scales, which belongs to piece j and set q of its products
+  static __device__ __forceinline__ constexpr int group_of(int q, int j) { return kSwap ? (q * 32 * P + 32 * j) / GROUP : (kSpread ? 32 * j / GROUP : 0); }
+  static __device__ __forceinline__ unsigned zero_of(const Weights& c, int q, int j) {
+    if constexpr (ZEROS) return c.zero.v[group_of(q, j)];
+    else return 8;
+  }
   // what a lane needs of `E`[N, GROUPS] for a block
   template <class V, class E>
   static __device__ __forceinline__ V load_groups(const E* p, long row, int block) {
@@ -1519,7 +1529,7 @@ struct MatvecW4 {
           const bool fresh = j == 0 || (32 * j) % GROUP == 0, done = (32 * (j + 1)) % GROUP == 0 || j + 1 == P;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const half8_t b = Nibbles<T>::operands(w[k]);
+            const half8_t b = Nibbles<T>::operands(w[k], zero_of(c, kSwap ? k : 0, j));
             constexpr float4_t kZero = {0.0f, 0.0f, 0.0f, 0.0f};
             const int set = kSwap ? k : 0;
             const bool start = fresh && (kSwap || k == 0);
@@ -1535,14 +1545,12 @@ struct MatvecW4 {
           if (done) {
 #pragma unroll
             for (int q = 0; q < SETS; ++q) {
-              const int at = kSwap ? (q * 32 * P + 32 * j) / GROUP : (kSpread ? 32 * j / GROUP : 0);
-              const float s = (float)c.scale.v[at];
-              const float z = ZEROS ? (float)((int)c.zero.v[at] - Nibbles<T>::kBias) : (float)(8 - Nibbles<T>::kBias);
+              const float s = (float)c.scale.v[group_of(q, j)];
 #pragma unroll
               for (int t = 0; t < MT; ++t)
 #pragma unroll
                 for (int e = 0; e < ROWS; ++e) {
-                  if constexpr (kSums) acc[t][e] += s * (dot[t][q][e] - z * sum[t][q][e]);
+                  if constexpr (kSums) acc[t][e] += s * (dot[t][q][e] - (float)(zero_of(c, q, j) + Nibbles<T>::kBias) * sum[t][q][e]);
                   else acc[t][e] += s * dot[t][q][e];
                 }
             }

@@ -419,7 +419,8 @@ class Computation:
     def matvec_w4(self, x: Value, weight: Value, scales: Value, zeros: Optional[Value] = None) -> Value:
         """`mononn$matvec_w4`: x [rows, k] (f16 or bf16) times the transpose of a matrix in 4 bits: weight u8[n, k / 2], two
         values to a byte, the low half first; scales [n, groups] of x's type and zeros u8[n, groups] (8 without it), one
-        of each for k / groups consecutive columns: w[n, k] = (value - zero) * scale."""
+        of each for k / groups consecutive columns: w[n, k] = (value - zero) * scale.  In bf16 the entries of x must be finite
+        and below 2^100 (a row that has others is not a number throughout); in f16 they may be anything."""
         return self._operator("matvec_w4", x.dtype, (x.dims[0], weight.dims[0]), [x, weight, scales] + ([zeros] if zeros is not None else []), {})
 
     def set_tuple_root(self, values: Sequence[Value]):

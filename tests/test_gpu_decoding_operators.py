@@ -371,6 +371,28 @@ def test_matvec_w4_of_wide_x(gpu_device, M, K, group, dtype, zeros, block):
     within(dc.values(got, dtype), want, dc.w4_bound(want, mags, K, group, dtype, zeros))
 
 
+@pytest.mark.parametrize("M, K, group, zeros", [(1, 256, 32, True), (3, 384, 64, True), (2, 512, 128, False), (6, 256, 32, True), (20, 384, 64, True), (9, 512, 256, True), (70, 256, 128, False)])
+def test_matvec_w4_of_infinite_x(gpu_device, M, K, group, zeros):
+    # f16: a column of a row is infinite; what the definition gives, infinity times value - zero among the rest
+    rng = np.random.default_rng(50)
+    N = 37
+    text, outs = dc.w4_module(M, N, K, group, "f16", zeros)
+    x, w = rng.normal(size=(M, K)).astype(np.float16), rng.integers(0, 256, (N, K // 2), dtype=np.uint8)
+    x[M // 2, rng.integers(K)] = -np.inf
+    s = rng.uniform(-0.02, 0.02, (N, K // group)).astype(np.float16)
+    z = rng.integers(0, 256, (N, K // group), dtype=np.uint8) if zeros else None
+    with np.errstate(invalid="ignore"):
+        want = decoding.matvec_w4(x, w, s, z)
+    (got,) = run(text, outs, [x, w, s] + ([z] if zeros else []))
+    assert np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(np.isposinf(got), np.isposinf(want)) and np.array_equal(np.isneginf(got), np.isneginf(want))
+    assert np.isinf(got).sum() >= N // 2 and np.isfinite(got).sum() == (M - 1) * N
+    finite = np.isfinite(want).all(1)
+    mags = {}
+    want = decoding.matvec_w4(x[finite], w, s, z, mags)
+    if finite.any():
+        within(got[finite].astype(np.float64), want, dc.w4_bound(want, mags, K, group, "f16", zeros))
+
+
 def test_matvec_w4_values_one_by_one(gpu_device):
     # unit rows of x pick single columns: every nibble value at every place of a byte, exactly
     K, N = 128, 16
