@@ -611,6 +611,35 @@ def test_a_cache_that_is_not_returned_is_guarded_too(gpu_device, returned):
     assert kc.sum() == vc.sum() == 5 * 128 and kc[1, 2].all() and vc[4, :3].all()
 
 
+@pytest.mark.parametrize("returned", [["out"], ["out", "kc", "vc"]])
+def test_autograd_notices_updated_inputs(gpu_device, returned):
+    import torch
+    from test_decoding_operators import append_and_attend
+    fn = _function(*append_and_attend(returned), checked=True)
+    k = torch.ones((5, 2, 64), dtype=torch.float16, device="cuda")
+    kc, vc = (torch.zeros((9, 16, 2, 64), dtype=torch.float16, device="cuda") for _ in range(2))
+    meta = [torch.tensor(a, dtype=torch.int32, device="cuda") for a in ([[0, 1, 2, 3], [4, 5, 6, 7]], [0, 2, 5], [20, 3])]
+    q = torch.ones((5, 4, 64), dtype=torch.float16, device="cuda")
+    leaf = torch.ones((), dtype=torch.float16, device="cuda", requires_grad=True)
+    product = (leaf * kc).sum()   # saves kc for its backward pass
+    before = [t._version for t in (k, kc, vc, q)]
+    fn(k, k, kc, vc, *meta, q)
+    assert [t._version for t in (k, kc, vc, q)] == [before[0], before[1] + 1, before[2] + 1, before[3]]
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        product.backward()
+    grows = torch.zeros_like(vc, requires_grad=True)
+    with pytest.raises(AssertionError, match="gradient"):
+        fn(k, k, kc, grows, *meta, q)
+    torch.cuda.synchronize()
+    assert not grows.any() and kc._version == before[1] + 1
+    with torch.no_grad():
+        fn(k, k, kc, grows, *meta, q)
+    with torch.inference_mode():
+        mine = [torch.zeros_like(kc) for _ in range(2)]
+        fn(k, k, *mine, *meta, q)
+        assert torch.equal(mine[0], kc) and torch.equal(mine[1], grows)
+
+
 def test_two_functions_in_two_graphs(gpu_device):
     """Parts of split sequences lie in each function's own memory: graphs of two, replayed in turn, keep their results."""
     import torch
