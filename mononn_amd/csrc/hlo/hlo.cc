@@ -7,7 +7,6 @@
 #include <cstdlib>
 #include <initializer_list>
 #include <limits>
-#include <limits>
 #include <set>
 #include <sstream>
 
@@ -460,7 +459,7 @@ void decode_operator_config(Instr* ins) {
                 "too many tokens, pages, sequences or keys of a sequence");
       supported(small({dims(1)[1], dims(1)[2], dims(1)[3]}), "a page has too many elements");
       // steps of the whole call are counted in 32 bits: 32 rows and 32 keys at least per step
-      supported((dims(0)[0] * dims(0)[1] / 32 + dims(1)[2] * (dims(3)[0] + 1)) * (dims(3)[1] * dims(1)[1] / 32 + 2) <= INT32_MAX, "too many tokens times keys");
+      supported(small({dims(0)[0] * dims(0)[1] / 32 + dims(1)[2] * (dims(3)[0] + 1), dims(3)[1] * dims(1)[1] / 32 + 2}), "too many tokens times keys");
       result(ins->shape, type(0), dims(0));
       break;
     }

@@ -283,6 +283,12 @@ def test_extents_beyond_32_bits_are_refused():
     refused(append_body(shapes, result=f"({c}, {c})"), "UNSUPPORTED", "too many tokens")
 
 
+def test_step_counts_beyond_64_bits_are_refused():
+    # 2^26 heads, 2^30 sequences (one entry of query_start more) and 8128 keys of each: 2^64 and a little in steps of 32 keys
+    shapes = ["f16[1,67108864,16]{2,1,0}"] + ["f16[9,1,67108864,16]{3,2,1,0}"] * 2 + ["s32[1073741823,8128]{1,0}", "s32[1073741824]{0}", "s32[1073741823]{0}"]
+    refused(params(*shapes) + call(shapes[0], "paged_attention", 6, '{\\"scale\\":1,\\"window\\":0}', "ROOT "), "UNSUPPORTED", "too many tokens times keys")
+
+
 def test_other_targets_stay_refused():
     refused(params("f32[4]{0}") + call("f32[4]{0}", "paged_attention_parts", 1, extra="ROOT "), "UNSUPPORTED", "is not supported")
     refused(params("f32[4]{0}") + call("f32[4]{0}", "nothing", 1, extra="ROOT "), "UNSUPPORTED", "is not supported")
