@@ -57,17 +57,19 @@ __device__ __forceinline__ int clamp_int(int v, int lo, int hi) { return v < lo 
 // ---------------------------------------------------------------------------------------------
 // Pair i of a head turns by position * inv_freq[i].  The angle is reduced to a fraction of a turn in 64 bits: at
 // position 10^6 a 32-bit angle is off by 0.03 rad.  The functions themselves take 32 bits of it; what those leave, up to
-// 9e-8 rad, turns their results further (to first order: its square is 10^-14), and the amplitude goes on before the one
-// rounding to f32.
+// 9e-8 rad, turns their results further (to first order: its square is 10^-14), and the amplitude goes on before they are
+// rounded to f32 again.
 __device__ __forceinline__ void rotation_of(int position, float inv_freq, double amplitude, float& c, float& s) {
   double half_turns = (double)position * (double)inv_freq * 0.31830988618379067154;
   half_turns -= 2.0 * __builtin_rint(0.5 * half_turns);
   const float near = (float)half_turns;
-  const double rest = (half_turns - (double)near) * 3.14159265358979323846;
+  const float rest = (float)((half_turns - (double)near) * 3.14159265358979323846);
   float sn, cs;
   sincospif(near, &sn, &cs);
-  c = (float)(((double)cs - (double)sn * rest) * amplitude);
-  s = (float)(((double)sn + (double)cs * rest) * amplitude);
+  // the amplitude in two f32 values (constants of the call): products in 64 bits would cost 10122 appended tokens 1 us of 16
+  const float a = (float)amplitude, a_rest = (float)(amplitude - (double)a), turn = rest * a;
+  c = __builtin_fmaf(cs, a, __builtin_fmaf(-sn, turn, cs * a_rest));
+  s = __builtin_fmaf(sn, a, __builtin_fmaf(cs, turn, sn * a_rest));
 }
 
 // A head of D elements, the first R of them rotated, cut into pieces a thread handles: VEC pairs (two runs of VEC
