@@ -76,9 +76,10 @@ class MonoNNFunction:
                 ptr = t.data_ptr()
             ptrs.append(ptr)
         if self._updated:
-            recording = torch.is_grad_enabled()
+            recording, mine = torch.is_grad_enabled(), []
             for i, dtype in self._updated.items():
                 t = held[i]
+                mine.append(t)
                 assert t.dtype == dtype, "an input that the call updates in place must have the declared type"
                 assert ptrs.count(ptrs[i]) == 1, "an input that the call updates in place must not be passed twice"
                 assert not (recording and t.requires_grad), "an input that the call updates in place must not require a gradient: the call records none"
@@ -98,7 +99,7 @@ class MonoNNFunction:
         stream = torch._C._cuda_getCurrentRawStream(device.index)   # what torch.cuda.current_stream(device).cuda_stream says, without the stream object
         self.module.launch_arguments(args, stream)
         if self._updated:   # as torch's own in-place operations do: a backward pass that has saved such a tensor is to notice
-            torch._C._increment_version([held[i] for i in self._updated])   # what torch.autograd.graph.increment_version calls
+            torch._C._increment_version(mine)   # what torch.autograd.graph.increment_version calls
         if self.checked:
             self.module.synchronize(stream)
         return outs
