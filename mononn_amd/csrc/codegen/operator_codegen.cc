@@ -61,7 +61,7 @@ struct MatvecPlan {
   int64_t lds_bytes(int64_t waves) const { return x_bytes() + (wk > 1 ? waves * row_blocks() * 1024 : 0); }   // and the shares of a tile's waves
   bool fits(int64_t waves) const { return x_bytes() <= hlo::kMatvecW4XBytes && lds_bytes(waves) <= 160 * 1024; }
 };
-// The plan whose busiest workgroup reads least: weights, its slice of x (16 rows of x on 4096 x 14336 weights: 13.4 us with
+// The plan whose busiest workgroup reads least: weights, its slice of x (16 rows of x on 4096 x 14336 weights: 12.9 us with
 // slices of 57 KB of x, 17 with the 115 KB that the weights alone would choose) and its share of the parts (7 rows on
 // 5185 x 10880 weights: 12.6 us with 6 slices, 20 with the 43 that would be chosen without).  Among equals larger blocks
 // (fewer loads of scales), then fewer slices, then fewer shares (fewer starts of a workgroup's loads).

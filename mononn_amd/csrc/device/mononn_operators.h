@@ -185,9 +185,10 @@ __device__ __forceinline__ int sequence_of(const int* query_start, int t) {
 // ---------------------------------------------------------------------------------------------
 // Token i of sequence b has position context_len[b] - new tokens + i and goes to row position % PAGE of page
 // page_table[b, position / PAGE]; the key is turned by its position on the way.  Positions outside the table and
-// pages outside the pool are left out.  Bound by the bytes of k and v, read once and written once, as the rotation is:
-// 10122 tokens of 9 sequences, 8 heads of 128 in bf16: 15.7 us (83 MB, 5.3 TB/s); 48 sequences of one token: 4.3
-// us, a chain of small loads (the token's sequence, its lengths, its page) behind the launch.
+// pages outside the pool are left out.  10122 tokens of 9 sequences, 8 heads of 128 in bf16: 15.8 us while k and v are in the
+// last-level cache (83 MB, 5.2 TB/s: the bytes, read once and written once, as in the rotation), 22 from memory, where their
+// loads stand behind a chain of small ones (the token's sequence, its lengths, its page); 48 sequences of one token: 4.4
+// us, that chain behind the launch.
 template <class T, int TOKENS, int SEQS, int H, int D, int R, bool INTERLEAVED, int VEC, int HEADS, int PAGE, int PAGES, int WIDTH, bool COHERENT>
 __device__ __forceinline__ void kv_append_unit(int unit, const T* k, const T* v, T* k_cache, T* v_cache, const int* page_table, const int* query_start, const int* context_len,
                                                const float* inv_freq, double amplitude) {
@@ -366,9 +367,9 @@ struct PagedAttention {
   // Where there are no more items than ranges, an item may be a range, uncut: as long as the longest takes no more steps
   // than an equal share and what the parts would cost.  In steps, that is two for the barrier and the join, and one for
   // 256 blocks of 32 rows in parts, written and read (a wide block of 128 elements is 17 KB).
-  //   32 / 8 heads of 128 elements in bf16, us uncut and cut: one prompt of 256 tokens 16.7 and 21.3, of 1024 36 and 47, of
-  //   2048 63 and 100; 32 tokens each behind two caches of 1200 keys 33 and 19 (cut, by the rule)
-  //   12 heads of 64 elements, single tokens of 4 sequences of 210 .. 505 keys: 8.5 and 8.9
+  //   32 / 8 heads of 128 elements in bf16, us uncut and cut: one prompt of 256 tokens 19 and 21, of 1024 43 and 50, of
+  //   2048 79 and 110; 32 tokens each behind two caches of 1200 keys 40 and 19 (cut, by the rule)
+  //   12 heads of 64 elements, single tokens of 4 sequences of 210 .. 505 keys: 8.7 and 9.2
   struct Uncut {   // what a sequence adds to the decision
     int items, steps, longest, blocks;
   };
@@ -647,7 +648,7 @@ struct PagedAttention {
   // Rounded to the element type, probabilities would cost a result as much as its own rounding does (its error against 64
   // bits grows by 25 to 45 %), so each goes into the second product as two values of that type: its leading bits, and what
   // they leave.  Together they hold 16 bits of it in bf16, 22 in f16.  Single tokens, bound by the reads, take the same time
-  // (1 % more at most); 6830 prompt tokens, bound by the products, take 645 us instead of 486.
+  // (2 % more at most); 6830 prompt tokens, bound by the products, take 612 us instead of 476.
   struct Probabilities {
     half8_t lead[4], rest[4];   // 16 keys each
   };
@@ -799,15 +800,15 @@ struct PagedAttention {
   static __device__ __forceinline__ float inverse(float l) { return l > 0.0f || l != l ? 1.0f / l : 0.0f; }   // a row without keys: zeros
 
   // ---- wide items ------------------------------------------------------------------------------------------------
-  // Bound by the matrix units, and by how well two waves per SIMD hide the rest behind them: of the 5200 clocks of a step they
-  // are busy for 3070 (two waves; a third of it the remainders of the probabilities), the vector units for 2600 (an
+  // Bound by the matrix units, and by how well two waves per SIMD hide the rest behind them: of the 5000 clocks of a step they
+  // are busy for 3070 (two waves; a third of it the remainders of the probabilities), the vector units for 2700 (an
   // exponential per score takes a fifth of that), the LDS reads of K and V for 2000.  One barrier per step: it ends the stores of the
   // step's tile, while the next one is on its way in registers.  So that a SIMD's two waves are not at the same part at
   // the same time, the later one runs half a step behind: it begins with the products of the last step's values, which
   // therefore stay a step longer (three buffers).  Waves at their products go first where both could issue.
-  // At 5 prompts of 6830 tokens in all on 32 / 8 heads of 128 elements in bf16: 645 us with the join, 682 TFLOP/s, 1020 with
+  // At 5 prompts of 6830 tokens in all on 32 / 8 heads of 128 elements in bf16: 612 us with the join, 720 TFLOP/s, 1080 with
   // the remainders' products, at a clock that falls to 1.9 GHz.
-  // With probabilities in one value (486 us): without the shift 3 % more, without the priority 2 %, with a barrier per half step
+  // With probabilities in one value (476 us): without the shift 3 % more, without the priority 2 %, with a barrier per half step
   // that forces the waves to take turns 6 %, with the next item's first tile and queries requested before the last one's
   // results are stored 5 %.
   static constexpr int kRuns = (kWideKeys * CPR + MONONN_BLOCK_SIZE - 1) / MONONN_BLOCK_SIZE;   // pieces of K (and of V) a thread moves per step
@@ -913,9 +914,9 @@ struct PagedAttention {
   }
 
   // ---- narrow items ----------------------------------------------------------------------------------------------
-  // Bound by the reads of keys and values: 32 sequences of 200 .. 8191 keys on 32 / 8 heads of 128 in bf16 take 120 us, 108
-  // of them at 5.0 TB/s in this stage (a large copy reaches 5.2); one of 131071 keys 104 us, 5.1 TB/s; 4 sequences of up to
-  // 512 keys on 12 heads of 64, where the chain of lengths, pages, rows counts, 8.5 us.  Every wave streams its own 32 keys of a step: requested a step ahead into
+  // Bound by the reads of keys and values: 32 sequences of 200 .. 8191 keys on 32 / 8 heads of 128 in bf16 take 121 us, 108
+  // of them at 5.0 TB/s in this stage (a large copy reaches 5.2); one of 131071 keys 106 us, 5.1 TB/s; 4 sequences of up to
+  // 512 keys on 12 heads of 64, where the chain of lengths, pages, rows counts, 8.7 us.  Every wave streams its own 32 keys of a step: requested a step ahead into
   // registers, through the wave's own LDS rows (no workgroup barrier) into the products.  The next step may belong to
   // the next item: its keys, and that item's queries, are on their way while the waves' shares of the last one are added up.
   static constexpr int kMine = CPR / 2;   // pieces of K (and of V) a lane moves per step: 32 rows over 64 lanes
@@ -1183,7 +1184,7 @@ struct PagedAttention {
   template <int N>
   struct Count { static constexpr int value = N; };
   // Adds up the parts of the items that were split: a few loads behind each other, 3 us for single
-  // tokens; 29 us behind 460 of products for 6830 prompt tokens, whose 512 parts are 68 MB, written and read (left to the
+  // tokens; 29 us behind 580 of products for 6830 prompt tokens, whose 512 parts are 68 MB, written and read (left to the
   // range in which an item begins, one workgroup for each, one sequence of 131071 keys takes 157 us instead of 104).  The workgroups whose ranges hold a part of an item share its
   // output groups among them: `rank` of `count` is this workgroup's.  With many parts the waves of a workgroup take the
   // parts of a group between them, with few every wave its own groups.
@@ -1299,8 +1300,8 @@ struct PagedAttention {
 // byte along k (the low half is the lower k), zero = 8 without a tensor of zero points.
 //
 // Bound by the reads of the weights as long as a byte of them costs few instructions: one row on 4096 x 4096 weights 3.7
-// us (a launch is 2.5), 3 rows on 14337 x 4096 in groups of 32 with zero points 10.1 us (35 MB), 16 rows on 4096 x 14336 in
-// groups of 64 13.4 us (33 MB; 9.9 in this stage: x has to arrive before the first product, the rest streams).  A wave takes 16 weight rows; lane
+// us (a launch is 2.5), 3 rows on 14337 x 4096 in groups of 32 with zero points 10.2 us (35 MB), 16 rows on 4096 x 14336 in
+// groups of 64 12.9 us (33 MB: x has to arrive before the first product, the rest streams, then a barrier and the join).  A wave takes 16 weight rows; lane
 // (r, g) = (lane % 16, lane / 16) reads row r, of every 128 P columns the 32 P that belong to its lane group g, in P
 // pieces of 16 bytes.  The products run on v_mfma_f32_16x16x32 with x as the left operand and the weights, small
 // integers and so exact, as the right one: a lane's result column is one weight row, scales are applied to f32 results.

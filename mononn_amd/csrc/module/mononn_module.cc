@@ -75,8 +75,9 @@ void MonoNNModule::generate_code() {
   }
   if (!spec_given_) {
     // Default launch: four waves per compute unit, eight when every node is an operator call.  A second wave per SIMD hides
-    // the soft-max of attention over prompts (6830 tokens, 256 -> 512 threads: 742 -> 490 us; single tokens, bound by
-    // memory, take the same); GEMM tiles want the registers of one (the 12-layer decoder step of four tokens 426 -> 453 us).
+    // the soft-max of attention over prompts (6830 tokens, 256 -> 512 threads: 909 -> 612 us; single tokens, bound by
+    // memory, take the same); GEMM tiles want the registers of one (the 12-layer decoder step of four tokens 423 -> 454 us,
+    // of two prompts of 256 tokens 1013 -> 1065).
     bool operators = false, others = false;
     for (auto& up : mod->entry->instrs) {
       const hlo::Instr& i = *up;
