@@ -665,8 +665,10 @@ struct PagedAttention {
   // The reference of a query's exponentials only has to stay near its maximum: it moves, and what has been added up
   // is rescaled, when some query of the wave has outgrown its own by 2^6, which after the first steps is rare.  In f16 it
   // is set 2^9 below the maximum: exponentials up to 2^15 are in range, and keys count that lie 2^34 below the maximum
-  // (without it those 2^25 below would vanish from the product, but not from the sum: 131071 of them are 0.4 % of it).
-  static constexpr float kOutgrown = 6.0f, kBelow = kBf16 ? 0.0f : 9.0f;
+  // (without it those 2^25 below would vanish from the product, but not from the sum: 131071 of them are 0.4 % of it).  In
+  // bf16 it is set 2^32 above: values up to the type's largest times exponentials up to 2^-26, added up over 2^25 keys, stay
+  // in the range of f32, and keys count that lie 2^94 below the maximum.
+  static constexpr float kOutgrown = 6.0f, kBelow = kBf16 ? -32.0f : 9.0f;
   static __device__ __forceinline__ float moved(float reference, float top) { return fmaxf(reference, top - kBelow); }
   static __device__ __forceinline__ bool outgrown(float reference, float top) { return __any(top - kBelow > reference + kOutgrown); }
   static __device__ __forceinline__ void score(const char* row, const Rows& r, Scores& s) {   // row: the lane's first operand

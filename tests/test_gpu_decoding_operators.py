@@ -337,6 +337,24 @@ def test_paged_attention_counts_keys_far_below_the_maximum(gpu_device, n):
     within(got.astype(np.float64), want, dc.split_attention_bound(want, mags, D, "f16"))
 
 
+@pytest.mark.parametrize("n", [1, 30])
+@pytest.mark.parametrize("dtype, largest", [("f16", 65504.0), ("bf16", float.fromhex("0x1.fep127"))])
+def test_paged_attention_of_the_largest_values(gpu_device, n, dtype, largest):
+    # their weighted sum stays below them, whatever the weights are before they are divided by their sum
+    rng = np.random.default_rng(51)
+    H, D, page, B = 2, 32, 16, 5
+    new, ctx = [n] * B, [n, n + 3, 150, 700, 2000]
+    table, qs, cl, pages = dc.paged_batch(rng, new, ctx, page)
+    text, outs = dc.attention_module(sum(new), H, H, D, pages, page, B, table.shape[1], dtype, 0.25)
+    q, kc = dc.bits(rng.normal(size=(sum(new), H, D)), dtype), dc.bits(rng.normal(size=(pages, page, H, D)), dtype)
+    vc = dc.bits(rng.choice([-0.5, 0.25, 0.5, 0.75], (pages, page, H, D)) * largest, dtype)
+    vc[..., :4] = dc.bits(np.full(1, 0.75 * largest), dtype)[0]
+    mags = {}
+    want = decoding.paged_attention(dc.values(q, dtype), dc.values(kc, dtype), dc.values(vc, dtype), table, qs, cl, 0.25, 0, mags)
+    (got,) = run(text, outs, [q, kc, vc, table, qs, cl])
+    within(dc.values(got, dtype), want, dc.split_attention_bound(want, mags, D, dtype))
+
+
 # ---- 4-bit products -----------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("block", [256, 512])
 @pytest.mark.parametrize("M, N, K, group, dtype, zeros", [
